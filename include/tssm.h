@@ -453,6 +453,39 @@ int tssm_mh_output(const void* loc_a, const void* loc_x, const void* carry, cons
                    int64_t stride_Ch, int64_t BLK, int64_t NBLK, int dtype, tssm_stream_t stream);
 
 /*
+ * Single-token gated delta rule, the state updated in place:
+ *   hd = exp(-exp(A_log) dt) h ;  e = beta (x - hd B) ;  h = hd + e B^T ;
+ *   y = scale h C.
+ *   x, y [S,H,P] io; dt, beta [S,H] f32; h [S,H,P,N] f32; A_log [H] f32;
+ *   B, C [S,G,N] io (head i uses key head i / (H/G)); N <= 256; io f32 or
+ *   bf16.  All contiguous.  No reference counterpart (the delta rule is an
+ *   addition next to tssm_streaming_step).
+ */
+int tssm_gated_delta_step(const void* x, const void* dt, void* h, const void* A_log, const void* B,
+                          const void* C, const void* beta, void* y, int64_t S, int64_t H, int64_t G,
+                          int64_t P, int64_t N, double scale, int dtype, tssm_stream_t stream);
+
+/*
+ * Group norm with an activation, channels last: x, y [Bt,L,C] (dtype f32 or
+ * bf16), mean and variance over L and the C/groups channels of a group,
+ * weight, bias [C] f32, act 0 (none) or 1 (SiLU).  mean, rstd [Bt,groups] f32
+ * receive the statistics; they may be null when L == 1 and C/groups <= 128.
+ * workspace: tssm_group_norm_workspace_size(..., backward = 0) bytes.
+ * The backward takes the statistics and returns dx, and dweight, dbias [C]
+ * f32 (summed in a fixed order); its workspace is the size for backward = 1.
+ * No reference counterpart.
+ */
+int64_t tssm_group_norm_workspace_size(int64_t Bt, int64_t L, int64_t C, int64_t groups, int dtype,
+                                       int backward);
+int tssm_group_norm_act(const void* x, const void* weight, const void* bias, void* y, void* mean,
+                        void* rstd, void* workspace, int64_t workspace_bytes, int64_t Bt, int64_t L,
+                        int64_t C, int64_t groups, double eps, int act, int dtype, tssm_stream_t stream);
+int tssm_group_norm_act_bwd(const void* dy, const void* x, const void* weight, const void* bias,
+                            const void* mean, const void* rstd, void* dx, void* dweight, void* dbias,
+                            void* workspace, int64_t workspace_bytes, int64_t Bt, int64_t L, int64_t C,
+                            int64_t groups, int act, int dtype, tssm_stream_t stream);
+
+/*
  * Synchronise `stream` and report (then clear) this device's status word:
  * TSSM_ERR_TIMEOUT if a kernel's bounded device-side wait gave up since the
  * last check, else TSSM_OK.  No reference counterpart (the reference has no

@@ -17,9 +17,12 @@ from .multihead import (ssd_scan, ssd_scan_chunked, multihead_diag, ssd_sharded_
                         ssd_slice_scan, ssd_carry_fixup)
 from .interp import (time_aware_interp, interp_neighbors_index, interp_neighbors_time,
                      interp_gather, interp_ssm_step, interp_ssm, linspace_queries)
+from .delta import gated_delta, gated_delta_grads
+from .norm import group_norm_act
 from .streaming import (streaming_ssm_inplace, streaming_step, ring_interp_then_ssm, mean_pool_logit)
 
 __all__ = [
+    "gated_delta", "gated_delta_grads", "group_norm_act",
     "zoh_discretize", "zoh_discretize_bwd", "expm1_ref", "dt_project_softplus", "zoh_discretize_dt",
     "ssm_forward", "ssm_backward", "selective_scan",
     "ssd_scan", "ssd_scan_chunked", "multihead_diag", "ssd_sharded_compose", "ssd_slice_scan",

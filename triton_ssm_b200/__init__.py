@@ -6,7 +6,12 @@ hand-written CUDA kernel through the C ABI in ``include/tssm.h``.
 from ._lib import load_library, LIB_PATH, TSSMError  # noqa: F401
 from .ops import *  # noqa: F401,F403
 from .ops import __all__ as _ops_all
+from .delta import *  # noqa: F401,F403
+from .delta import __all__ as _delta_all
+from .norm import *  # noqa: F401,F403
+from .norm import __all__ as _norm_all
 from .streaming import StreamingRing  # noqa: F401
 
-__all__ = ["load_library", "LIB_PATH", "TSSMError", "StreamingRing"] + list(_ops_all)
+__all__ = ["load_library", "LIB_PATH", "TSSMError", "StreamingRing"] + list(_ops_all) + \
+    list(_delta_all) + list(_norm_all)
 __version__ = "0.1.0"

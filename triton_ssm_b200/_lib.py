@@ -54,6 +54,10 @@ SIGNATURES = {
     "tssm_ssm_bwd_apply": ([P] * 12 + [I64] * 5 + [P], I32),
     "tssm_mh_fwd_local": ([P] * 7 + [I64] * 4 + [I64] * 9 + [I64] * 2 + [I32, P], I32),
     "tssm_mh_output": ([P] * 7 + [I64] * 4 + [I64] * 5 + [I64] * 2 + [I32, P], I32),
+    "tssm_gated_delta_step": ([P] * 8 + [I64] * 5 + [F64, I32, P], I32),
+    "tssm_group_norm_workspace_size": ([I64] * 4 + [I32, I32], I64),
+    "tssm_group_norm_act": ([P] * 7 + [I64] * 5 + [F64, I32, I32, P], I32),
+    "tssm_group_norm_act_bwd": ([P] * 10 + [I64] * 5 + [I32, I32, P], I32),
     "tssm_check_device_status": ([P], I32),
     "tssm_selftest_wait_timeout": ([I64, P], I32),
     "tssm_time_aware_interp": ([P] * 4 + [I64] * 3 + [I64] * 7 + [I64] * 2 + [I32, I32, P], I32),
@@ -101,6 +105,24 @@ def dtype_code(t):
 
 def stream_of(t):
     return ctypes.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+
+
+class _Same:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_SAME = _Same()
+
+
+def device_of(t):
+    """A context in which t's device is the current one (launches and the
+    device's status word follow the current device)."""
+    i = t.device.index
+    return _SAME if i is None or i == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
 def ptr(t):

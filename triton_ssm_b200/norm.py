@@ -1,0 +1,93 @@
+"""Group norm with an activation, channels last (forward and backward).
+
+It normalises the channels-last outputs of the scans: per token and head
+(a [rows, C] tensor, ``groups`` = heads), or over a whole feature map
+([Bt, L, C]).  Same conventions as ``ops.py``: bad arguments raise
+``ValueError``, outputs are new tensors, the kernel runs on the current stream
+of the inputs' device.
+"""
+import torch
+
+from . import _lib
+from ._lib import call, device_of, dtype_code, ptr, stream_of
+from .ops import _cuda, _need
+
+__all__ = ["group_norm_act", "group_norm_act_bwd"]
+
+_ACT = {"none": 0, "silu": 1}
+
+
+def _norm_args(name, x, weight, bias, groups, act):
+    _need(x, (torch.float32, torch.bfloat16), "x")
+    _need(weight, (torch.float32,), "weight")
+    _need(bias, (torch.float32,), "bias")
+    if x.dim() not in (2, 3):
+        raise ValueError("%s: expected x [Bt,L,C] or [rows,C]" % name)
+    C = x.shape[-1]
+    if tuple(weight.shape) != (C,) or tuple(bias.shape) != (C,):
+        raise ValueError("%s: weight and bias must be [C]" % name)
+    if groups < 1 or C % groups:
+        raise ValueError("%s: C (%d) must be a multiple of groups (%d)" % (name, C, groups))
+    if act not in _ACT:
+        raise ValueError("%s: act must be 'silu' or 'none' (got %r)" % (name, act))
+    return x.shape[0], (x.shape[1] if x.dim() == 3 else 1), C
+
+
+def _workspace(x, Bt, L, C, groups, backward):
+    need = int(_lib.load_library().tssm_group_norm_workspace_size(Bt, L, C, groups, dtype_code(x), int(backward)))
+    return torch.empty(need, dtype=torch.uint8, device=x.device) if need else None, need
+
+
+def group_norm_act(x, weight, bias, groups, eps=1e-5, act="silu", return_stats=False, y=None):
+    """Group norm over channels-last x, then the activation:
+    y = act((x - mean) / sqrt(var + eps) * weight + bias).
+
+    x [Bt,L,C] (mean and variance per batch row and group, over L and the
+    C/groups channels) or [rows,C] (per row and group, the head norm of single
+    tokens); f32 or bf16.  weight, bias [C] f32; act "silu" or "none".
+    Returns y in x's dtype, or (y, mean, rstd) with the statistics
+    [Bt,groups] f32 when ``return_stats`` (the backward takes them).
+    """
+    _cuda(x, weight, bias, y)
+    groups = int(groups)
+    Bt, L, C = _norm_args("group_norm_act", x, weight, bias, groups, act)
+    x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
+    if y is None:
+        y = torch.empty_like(x)
+    elif y.shape != x.shape or y.dtype != x.dtype or not y.is_contiguous():
+        raise ValueError("group_norm_act: y must be contiguous and match x")
+    mean = rstd = None
+    if return_stats or L != 1 or C // groups > 128:
+        mean, rstd = torch.empty(2, Bt, groups, device=x.device, dtype=torch.float32)
+        if L == 0:
+            mean.zero_()
+            rstd.fill_(float(eps) ** -0.5)
+    ws, need = _workspace(x, Bt, L, C, groups, False)
+    with device_of(x):
+        call("tssm_group_norm_act", ptr(x), ptr(weight), ptr(bias), ptr(y), ptr(mean), ptr(rstd), ptr(ws), need, Bt, L,
+             C, groups, float(eps), _ACT[act], dtype_code(x), stream_of(x))
+    return (y, mean, rstd) if return_stats else y
+
+
+def group_norm_act_bwd(dy, x, weight, bias, mean, rstd, act="silu"):
+    """Backward of ``group_norm_act``.
+
+    dy, x [Bt,L,C] or [rows,C] (one dtype); weight, bias [C] f32; mean, rstd
+    [Bt,groups] f32 from the forward.  Returns (dx in x's dtype, dweight [C],
+    dbias [C] f32); the sums over rows run in a fixed order.
+    """
+    _cuda(dy, x, weight, bias, mean, rstd)
+    if mean.dim() != 2 or mean.shape != rstd.shape or mean.dtype != torch.float32 or rstd.dtype != torch.float32:
+        raise ValueError("group_norm_act_bwd: mean and rstd must be [Bt,groups] f32")
+    groups = mean.shape[1]
+    Bt, L, C = _norm_args("group_norm_act_bwd", x, weight, bias, groups, act)
+    if dy.shape != x.shape or dy.dtype != x.dtype or mean.shape[0] != Bt:
+        raise ValueError("group_norm_act_bwd: dy must match x, and mean and rstd its batch rows")
+    dy, x, weight, bias, mean, rstd = (t.contiguous() for t in (dy, x, weight, bias, mean, rstd))
+    dx = torch.empty_like(x)
+    dw, db = torch.empty(2, C, device=x.device, dtype=torch.float32)
+    ws, need = _workspace(x, Bt, L, C, groups, True)
+    with device_of(x):
+        call("tssm_group_norm_act_bwd", ptr(dy), ptr(x), ptr(weight), ptr(bias), ptr(mean), ptr(rstd), ptr(dx),
+             ptr(dw), ptr(db), ptr(ws), need, Bt, L, C, groups, _ACT[act], dtype_code(x), stream_of(x))
+    return dx, dw, db
