@@ -466,6 +466,19 @@ int tssm_gated_delta_step(const void* x, const void* dt, void* h, const void* A_
                           int64_t P, int64_t N, double scale, int dtype, tssm_stream_t stream);
 
 /*
+ * Gated delta rule over whole sequences (chunked; tssm_gated_delta_step for a
+ * single token).  u, y [Bt,L,H,P] and B, C [Bt,L,G,N] io (f32 or bf16); dt,
+ * beta [Bt,L,H] f32; A_log [H] f32; h0, h_last [Bt,H,P,N] f32 (either may be
+ * null); N <= 128; all contiguous.  states [Bt,H,ceil(L/64),P,N] f32 (the
+ * state before every 64-token chunk) and errors [Bt,L,H,P] f32 (u - hd B) are
+ * what the backward reads; both null when none follows.
+ */
+int tssm_gated_delta_rule(const void* u, const void* A_log, const void* B, const void* C, const void* dt,
+                          const void* beta, const void* h0, void* y, void* h_last, void* states,
+                          void* errors, int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N,
+                          double scale, int dtype, tssm_stream_t stream);
+
+/*
  * Group norm with an activation, channels last: x, y [Bt,L,C] (dtype f32 or
  * bf16), mean and variance over L and the C/groups channels of a group,
  * weight, bias [C] f32, act 0 (none) or 1 (SiLU).  mean, rstd [Bt,groups] f32

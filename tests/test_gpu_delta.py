@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from oracle.delta import gated_delta, gated_delta_grads
+from oracle.delta import gated_delta
 
 dev = "cuda"
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
@@ -89,3 +89,160 @@ def test_step_refusals_without_gpu():
     for kw in (dict(S=-1), dict(G=3), dict(G=0), dict(N=0), dict(N=257), dict(dtype=2), dict(x=0), dict(S=1 << 40)):
         assert step(**kw) == 1, kw
     assert step(S=0) == 0
+
+
+# ------------------------------------------------------------------ whole sequences
+def off(out, ref):
+    """2-norm of the difference over the 2-norm of the result."""
+    return ((out.double().cpu() - ref).norm() / ref.norm().clamp_min(1e-300)).item()
+
+
+# Relative 2-norm tolerances.  A bf16 result: its own rounding is uniform within half a step of
+# 2^-9 to 2^-8 of the value, 2-norm 2^-8 / sqrt(3) at most, and y has two planes (2^-16) of slack:
+# 2^-8.  An f32 result goes through at most L / 64 + 1 chunks, each a chain of five products of
+# f32-exact operands whose sums round once per 16 terms (N / 16 + 2 roundings of 2^-24, at most 10),
+# and an inverse whose entries round 64 times: (5 * 10 + 64) * 2^-24 a chunk; errors decay or stay
+# bounded with the state, so chunks add at most like their number's square root: 2^-17 sqrt(chunks).
+def tol(dtype, L):
+    return 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -17 * max(1.0, (L / 64) ** 0.5)
+
+
+SHAPES = [(2, 1, 2, 1, 64, 64), (1, 63, 1, 1, 64, 64), (2, 64, 2, 2, 128, 128), (1, 65, 4, 2, 128, 64),
+          (2, 200, 3, 1, 64, 128), (1, 150, 2, 2, 40, 24), (1, 129, 2, 1, 17, 5), (2, 333, 4, 2, 128, 130),
+          (3, 70, 60, 30, 64, 128), (1, 100, 1, 1, 1, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("Bt,L,H,G,N,P", SHAPES)
+def test_rule(cuda_ops, Bt, L, H, G, N, P, dtype):
+    a, h0 = make(Bt, L, H, G, N, P, dtype, seed=L)
+    d = {k: v.to(dev) for k, v in a.items()}
+    d["u"] = d["u"].reshape(Bt, L, H * P)
+    y, h, (states, errors) = cuda_ops.gated_delta_rule(**d, scale=0.3, h0=h0.to(dev), return_state=True, save=True)
+    ry, rh = gated_delta(**a, scale=0.3, h0=h0)
+    assert y.dtype == dtype and y.shape == (Bt, L, H * P)
+    assert off(y.view(Bt, L, H, P), ry) < tol(dtype, L)
+    assert off(h, rh) < tol(torch.float32, L)
+    assert torch.equal(states[:, :, 0].cpu(), h0)
+    if L > 64:
+        cut = {k: (v if k == "A_log" else v[:, :64]) for k, v in a.items()}
+        assert off(states[:, :, 1], gated_delta(**cut, h0=h0)[1]) < tol(torch.float32, 64)
+    # without a state, y comes from two planes
+    y2 = cuda_ops.gated_delta_rule(**d, scale=0.3)
+    assert off(y2.view(Bt, L, H, P), gated_delta(**a, scale=0.3)[0]) < tol(dtype, L)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rule_same_key_again_and_again(cuda_ops, dtype):
+    """One key for every token, beta 1, next to no decay: A is all ones below the diagonal, where the
+    powers of A overflow any expansion; each write replaces the value before it."""
+    a, h0 = make(1, 130, 1, 1, 64, 64, dtype, seed=7)
+    a["B"][:] = 0
+    a["B"][..., 3] = 1
+    a["beta"][:] = 1
+    a["dt"][:] = 1e-6
+    d = {k: v.to(dev) for k, v in a.items()}
+    y, h = cuda_ops.gated_delta_rule(d["u"].flatten(2), d["A_log"], d["B"], d["C"], d["dt"], d["beta"], h0=h0.to(dev),
+                                     return_state=True)
+    ry, rh = gated_delta(**a, h0=h0)
+    assert off(y.view_as(ry), ry) < tol(dtype, 130) and off(h, rh) < tol(torch.float32, 130)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rule_resets_strong_decay_and_padding(cuda_ops, dtype):
+    """Infinite and large steps forget the state; padded tokens (zeros) leave it; what follows still fits."""
+    a, h0 = make(2, 200, 2, 1, 64, 64, dtype, seed=9, decay=20.0)
+    a["dt"][0, 70], a["dt"][1, 3] = float("inf"), 1e30
+    for k in ("u", "B", "C", "dt", "beta"):
+        a[k][0, 150:] = 0
+    d = {k: v.to(dev) for k, v in a.items()}
+    y, h = cuda_ops.gated_delta_rule(d["u"].flatten(2), d["A_log"], d["B"], d["C"], d["dt"], d["beta"], h0=h0.to(dev),
+                                     return_state=True)
+    ry, rh = gated_delta(**a, h0=h0)
+    assert off(y.view_as(ry), ry) < tol(dtype, 200) and off(h, rh) < tol(torch.float32, 200)
+    cut = cuda_ops.gated_delta_rule(d["u"][:1, :150].flatten(2), d["A_log"], d["B"][:1, :150], d["C"][:1, :150],
+                                    d["dt"][:1, :150], d["beta"][:1, :150], h0=h0[:1].to(dev), return_state=True)[1]
+    assert off(h[:1], cut.double().cpu()) < 2.0 ** -22
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rule_meets_step(cuda_ops, dtype):
+    """A prompt in one call, then tokens one by one, is the whole sequence; two calls are one."""
+    a, h0 = make(2, 100, 4, 2, 128, 64, dtype, seed=11)
+    d = {k: v.to(dev) for k, v in a.items()}
+    ry, rh = gated_delta(**a)
+    part = lambda s: (d["u"][:, s].flatten(2), d["A_log"], d["B"][:, s], d["C"][:, s], d["dt"][:, s], d["beta"][:, s])  # noqa: E731
+    y, h = cuda_ops.gated_delta_rule(*part(slice(0, 90)), return_state=True)
+    h2 = h.clone()
+    outs = [y.view(2, 90, 4, 64)]
+    for t in range(90, 100):
+        outs.append(cuda_ops.gated_delta_step(d["u"][:, t], d["dt"][:, t], h, d["A_log"], d["B"][:, t], d["C"][:, t],
+                                              d["beta"][:, t])[:, None])
+    assert off(torch.cat(outs, 1), ry) < tol(dtype, 100) and off(h, rh) < tol(torch.float32, 100)
+    y2, h2 = cuda_ops.gated_delta_rule(*part(slice(90, 100)), h0=h2, return_state=True)
+    assert off(y2.view(2, 10, 4, 64), ry[:, 90:]) < tol(dtype, 100) and off(h2, rh) < tol(torch.float32, 100)
+
+
+@pytest.mark.gpu
+def test_rule_empty_strided_stream_and_graph(cuda_ops):
+    a, h0 = make(2, 77, 2, 2, 64, 64, torch.bfloat16, seed=13)
+    d = {k: v.to(dev) for k, v in a.items()}
+    args = (d["u"].flatten(2), d["A_log"], d["B"], d["C"], d["dt"], d["beta"])
+    y, h = cuda_ops.gated_delta_rule(*args, h0=h0.to(dev), return_state=True)
+    # no tokens: the state passes through
+    none = cuda_ops.gated_delta_rule(*(t if t.dim() == 1 else t[:, :0] for t in args), h0=h0.to(dev), return_state=True)
+    assert none[0].shape == (2, 0, 128) and torch.equal(none[1].cpu(), h0)
+    # a transposed view and an odd offset
+    wide = torch.zeros(2, 77, 2, 80, device=dev, dtype=torch.bfloat16)
+    wide[..., 16:] = d["B"]
+    buf = torch.zeros(args[0].numel() + 1, device=dev, dtype=torch.bfloat16)
+    buf[1:] = args[0].flatten()
+    y2 = cuda_ops.gated_delta_rule(buf[1:].view_as(args[0]), d["A_log"], wide[..., 16:], *args[3:], h0=h0.to(dev), return_state=True)
+    assert torch.equal(y2[0], y) and torch.equal(y2[1], h)
+    # another stream, and a captured call replayed on new inputs
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        y3 = cuda_ops.gated_delta_rule(*args, h0=h0.to(dev), return_state=True)
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(y3[0], y) and torch.equal(y3[1], h)
+    graph, u = torch.cuda.CUDAGraph(), torch.zeros_like(args[0])
+    with torch.cuda.graph(graph):
+        y4, h4 = cuda_ops.gated_delta_rule(u, *args[1:], h0=None, return_state=True)
+    u.copy_(args[0])
+    graph.replay()
+    torch.cuda.synchronize()
+    y5, h5 = cuda_ops.gated_delta_rule(*args, return_state=True)
+    assert torch.equal(y4, y5) and torch.equal(h4, h5)
+
+
+def test_rule_refusals_without_gpu():
+    import triton_ssm_b200 as ts
+    from triton_ssm_b200 import _lib
+    from triton_ssm_b200.delta import _rule_args
+    a, h0 = make(2, 5, 4, 2, 16, 8, torch.float32)
+    a["u"] = a["u"].flatten(2)
+    with pytest.raises(ValueError, match="CUDA"):
+        ts.gated_delta_rule(**a)
+    order = ("u", "A_log", "B", "C", "dt", "beta")
+    for bad in (dict(u=a["u"].double()), dict(u=a["u"][..., :-1]), dict(B=a["B"][:, :, :1]), dict(C=a["C"].bfloat16()),
+                dict(beta=a["beta"][:, :4]), dict(A_log=a["A_log"][:3]), dict(h0=h0[:, :, :4]), dict(dt=a["dt"][0]),
+                dict(B=a["B"][:, :, [0, 1, 1]], C=a["C"][:, :, [0, 1, 1]])):
+        kw = dict(a, h0=h0, **{}) | bad
+        with pytest.raises(ValueError):
+            _rule_args("gated_delta_rule", *(kw[k] for k in order), kw["h0"])
+    lib = _lib.load_library()
+    one = 4096   # a non-null address that nothing reads
+
+    def rule(Bt=2, L=3, H=4, G=2, P=8, N=16, dtype=0, u=one, states=0, errors=0):
+        return lib.tssm_gated_delta_rule(u, one, one, one, one, one, 0, one, 0, states, errors, Bt, L, H, G, P, N, 1.0,
+                                         dtype, 0)
+
+    for kw in (dict(Bt=-1), dict(G=3), dict(G=0), dict(N=0), dict(N=129), dict(dtype=2), dict(u=0), dict(L=1 << 31),
+               dict(states=one), dict(errors=one)):
+        assert rule(**kw) == 1, kw
+    assert rule(Bt=0) == 0

@@ -55,6 +55,7 @@ SIGNATURES = {
     "tssm_mh_fwd_local": ([P] * 7 + [I64] * 4 + [I64] * 9 + [I64] * 2 + [I32, P], I32),
     "tssm_mh_output": ([P] * 7 + [I64] * 4 + [I64] * 5 + [I64] * 2 + [I32, P], I32),
     "tssm_gated_delta_step": ([P] * 8 + [I64] * 5 + [F64, I32, P], I32),
+    "tssm_gated_delta_rule": ([P] * 11 + [I64] * 6 + [F64, I32, P], I32),
     "tssm_group_norm_workspace_size": ([I64] * 4 + [I32, I32], I64),
     "tssm_group_norm_act": ([P] * 7 + [I64] * 5 + [F64, I32, I32, P], I32),
     "tssm_group_norm_act_bwd": ([P] * 10 + [I64] * 5 + [I32, I32, P], I32),

@@ -1,0 +1,367 @@
+// Chunked gated delta rule, forward (formulas and precision: delta.cuh).
+//
+// A block walks one (batch row, head) and 16 NCW value channels through the
+// sequence, 64 tokens at a time.  Value channels never mix, so each of the NCW
+// chain warps owns 16 of them and carries its state S^T [16 x N] in registers:
+//     KS^T = S^T K^T,  X^T = V^T - exp(l) KS^T,  E^T = X^T T^T,
+//     O^T  = scale exp(l) S^T Q^T + E^T (Aq diag(beta))^T,
+//     S^T  = exp(l_last) S^T + (E diag(w beta))^T K
+// Transposed, every product's result has the register layout of the next one's
+// left operand, so the chain needs no shared memory and no barrier; K, Q, T and
+// Aq are shared by the warps as right operands.  Four more warps load the next
+// chunk and build its A, T and Aq meanwhile (BUFS = 2), one barrier a chunk.
+#include "delta.cuh"
+
+namespace tssm {
+namespace delta {
+namespace {
+
+// XS: planes of an io value (1: bf16, 3: f32).  KN: N padded to 64 or 128.  NCW: chain warps.
+template <int XS, int KN, int NCW>
+struct FwdSmem {
+  static constexpr int BUFS = XS == 1 ? 2 : 1;
+  static constexpr int PB = 16 * NCW;                    // value channels of the block
+  static constexpr int PLANE = Q * KN * 2;
+  static constexpr int NAQ = XS == 1 ? 2 : 3;            // planes of Aq diag(beta)
+  static constexpr int VROW = XS == 1 ? PB * 2 : (PB + 4) * 4;   // f32 values: padded rows
+  static constexpr int K = 0, QQ = K + XS * PLANE, V = QQ + XS * PLANE, T = V + Q * VROW, AQ = T + 3 * SQ_BYTES,
+                       G = AQ + NAQ * SQ_BYTES, BUF = (G + (int)sizeof(Gates) + 127) / 128 * 128;
+  static constexpr int M = BUFS * BUF, BYTES = M + Q * AM * 4 + 128;
+};
+
+struct FwdArgs {
+  const void *u, *B, *C;
+  const float *A_log, *dt, *beta, *h0;
+  void* y;
+  float *h_last, *states, *errs;
+  int64_t L;
+  int H, G, P, N, npb;
+  int64_t nc;
+  float scale;
+  int vec_kq, vec_v;
+};
+
+template <int XS, int KN, int NCW, int NS>
+__global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdArgs a) {
+  using T = typename std::conditional<XS == 1, __nv_bfloat16, float>::type;
+  using SM = FwdSmem<XS, KN, NCW>;
+  constexpr int PB = SM::PB, RB = KN * 2, NT = KN / 8, NQ = XS == 1 ? 2 : 3;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((128u - (smem_addr(smem_raw) & 127u)) & 127u);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t bh = blockIdx.x / a.npb;
+  const int pb = (int)(blockIdx.x - bh * a.npb) * PB;
+  const int64_t b = bh / a.H;
+  const int h = (int)(bh - b * a.H), g = h / (a.H / a.G);
+  const int64_t su = (int64_t)a.H * a.P, sk = (int64_t)a.G * a.N;
+  const T* kp = (const T*)a.B + (b * a.L) * sk + (int64_t)g * a.N;
+  const T* qp = (const T*)a.C + (b * a.L) * sk + (int64_t)g * a.N;
+  const T* vp = (const T*)a.u + (b * a.L) * su + (int64_t)h * a.P + pb;
+  const int pvalid = min(PB, a.P - pb);
+
+  auto prep = [&](int64_t c) {   // 128 threads
+    const int t = threadIdx.x - NCW * 32;
+    uint8_t* buf = smem + (SM::BUFS == 2 ? (int)(c & 1) * SM::BUF : 0);
+    const uint32_t s = smem_addr(buf);
+    const int64_t t0 = c * Q;
+    const int rows = (int)min((int64_t)Q, a.L - t0);
+    load_planes<XS, KN, 128>(s + SM::K, SM::PLANE, kp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
+    load_planes<XS, KN, 128>(s + SM::QQ, SM::PLANE, qp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
+    if constexpr (XS == 1) {
+      load_planes<1, PB, 128>(s + SM::V, 0, vp + t0 * su, su, rows, pvalid, a.vec_v, t);
+    } else {
+      float* vs = reinterpret_cast<float*>(buf + SM::V);
+      for (int i = t; i < Q * PB; i += 128) {
+        const int r = i / PB, p = i % PB;
+        vs[r * (PB + 4) + p] = r < rows && p < pvalid ? ldf(vp + (t0 + r) * su + p) : 0.f;
+      }
+    }
+    Gates& gt = *reinterpret_cast<Gates*>(buf + SM::G);
+    if (t < 32)
+      gates_warp(gt, a.dt + b * a.L * a.H + h, a.beta + b * a.L * a.H + h, a.H, a.A_log[h], t0, a.L, t);
+    cp_async_wait_all();
+    bar_sync(1, 128);
+    chunk_matrices<XS, KN, SM::NAQ, 3>(s + SM::K, s + SM::QQ, gt, a.scale, reinterpret_cast<float*>(smem + SM::M),
+                                       s + SM::AQ, s + SM::T, t, 1);
+  };
+
+  // ---- chain state
+  const int p0 = 16 * warp;   // of the block's channels
+  const int pr = lane / 4, q2 = 2 * (lane % 4);
+  float S[NT][4];
+  const int64_t srow = (bh * a.P + pb + p0 + pr) * (int64_t)a.N;   // of h0, h_last
+  auto state_io = [&](float* dst, const float* src) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int n = 8 * j + q2 + (e & 1), p = pb + p0 + pr + (e >> 1) * 8;
+        const bool in = n < a.N && p < a.P;
+        const int64_t at = (int64_t)(e >> 1) * 8 * a.N + n;
+        if (dst) {
+          if (in) dst[at] = S[j][e];
+        } else {
+          S[j][e] = src && in ? src[at] : 0.f;
+        }
+      }
+  };
+
+  auto chain = [&](int64_t c) {
+    uint8_t* buf = smem + (SM::BUFS == 2 ? (int)(c & 1) * SM::BUF : 0);
+    const uint32_t s = smem_addr(buf);
+    const Gates& gt = *reinterpret_cast<const Gates*>(buf + SM::G);
+    const int64_t t0 = c * Q;
+    const int rows = (int)min((int64_t)Q, a.L - t0);
+    if (a.states) state_io(a.states + ((bh * a.nc + c) * a.P + pb + p0 + pr) * a.N, nullptr);
+    // KS^T, then X^T
+    float x[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < KN / 16; ++kk) {
+      uint32_t f[NS][4];
+      split_a<NS>(S[2 * kk], S[2 * kk + 1], f);
+#pragma unroll
+      for (int np = 0; np < 4; ++np) {
+        uint32_t w[XS][4];
+#pragma unroll
+        for (int z = 0; z < XS; ++z) ldsm4(w[z], at_b<RB>(s + SM::K + z * SM::PLANE, 16 * np, 2 * kk, lane));
+        mma_planes<NS, XS, NS>(x[2 * np], x[2 * np + 1], f, w);
+      }
+    }
+#pragma unroll
+    for (int np = 0; np < 4; ++np) {
+      float v[2][4];
+      if constexpr (XS == 1) {
+        uint32_t w[4];
+        ldsm4t(w, s + SM::V + tile_off<PB * 2>(16 * np + ((lane >> 4) << 3) + (lane & 7), p0 / 8 + ((lane >> 3) & 1)));
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          v[m >> 1][(m & 1) * 2] = lo2(w[m]);
+          v[m >> 1][(m & 1) * 2 + 1] = hi2(w[m]);
+        }
+      } else {
+        const float* vs = reinterpret_cast<const float*>(buf + SM::V) + p0 + pr;
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[m][e] = vs[(16 * np + 8 * m + q2 + (e & 1)) * (PB + 4) + (e >> 1) * 8];
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const float2 eg = *reinterpret_cast<const float2*>(gt.eg + 16 * np + 8 * m + q2);
+        float(&xx)[4] = x[2 * np + m];
+        xx[0] = v[m][0] - eg.x * xx[0];
+        xx[1] = v[m][1] - eg.y * xx[1];
+        xx[2] = v[m][2] - eg.x * xx[2];
+        xx[3] = v[m][3] - eg.y * xx[3];
+      }
+    }
+    // E^T = X^T T^T (T lower triangular: 16-blocks i >= j)
+    float er[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) er[i][e] = 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      uint32_t f[NS][4];
+      split_a<NS>(x[2 * t], x[2 * t + 1], f);
+#pragma unroll
+      for (int np = t; np < 4; ++np) {
+        uint32_t w[NS][4];
+#pragma unroll
+        for (int z = 0; z < NS; ++z) ldsm4(w[z], at_b<SQ_RB>(s + SM::T + z * SQ_BYTES, 16 * np, 2 * t, lane));
+        mma_planes<NS, NS, NS>(er[2 * np], er[2 * np + 1], f, w);
+      }
+    }
+    if (a.errs) {
+      float* ep = a.errs + ((b * a.L + t0) * a.H + h) * (int64_t)a.P + pb + p0 + pr;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int tk = 8 * i + q2 + (e & 1), p = (e >> 1) * 8;
+          if (tk < rows && p0 + pr + p < pvalid) ep[(int64_t)tk * su + p] = er[i][e];
+        }
+    }
+    // O^T: the state's part (x is free now), then the chunk's own
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < KN / 16; ++kk) {
+      uint32_t f[NQ][4];
+      split_a<NQ>(S[2 * kk], S[2 * kk + 1], f);
+#pragma unroll
+      for (int np = 0; np < 4; ++np) {
+        uint32_t w[XS][4];
+#pragma unroll
+        for (int z = 0; z < XS; ++z) ldsm4(w[z], at_b<RB>(s + SM::QQ + z * SM::PLANE, 16 * np, 2 * kk, lane));
+        mma_planes<NQ, XS, NQ>(x[2 * np], x[2 * np + 1], f, w);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 eg = *reinterpret_cast<const float2*>(gt.eg + 8 * i + q2);
+      x[i][0] *= a.scale * eg.x;
+      x[i][1] *= a.scale * eg.y;
+      x[i][2] *= a.scale * eg.x;
+      x[i][3] *= a.scale * eg.y;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      uint32_t f[NQ][4];
+      split_a<NQ>(er[2 * t], er[2 * t + 1], f);
+#pragma unroll
+      for (int np = t; np < 4; ++np) {
+        uint32_t w[NQ][4];
+#pragma unroll
+        for (int z = 0; z < NQ; ++z) ldsm4(w[z], at_b<SQ_RB>(s + SM::AQ + z * SQ_BYTES, 16 * np, 2 * t, lane));
+        mma_planes<NQ, NQ, NQ>(x[2 * np], x[2 * np + 1], f, w);
+      }
+    }
+    // y: through this warp's own columns of the value tile (bf16), one 16-byte piece a lane
+    T* yp = (T*)a.y + (b * a.L + t0) * su + (int64_t)h * a.P + pb;
+    if constexpr (XS == 1) {
+      __syncwarp();
+#pragma unroll
+      for (int np = 0; np < 4; ++np) {
+        const uint32_t w[4] = {pack2(x[2 * np][0], x[2 * np][1]), pack2(x[2 * np][2], x[2 * np][3]),
+                               pack2(x[2 * np + 1][0], x[2 * np + 1][1]), pack2(x[2 * np + 1][2], x[2 * np + 1][3])};
+        stsm4t(s + SM::V + tile_off<PB * 2>(16 * np + ((lane >> 4) << 3) + (lane & 7), p0 / 8 + ((lane >> 3) & 1)), w);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 16 + lane / 2, c8 = lane % 2;
+        const uint4 v = *reinterpret_cast<const uint4*>(buf + SM::V + tile_off<PB * 2>(r, p0 / 8 + c8));
+        const int p = p0 + 8 * c8;
+        if (r >= rows || p >= pvalid) continue;
+        if (a.vec_v) {
+          *reinterpret_cast<uint4*>(yp + (int64_t)r * su + p) = v;
+        } else {
+          const uint32_t vv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (p + e < pvalid) stf(yp + (int64_t)r * su + p + e, e & 1 ? hi2(vv[e / 2]) : lo2(vv[e / 2]));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int tk = 8 * i + q2 + (e & 1), p = p0 + pr + (e >> 1) * 8;
+          if (tk < rows && p < pvalid) stf(yp + (int64_t)tk * su + p, x[i][e]);
+        }
+    }
+    // S^T = exp(l_last) S^T + (E diag(w beta))^T K
+    const float el = gt.eg[Q - 1];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) S[j][e] *= el;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        const float2 wb = *reinterpret_cast<const float2*>(gt.wb + 16 * t + 8 * m + q2);
+        float(&ee)[4] = er[2 * t + m];
+        ee[0] *= wb.x;
+        ee[1] *= wb.y;
+        ee[2] *= wb.x;
+        ee[3] *= wb.y;
+      }
+      uint32_t f[NS][4];
+      split_a<NS>(er[2 * t], er[2 * t + 1], f);
+#pragma unroll
+      for (int nn = 0; nn < KN / 16; ++nn) {
+        uint32_t w[XS][4];
+#pragma unroll
+        for (int z = 0; z < XS; ++z) ldsm4t(w[z], at_a<RB>(s + SM::K + z * SM::PLANE, 16 * t, 2 * nn, lane));
+        mma_planes<NS, XS, NS>(S[2 * nn], S[2 * nn + 1], f, w);
+      }
+    }
+  };
+
+  if (warp < NCW) state_io(nullptr, a.h0 ? a.h0 + srow : nullptr);
+  if constexpr (SM::BUFS == 2) {
+    if (warp >= NCW && a.nc > 0) prep(0);
+    __syncthreads();
+    for (int64_t c = 0; c < a.nc; ++c) {
+      if (warp < NCW) chain(c);
+      else if (c + 1 < a.nc) prep(c + 1);
+      __syncthreads();
+    }
+  } else {
+    for (int64_t c = 0; c < a.nc; ++c) {
+      if (warp >= NCW) prep(c);
+      __syncthreads();
+      if (warp < NCW) chain(c);
+      __syncthreads();
+    }
+  }
+  if (warp < NCW && a.h_last) state_io(a.h_last + srow, nullptr);
+}
+
+template <int XS, int KN, int NCW, int NS>
+int launch(FwdArgs a, int64_t Bt, cudaStream_t st) {
+  constexpr int bytes = FwdSmem<XS, KN, NCW>::BYTES;
+  static_assert(bytes <= 232448, "shared-memory layout exceeds the per-block limit");
+  auto kern = delta_fwd_kernel<XS, KN, NCW, NS>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return check_launch("gated_delta_rule: set smem attribute");
+  a.npb = (int)cdiv(a.P, 16 * NCW);
+  const int64_t blocks = Bt * a.H * a.npb;
+  TSSM_REQUIRE(blocks < (int64_t(1) << 31), "gated_delta_rule: size out of range");
+  kern<<<(unsigned)blocks, (NCW + 4) * 32, bytes, st>>>(a);
+  return check_launch("gated_delta_rule");
+}
+
+template <int XS, int KN, int NS>
+int by_block(const FwdArgs& a, int64_t Bt, cudaStream_t st) {
+  // 128 channels a block when that still fills the SMs, else 64
+  if (a.P > 64 && Bt * a.H * cdiv(a.P, 128) >= num_sms()) return launch<XS, KN, 8, NS>(a, Bt, st);
+  return launch<XS, KN, 4, NS>(a, Bt, st);
+}
+
+}  // namespace
+}  // namespace delta
+}  // namespace tssm
+
+extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const void* B, const void* C, const void* dt,
+                                     const void* beta, const void* h0, void* y, void* h_last, void* states,
+                                     void* errors, int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N,
+                                     double scale, int dtype, tssm_stream_t stream) {
+  using namespace tssm;
+  using namespace tssm::delta;
+  TSSM_REQUIRE(Bt >= 0 && L >= 0 && H >= 0 && G >= 0 && P >= 0 && N >= 0, "gated_delta_rule: negative size");
+  if (Bt * H * P == 0) return TSSM_OK;
+  TSSM_REQUIRE(N >= 1 && N <= 128, "gated_delta_rule: state size N must be 1 to 128 (got %lld)", (long long)N);
+  TSSM_REQUIRE(G >= 1 && H % G == 0, "gated_delta_rule: H (%lld) must be a multiple of the key heads G (%lld)",
+               (long long)H, (long long)G);
+  TSSM_REQUIRE(A_log && (L == 0 || (u && B && C && dt && beta && y)), "gated_delta_rule: null pointer");
+  TSSM_REQUIRE((states != nullptr) == (errors != nullptr), "gated_delta_rule: states and errors go together");
+  TSSM_REQUIRE(dtype == TSSM_F32 || dtype == TSSM_BF16, "gated_delta_rule: dtype must be f32 or bf16 (got %d)", dtype);
+  TSSM_REQUIRE(L < (int64_t(1) << 31) && Bt < (int64_t(1) << 31) && H <= 1 << 20 && P <= 1 << 20,
+               "gated_delta_rule: size out of range");
+  FwdArgs a{};
+  a.u = u; a.B = B; a.C = C;
+  a.A_log = (const float*)A_log; a.dt = (const float*)dt; a.beta = (const float*)beta; a.h0 = (const float*)h0;
+  a.y = y; a.h_last = (float*)h_last; a.states = (float*)states; a.errs = (float*)errors;
+  a.L = L; a.H = (int)H; a.G = (int)G; a.P = (int)P; a.N = (int)N;
+  a.nc = cdiv(L, delta::Q);
+  a.scale = (float)scale;
+  const int per = dtype == TSSM_F32 ? 4 : 8;   // elements of 16 bytes
+  a.vec_kq = N % per == 0 && aligned16(B) && aligned16(C);
+  a.vec_v = P % per == 0 && aligned16(u) && aligned16(y);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  if (dtype == TSSM_F32) return N <= 64 ? by_block<3, 64, 3>(a, Bt, st) : by_block<3, 128, 3>(a, Bt, st);
+  // f32 results (the state, what the backward reads) want three planes; y alone is bf16: two
+  if (h_last || states) return N <= 64 ? by_block<1, 64, 3>(a, Bt, st) : by_block<1, 128, 3>(a, Bt, st);
+  return N <= 64 ? by_block<1, 64, 2>(a, Bt, st) : by_block<1, 128, 2>(a, Bt, st);
+}

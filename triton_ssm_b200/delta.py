@@ -18,7 +18,64 @@ import torch
 from ._lib import call, device_of, dtype_code, ptr, stream_of
 from .ops import _cuda, _need
 
-__all__ = ["gated_delta_step"]
+__all__ = ["gated_delta_rule", "gated_delta_step"]
+
+CHUNK = 64
+
+
+def _rule_args(name, u, A_log, B, C, dt, beta, h0):
+    _need(u, (torch.float32, torch.bfloat16), "u")
+    if u.dim() != 3 or B.dim() != 4 or dt.dim() != 3:
+        raise ValueError("%s: expected u [Bt,L,H*P], B, C [Bt,L,G,N], dt [Bt,L,H]" % name)
+    Bt, L, HP = u.shape
+    G, N = B.shape[2:]
+    H = dt.shape[2]
+    if H < 1 or G < 1 or HP % H or H % G:
+        raise ValueError("%s: u's last dim (%d) must be H*P and H (%d) a multiple of G (%d)" % (name, HP, H, G))
+    P = HP // H
+    if tuple(B.shape) != (Bt, L, G, N) or C.shape != B.shape or tuple(dt.shape) != (Bt, L, H) or \
+            beta.shape != dt.shape or tuple(A_log.shape) != (H,) or \
+            (h0 is not None and tuple(h0.shape) != (Bt, H, P, N)):
+        raise ValueError("%s: shape mismatch" % name)
+    if B.dtype != u.dtype or C.dtype != u.dtype:
+        raise ValueError("%s: B and C must have u's dtype" % name)
+    return Bt, L, H, G, P, N
+
+
+def gated_delta_rule(u, A_log, B, C, dt, beta, scale=1.0, h0=None, return_state=False, save=False, y=None):
+    """The gated delta rule over whole sequences.
+
+    u [Bt,L,H*P] f32 or bf16; A_log [H] f32 (log(-A_h)); B, C [Bt,L,G,N] in
+    u's dtype, H a multiple of G, N <= 128; dt, beta [Bt,L,H] f32; h0
+    [Bt,H,P,N] f32 or None.  Values must be finite (a chunk of 64 tokens is one
+    matrix problem); pad with zeros, dt = 0 and beta = 0.
+    Returns y [Bt,L,H*P] in u's dtype, or a tuple: y, then h_last [Bt,H,P,N]
+    f32 when ``return_state``, then, when ``save``, what
+    ``gated_delta_rule_bwd`` reads: (the state before every chunk
+    [Bt,H,ceil(L/64),P,N], the prediction errors u_t - hd B_t [Bt,L,H,P]), f32.
+    """
+    _cuda(u, A_log, B, C, dt, beta, h0, y)
+    Bt, L, H, G, P, N = _rule_args("gated_delta_rule", u, A_log, B, C, dt, beta, h0)
+    u, B, C = u.contiguous(), B.contiguous(), C.contiguous()
+    A_log, dt, beta = (t.float().contiguous() for t in (A_log, dt, beta))
+    h0 = h0.float().contiguous() if h0 is not None else None
+    if y is None:
+        y = torch.empty_like(u)
+    elif y.shape != u.shape or y.dtype != u.dtype or not y.is_contiguous():
+        raise ValueError("gated_delta_rule: y must be contiguous and match u")
+    f32 = dict(device=u.device, dtype=torch.float32)
+    hl = torch.empty(Bt, H, P, N, **f32) if return_state else None
+    states = torch.empty(Bt, H, -(-L // CHUNK), P, N, **f32) if save else None
+    errors = torch.empty(Bt, L, H, P, **f32) if save else None
+    with device_of(u):
+        call("tssm_gated_delta_rule", ptr(u), ptr(A_log), ptr(B), ptr(C), ptr(dt), ptr(beta), ptr(h0), ptr(y), ptr(hl),
+             ptr(states), ptr(errors), Bt, L, H, G, P, N, float(scale), dtype_code(u), stream_of(u))
+    out = [y]
+    if return_state:
+        out.append(hl)
+    if save:
+        out.append((states, errors))
+    return out[0] if len(out) == 1 else tuple(out)
 
 
 def gated_delta_step(x, dt, h, A_log, B, C, beta, scale=1.0, y=None):
