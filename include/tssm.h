@@ -479,6 +479,21 @@ int tssm_gated_delta_rule(const void* u, const void* A_log, const void* B, const
                           double scale, int dtype, tssm_stream_t stream);
 
 /*
+ * Backward of tssm_gated_delta_rule: from the same inputs, dy (as y), the
+ * forward's states and errors, and dh_last (f32 or null), the gradients du,
+ * dB, dC (io), dA_log [H], ddt, dbeta [Bt,L,H] and dh0 (f32).  Deterministic.
+ * workspace: tssm_gated_delta_rule_bwd_workspace_size bytes, 16-byte aligned.
+ */
+int64_t tssm_gated_delta_rule_bwd_workspace_size(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P,
+                                                 int64_t N);
+int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const void* B, const void* C, const void* dt,
+                              const void* beta, const void* dy, const void* states, const void* errors,
+                              const void* dh_last, void* du, void* dA_log, void* dB, void* dC, void* ddt,
+                              void* dbeta, void* dh0, void* workspace, int64_t workspace_bytes, int64_t Bt,
+                              int64_t L, int64_t H, int64_t G, int64_t P, int64_t N, double scale, int dtype,
+                              tssm_stream_t stream);
+
+/*
  * Group norm with an activation, channels last: x, y [Bt,L,C] (dtype f32 or
  * bf16), mean and variance over L and the C/groups channels of a group,
  * weight, bias [C] f32, act 0 (none) or 1 (SiLU).  mean, rstd [Bt,groups] f32

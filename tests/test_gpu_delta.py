@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from oracle.delta import gated_delta
+from oracle.delta import gated_delta, gated_delta_grads
 
 dev = "cuda"
 HALF = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8}
@@ -246,3 +246,133 @@ def test_rule_refusals_without_gpu():
                dict(states=one), dict(errors=one)):
         assert rule(**kw) == 1, kw
     assert rule(Bt=0) == 0
+
+
+# ------------------------------------------------------------------ backward
+NAMES = ("du", "dA_log", "dB", "dC", "ddt", "dbeta", "dh0")
+
+
+def run_bwd(ts, a, h0, dy, dh, scale):
+    d = {k: v.to(dev) for k, v in a.items()}
+    args = (d["u"].flatten(2), d["A_log"], d["B"], d["C"], d["dt"], d["beta"])
+    _, saved = ts.gated_delta_rule(*args, scale=scale, h0=None if h0 is None else h0.to(dev), save=True)
+    return ts.gated_delta_rule_bwd(*args, dy.to(dev).flatten(2), saved, scale=scale,
+                                   dh_last=None if dh is None else dh.to(dev))
+
+
+def check_grads(grads, ref, a, dtype, L):
+    """The forward's chain and the backward's: twice the forward's f32 tolerance.  A dt's gradient is a sum of
+    up to 64 x 64 paths within a chunk, 16 more roundings.  dA_log sums ddt dt over all tokens with either sign:
+    its tolerance is of the sum of magnitudes."""
+    f32 = 4 * tol(torch.float32, L)
+    for name, x, r in zip(NAMES, grads, ref):
+        r = r.reshape(x.shape)
+        if name == "dA_log":
+            size = (ref[4].abs() * a["dt"].double().clamp(max=1e6)).sum((0, 1))
+            assert bool(((x.double().cpu() - r).abs() <= f32 * size).all()), name
+        else:
+            t = f32 if x.dtype == torch.float32 else tol(dtype, L)
+            assert off(x, r) < t, "%s: %.3g, tolerance %.3g" % (name, off(x, r), t)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("Bt,L,H,G,N,P", SHAPES)
+def test_backward(cuda_ops, Bt, L, H, G, N, P, dtype):
+    a, h0 = make(Bt, L, H, G, N, P, dtype, seed=L + 1)
+    g = torch.Generator().manual_seed(L)
+    dy, dh = torch.randn(Bt, L, H, P, generator=g).to(dtype), 0.3 * torch.randn(Bt, H, P, N, generator=g)
+    grads = run_bwd(cuda_ops, a, h0, dy, dh, 0.3)
+    check_grads(grads, gated_delta_grads(*a.values(), dy, scale=0.3, h0=h0, dh_last=dh), a, dtype, L)
+    for x, like in zip(grads, (a["u"], a["A_log"], a["B"], a["C"], a["dt"], a["beta"], h0)):
+        assert x.dtype == like.dtype and x.numel() == like.numel()
+
+
+@pytest.mark.gpu
+def test_backward_without_states(cuda_ops):
+    """No h0, no gradient of the final state."""
+    a, _ = make(2, 130, 2, 2, 64, 64, torch.float32, seed=21)
+    dy = torch.randn(2, 130, 2, 64, generator=torch.Generator().manual_seed(1))
+    check_grads(run_bwd(cuda_ops, a, None, dy, None, 1.0), gated_delta_grads(*a.values(), dy), a, torch.float32, 130)
+
+
+@pytest.mark.gpu
+def test_backward_same_key_resets_and_zero_beta(cuda_ops):
+    """One key again and again, beta 0 and 1, infinite steps and padding."""
+    a, h0 = make(2, 140, 1, 1, 64, 64, torch.float32, seed=22)
+    a["B"][0] = 0
+    a["B"][0, ..., 3] = 1
+    a["beta"][0], a["dt"][0] = 1, 1e-6
+    a["beta"][1, ::3] = 0
+    a["dt"][1, 50] = 1e4    # exp(-5000) is 0 in both precisions
+    for k in ("u", "B", "C", "dt", "beta"):
+        a[k][1, 120:] = 0
+    g = torch.Generator().manual_seed(2)
+    dy, dh = torch.randn(2, 140, 1, 64, generator=g), torch.randn(2, 1, 64, 64, generator=g)
+    grads = run_bwd(cuda_ops, a, h0, dy, dh, 1.0)
+    check_grads(grads, gated_delta_grads(*a.values(), dy, h0=h0, dh_last=dh), a, torch.float32, 140)
+    a["dt"][1, 50] = float("inf")
+    again = run_bwd(cuda_ops, a, h0, dy, dh, 1.0)
+    for x, y in zip(grads, again):
+        assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+def test_backward_against_differences(cuda_ops):
+    a, h0 = make(1, 70, 2, 1, 32, 16, torch.float32, seed=23)
+    g = torch.Generator().manual_seed(3)
+    dy, dh = torch.randn(1, 70, 2, 16, generator=g).double(), torch.randn(1, 2, 16, 32, generator=g).double()
+    grads = run_bwd(cuda_ops, a, h0, dy.float(), dh.float(), 0.5)
+    dy, dh = dy.float().double(), dh.float().double()
+    leaves = [t.double() for t in (*a.values(), h0)]
+    e = 1e-5
+    for i, gr in enumerate(grads):
+        d = torch.randn(leaves[i].shape, generator=g).double()
+        f = []
+        for s in (e, -e):
+            x = list(leaves)
+            x[i] = x[i] + s * d
+            y, h = gated_delta(*x[:6], scale=0.5, h0=x[6])
+            f.append(((y * dy).sum() + (h * dh).sum()).item())
+        got = (gr.double().cpu().reshape(d.shape) * d).sum().item()
+        size = (gr.double().cpu().reshape(d.shape) * d).abs().sum().item()
+        assert abs((f[0] - f[1]) / (2 * e) - got) < 1e-5 * size + 1e-6, NAMES[i]
+
+
+@pytest.mark.gpu
+def test_backward_graph_repeats_and_empty(cuda_ops):
+    a, h0 = make(2, 100, 4, 2, 128, 64, torch.bfloat16, seed=24)
+    g = torch.Generator().manual_seed(4)
+    dy, dh = torch.randn(2, 100, 4, 64, generator=g).bfloat16(), torch.randn(2, 4, 64, 128, generator=g)
+    first = run_bwd(cuda_ops, a, h0, dy, dh, 1.0)
+    d = {k: v.to(dev) for k, v in a.items()}
+    args = (d["u"].flatten(2), d["A_log"], d["B"], d["C"], d["dt"], d["beta"])
+    hd, dyd, dhd = h0.to(dev), dy.to(dev).flatten(2), dh.to(dev)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        _, saved = cuda_ops.gated_delta_rule(*args, h0=hd, save=True)
+        again = cuda_ops.gated_delta_rule_bwd(*args, dyd, saved, dh_last=dhd)
+    graph.replay()
+    graph.replay()
+    torch.cuda.synchronize()
+    for x, y in zip(first, again):
+        assert torch.equal(x, y)
+    none = tuple(t if t.dim() == 1 else t[:, :0] for t in args)
+    _, saved = cuda_ops.gated_delta_rule(*none, h0=hd, save=True)
+    out = cuda_ops.gated_delta_rule_bwd(*none, dyd[:, :0], saved, dh_last=dhd)
+    assert torch.equal(out[6], dhd) and not out[1].any()
+
+
+def test_backward_refusals_without_gpu():
+    from triton_ssm_b200 import _lib
+    lib = _lib.load_library()
+    one = 4096   # a non-null address that nothing reads
+
+    def bwd(Bt=2, L=3, H=4, G=2, P=8, N=16, dtype=0, dy=one, ws=one, nbytes=1 << 30):
+        return lib.tssm_gated_delta_rule_bwd(one, one, one, one, one, one, dy, one, one, 0, one, one, one, one, one, one,
+                                             one, ws, nbytes, Bt, L, H, G, P, N, 1.0, dtype, 0)
+
+    for kw in (dict(Bt=-1), dict(G=3), dict(G=0), dict(N=0), dict(N=129), dict(dtype=2), dict(dy=0), dict(ws=0),
+               dict(nbytes=100), dict(ws=one + 4), dict(L=1 << 31)):
+        assert bwd(**kw) == 1, kw

@@ -120,7 +120,8 @@ __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync
 struct Gates {        // in shared memory
   float lh[Q], ll[Q];   // l_i in log2 units as a sum of two floats (differences of long sums stay exact)
   float eg[Q];          // exp(l_i)
-  float wb[Q];          // exp(l_last - l_i) beta_i
+  float w[Q];           // exp(l_last - l_i)
+  float wb[Q];          // w_i beta_i
   float beta[Q];
 };
 
@@ -163,7 +164,8 @@ __device__ __forceinline__ void gates_warp(Gates& g, const float* dt, const floa
     g.eg[i] = exp2_pair(h, lo);
     const double d = last - li[e];
     const float dh = (float)d;
-    g.wb[i] = exp2_pair(dh, (float)(d - (double)dh)) * b[e];
+    g.w[i] = exp2_pair(dh, (float)(d - (double)dh));
+    g.wb[i] = g.w[i] * b[e];
     g.beta[i] = b[e];
   }
 }

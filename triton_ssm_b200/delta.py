@@ -15,10 +15,11 @@ key head i // (H // G).
 """
 import torch
 
+from . import _lib
 from ._lib import call, device_of, dtype_code, ptr, stream_of
 from .ops import _cuda, _need
 
-__all__ = ["gated_delta_rule", "gated_delta_step"]
+__all__ = ["gated_delta_rule", "gated_delta_rule_bwd", "gated_delta_step"]
 
 CHUNK = 64
 
@@ -76,6 +77,38 @@ def gated_delta_rule(u, A_log, B, C, dt, beta, scale=1.0, h0=None, return_state=
     if save:
         out.append((states, errors))
     return out[0] if len(out) == 1 else tuple(out)
+
+
+def gated_delta_rule_bwd(u, A_log, B, C, dt, beta, dy, saved, scale=1.0, dh_last=None):
+    """Backward of ``gated_delta_rule``.
+
+    The forward's inputs, dy [Bt,L,H*P] in u's dtype, ``saved`` from a forward
+    with ``save=True`` (and the same ``scale``), dh_last [Bt,H,P,N] f32 or None
+    (the gradient of the final state).  Returns (du, dA_log, dB, dC, ddt,
+    dbeta, dh0): du, dB, dC in u's dtype, the others f32; dB and dC are summed
+    over the heads that share a key head.  Every sum runs in a fixed order.
+    """
+    states, errors = saved
+    _cuda(u, A_log, B, C, dt, beta, dy, states, errors, dh_last)
+    Bt, L, H, G, P, N = _rule_args("gated_delta_rule_bwd", u, A_log, B, C, dt, beta, dh_last)
+    if dy.shape != u.shape or dy.dtype != u.dtype:
+        raise ValueError("gated_delta_rule_bwd: dy must match u")
+    for t, shape in ((states, (Bt, H, -(-L // CHUNK), P, N)), (errors, (Bt, L, H, P))):
+        if tuple(t.shape) != shape or t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError("gated_delta_rule_bwd: saved must be what gated_delta_rule(..., save=True) returned")
+    u, B, C, dy = u.contiguous(), B.contiguous(), C.contiguous(), dy.contiguous()
+    A_log, dt, beta = (t.float().contiguous() for t in (A_log, dt, beta))
+    dh_last = dh_last.float().contiguous() if dh_last is not None else None
+    f32 = dict(device=u.device, dtype=torch.float32)
+    du, dB, dC, dA_log = torch.empty_like(u), torch.empty_like(B), torch.empty_like(C), torch.empty_like(A_log)
+    ddt, dbeta, dh0 = torch.empty_like(dt), torch.empty_like(beta), torch.empty(Bt, H, P, N, **f32)
+    need = int(_lib.load_library().tssm_gated_delta_rule_bwd_workspace_size(Bt, L, H, G, P, N))
+    ws = torch.empty(need, dtype=torch.uint8, device=u.device) if need else None
+    with device_of(u):
+        call("tssm_gated_delta_rule_bwd", ptr(u), ptr(A_log), ptr(B), ptr(C), ptr(dt), ptr(beta), ptr(dy), ptr(states),
+             ptr(errors), ptr(dh_last), ptr(du), ptr(dA_log), ptr(dB), ptr(dC), ptr(ddt), ptr(dbeta), ptr(dh0), ptr(ws),
+             need, Bt, L, H, G, P, N, float(scale), dtype_code(u), stream_of(u))
+    return du, dA_log, dB, dC, ddt, dbeta, dh0
 
 
 def gated_delta_step(x, dt, h, A_log, B, C, beta, scale=1.0, y=None):
