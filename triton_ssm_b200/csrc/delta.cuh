@@ -117,8 +117,15 @@ __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wai
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
 // ------------------------------------------------------------------ one chunk's gates
+// D_ij of tokens in different 16-token blocks I > J is a_i c_IJ b_j, every factor at most 1
+// and from the 64-bit sums: a_i = exp(l_i - l_{16 I - 1}), b_j = exp(l_{16 J + 15} - l_j),
+// c_IJ = exp(l_{16 I - 1} - l_{16 J + 15}).
 struct Gates {        // in shared memory
   float lh[Q], ll[Q];   // l_i in log2 units as a sum of two floats (differences of long sums stay exact)
+  float a[Q];           // a_i (blocks 1 to 3)
+  float bb[Q];          // b_i beta_i
+  float b[Q];           // b_i
+  float c[16];          // c_IJ at 4 I + J
   float eg[Q];          // exp(l_i)
   float w[Q];           // exp(l_last - l_i)
   float wb[Q];          // w_i beta_i
@@ -168,6 +175,18 @@ __device__ __forceinline__ void gates_warp(Gates& g, const float* dt, const floa
     g.wb[i] = g.w[i] * b[e];
     g.beta[i] = b[e];
   }
+  const double blk = __shfl_sync(0xffffffffu, s, lane | 7);               // l at the end of this token's block
+  const double prv = __shfl_sync(0xffffffffu, s, ((lane & 24) - 1) & 31);   // and of the block before
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int i = 2 * lane + e;
+    g.a[i] = lane >= 8 ? exp2f((float)(li[e] - prv)) : 1.f;
+    g.b[i] = exp2f((float)(blk - li[e]));
+    g.bb[i] = g.b[i] * b[e];
+  }
+  const int I = (lane >> 2) & 3, J = lane & 3;
+  const double lI = __shfl_sync(0xffffffffu, s, (8 * I - 1) & 31), lJ = __shfl_sync(0xffffffffu, s, 8 * J + 7);
+  if (lane < 16) g.c[lane] = J < I ? exp2f((float)(lI - lJ)) : 1.f;
 }
 
 // ------------------------------------------------------------------ loading tiles
@@ -177,16 +196,23 @@ template <int XS, int W, int NTH, typename T>
 __device__ __forceinline__ void load_planes(uint32_t dst, int plane_bytes, const T* src, int64_t stride, int rows,
                                             int valid, bool vec, int t) {
   constexpr int RB = W * 2, PIECES = W / 8;
+  static_assert(NTH % PIECES == 0, "a thread keeps its column");
+  if constexpr (XS == 1) {
+    if (vec) {
+      constexpr int STEP = NTH / PIECES;   // rows per pass
+      const int c = t % PIECES, r0 = t / PIECES;
+      const bool col = c * 8 < valid;
+      const T* p = src + (col ? (int64_t)r0 * stride + c * 8 : 0);
+#pragma unroll 2
+      for (int r = r0; r < Q; r += STEP, p += STEP * stride)
+        cp_async16(dst + tile_off<RB>(r, c), r < rows && col ? p : src, r < rows && col);
+      return;
+    }
+  }
+#pragma unroll 1
   for (int i = t; i < Q * PIECES; i += NTH) {
     const int r = i / PIECES, c = i % PIECES;
     const uint32_t off = tile_off<RB>(r, c);
-    if constexpr (XS == 1) {
-      if (vec) {
-        const bool in = r < rows && c * 8 < valid;
-        cp_async16(dst + off, src + (in ? (int64_t)r * stride + c * 8 : 0), in);
-        continue;
-      }
-    }
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = 0.f;
@@ -218,58 +244,64 @@ __device__ __forceinline__ void load_planes(uint32_t dst, int plane_bytes, const
 // ------------------------------------------------------------------ A, Aq and T of one chunk
 constexpr int AM = Q + 4;   // floats per row of the f32 work matrix
 
-// Lower triangle of X K^T for the 16 rows from 16 w of X (one warp): g[nt] holds columns
-// 8 nt .., tiles behind the diagonal block are not computed.
-template <int XS, int KN>
-__device__ __forceinline__ void gram_rows(float (&g)[8][4], uint32_t x, uint32_t k, int w, int lane) {
-  constexpr int RB = KN * 2, PB = Q * RB;
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const float (&a)[4], float b0, float b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(__float_as_uint(a[0])), "r"(__float_as_uint(a[1])), "r"(__float_as_uint(a[2])), "r"(__float_as_uint(a[3])),
+        "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
+}
+// x = hi + lo: hi the 11 leading bits, lo the rest (of which the tensor core takes 11).
+__device__ __forceinline__ void tf32_split(float x, float& hi, float& lo) {
+  hi = __uint_as_float(__float_as_uint(x) & 0xffffe000u);
+  lo = x - hi;
+}
+
+// One warp: out [16 x 8 NT] = sign * X [16 x 8 KS] Y [8 KS x 8 NT], rows of AM floats, f32
+// accuracy from three products of tf32 halves.
+template <int KS, int NT>
+__device__ __forceinline__ void block_mma(const float* X, const float* Y, float* out, float sign, int lane) {
+  const int g = lane >> 2, t = lane & 3;
+  float d[NT][4];
 #pragma unroll
-  for (int nt = 0; nt < 8; ++nt)
+  for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) g[nt][i] = 0.f;
-#pragma unroll 2
-  for (int kk = 0; kk < KN / 16; ++kk) {
-    uint32_t a[XS][4];
+    for (int e = 0; e < 4; ++e) d[n][e] = 0.f;
 #pragma unroll
-    for (int s = 0; s < XS; ++s) ldsm4(a[s], at_a<RB>(x + s * PB, 16 * w, 2 * kk, lane));
+  for (int k = 0; k < KS; ++k) {
+    float ah[4], al[4];
 #pragma unroll
-    for (int np = 0; np < 4; ++np) {
-      if (np > w) break;
-      uint32_t b[XS][4];
+    for (int e = 0; e < 4; ++e) tf32_split(X[(g + 8 * (e & 1)) * AM + 8 * k + t + 4 * (e >> 1)], ah[e], al[e]);
 #pragma unroll
-      for (int s = 0; s < XS; ++s) ldsm4(b[s], at_b<RB>(k + s * PB, 16 * np, 2 * kk, lane));
-      mma_planes<XS, XS, XS>(g[2 * np], g[2 * np + 1], a, b);
+    for (int n = 0; n < NT; ++n) {
+      float bh[2], bl[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) tf32_split(Y[(8 * k + t + 4 * e) * AM + 8 * n + g], bh[e], bl[e]);
+      mma_tf32(d[n], al, bh[0], bh[1]);
+      mma_tf32(d[n], ah, bl[0], bl[1]);
+      mma_tf32(d[n], ah, bh[0], bh[1]);
     }
   }
+#pragma unroll
+  for (int n = 0; n < NT; ++n)
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<float2*>(out + (g + 8 * e) * AM + 8 * n + 2 * t) =
+          make_float2(sign * d[n][2 * e], sign * d[n][2 * e + 1]);
 }
 
-// c[2 rows x 4 columns] (+)= X[r.., k] Y[k, c..] over k in [0, KD): X, Y, out rows of AM floats.
-template <int KD>
-__device__ __forceinline__ void block_2x4(const float* X, const float* Y, float (&c)[2][4]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) c[i][j] = 0.f;
-#pragma unroll 8
-  for (int k = 0; k < KD; ++k) {
-    const float4 y = *reinterpret_cast<const float4*>(Y + k * AM);
-    const float x0 = X[k], x1 = X[AM + k];
-    c[0][0] += x0 * y.x; c[0][1] += x0 * y.y; c[0][2] += x0 * y.z; c[0][3] += x0 * y.w;
-    c[1][0] += x1 * y.x; c[1][1] += x1 * y.y; c[1][2] += x1 * y.z; c[1][3] += x1 * y.w;
-  }
-}
-
-// In place: the strictly lower M (row-major, AM floats a row) becomes (I + M)^-1.  128 threads
-// (t), named barrier `bar`.  16 x 16 diagonal blocks by forward substitution (a column per
-// thread), then 16 -> 32 -> 64 by T21 = -T22 (M21 T11); the unused upper blocks hold M21 T11.
+// In place: the strictly lower M (row-major, AM floats a row) becomes (I + M)^-1, on and below
+// the diagonal 16 x 16 blocks; the blocks above hold scratch.  128 threads (t), named barrier
+// `bar`.  Diagonal blocks by forward substitution (a column per thread), then 16 -> 32 -> 64 by
+// T21 = -T22 (M21 T11) on the tensor cores.
 __device__ __forceinline__ void invert_unit_lower(float* M, int t, int bar) {
+  const int w = t / 32, lane = t % 32;
   if (t < 64) {
     const int o = (t / 16) * 16, col = t % 16;
     const float* B = M + o * AM + o;
     float x[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      float v = i == col ? 1.f : 0.f;
+      float v = i == col ? 1.f : 0.f, v2 = 0.f;
 #pragma unroll
       for (int k = 0; k < 16; k += 4) {
         if (k >= i) break;
@@ -277,54 +309,31 @@ __device__ __forceinline__ void invert_unit_lower(float* M, int t, int bar) {
         const float mm[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (k + e < i) v -= mm[e] * x[k + e];
+          if (k + e < i) (e & 1 ? v2 : v) -= mm[e] * x[k + e];
       }
-      x[i] = v;
+      x[i] = v + v2;
     }
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < 16; ++i) M[(o + i) * AM + o + col] = x[i];
   }
   bar_sync(bar, 128);
-  {   // two pairs of 16-blocks, 32 threads each (2 x 4 outputs a thread)
-    float c[2][4];
-    const int o = (t / 32 & 1) * 32, r = (t % 32) / 4 * 2, cc = t % 4 * 4;
-    if (t < 64) {
-      block_2x4<16>(M + (o + 16 + r) * AM + o, M + o * AM + o + cc, c);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<float4*>(M + (o + r + i) * AM + o + 16 + cc) = make_float4(c[i][0], c[i][1], c[i][2], c[i][3]);
-      __syncwarp();
-      block_2x4<16>(M + (o + 16 + r) * AM + o + 16, M + o * AM + o + 16 + cc, c);
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<float4*>(M + (o + 16 + r + i) * AM + o + cc) = make_float4(-c[i][0], -c[i][1], -c[i][2], -c[i][3]);
-    }
-  }
-  bar_sync(bar, 128);
-  {
-    // The 16-blocks above the diagonal inside the 32-blocks held scratch: they are zero in T.
-    if (t >= 64) {
-      const int o = (t / 32 & 1) * 32, r = (t % 32) / 2, h = (t % 2) * 8;
-#pragma unroll
-      for (int e = 0; e < 8; e += 4)
-        *reinterpret_cast<float4*>(M + (o + r) * AM + o + 16 + h + e) = make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-  }
-  bar_sync(bar, 128);
-  {
-    float c[2][4];
-    const int r = t / 8 * 2, cc = t % 8 * 4;
-    block_2x4<32>(M + (32 + r) * AM, M + cc, c);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      *reinterpret_cast<float4*>(M + (r + i) * AM + 32 + cc) = make_float4(c[i][0], c[i][1], c[i][2], c[i][3]);
+  {   // two pairs of 16-blocks, two warps each
+    const int o = (w / 2) * 32, n = (w % 2) * 8;
+    block_mma<2, 1>(M + (o + 16) * AM + o, M + o * AM + o + n, M + o * AM + o + 16 + n, 1.f, lane);
     bar_sync(bar, 128);
-    block_2x4<32>(M + (32 + r) * AM + 32, M + 32 + cc, c);
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      *reinterpret_cast<float4*>(M + (32 + r + i) * AM + cc) = make_float4(-c[i][0], -c[i][1], -c[i][2], -c[i][3]);
+    block_mma<2, 1>(M + (o + 16) * AM + o + 16, M + o * AM + o + 16 + n, M + (o + 16) * AM + o + n, -1.f, lane);
+  }
+  bar_sync(bar, 128);
+  {   // the pair of 32-blocks, a 16 x 16 quarter per warp; blocks above T's diagonal are skipped
+    const int m = (w / 2) * 16, n = (w % 2) * 16;
+    const float *A21 = M + (32 + m) * AM, *T22 = M + (32 + m) * AM + 32;
+    float *Y = M + 32, *T21 = M + (32 + m) * AM + n;
+    if (n == 0) block_mma<4, 2>(A21, M, Y + m * AM, 1.f, lane);
+    else block_mma<2, 2>(A21 + 16, M + 16 * AM + 16, Y + m * AM + 16, 1.f, lane);
+    bar_sync(bar, 128);
+    if (m == 0) block_mma<2, 2>(T22, Y + n, T21, -1.f, lane);
+    else block_mma<4, 2>(T22, Y + n, T21, -1.f, lane);
   }
   bar_sync(bar, 128);
 }
@@ -338,45 +347,74 @@ constexpr int SQ_RB = 128, SQ_BYTES = Q * SQ_RB;
 template <int XS, int KN, int NA, int NTP>
 __device__ __forceinline__ void chunk_matrices(uint32_t k, uint32_t q, const Gates& g, float scale, float* M,
                                                uint32_t aq, uint32_t tp, int t, int bar) {
-  const int w = t / 32, lane = t % 32;
-  const int r0 = 16 * w + lane / 4;
-  float acc[8][4];
+  constexpr int RB = KN * 2, PB = Q * RB, KK = KN / 16;
+  const int w = t / 32, lane = t % 32, gr = lane / 4, q2 = 2 * (lane % 4);
 #pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {   // K K^T, then Q K^T
-    gram_rows<XS, KN>(acc, pass ? q : k, k, w, lane);
+  for (int pass = 0; pass < 2; ++pass) {   // K K^T, then Q K^T with the rows dealt the other way round
+    const int I = pass ? 3 - w : w, r0 = 16 * I + gr;
+    uint32_t a[XS == 1 ? KK : 1][XS][4];   // this row block's operand (bf16: kept for all column blocks)
+    if constexpr (XS == 1)
 #pragma unroll
-    for (int nt = 0; nt < 8; ++nt) {
-      if (nt > 2 * w + 1) break;
-      const int j = 8 * nt + 2 * (lane % 4);
-      const float2 bj = *reinterpret_cast<const float2*>(g.beta + j);
-      const float2 hj = *reinterpret_cast<const float2*>(g.lh + j);
-      const float2 lj = *reinterpret_cast<const float2*>(g.ll + j);
+      for (int kk = 0; kk < KK; ++kk) ldsm4(a[kk][0], at_a<RB>(pass ? q : k, 16 * I, 2 * kk, lane));
+    const float ra[2] = {g.a[r0], g.a[r0 + 8]};
+    const float sc = pass ? scale : 1.f;
+#pragma unroll 1
+    for (int J = 0; J <= I; ++J) {
+      float d[2][4];
 #pragma unroll
-      for (int hrow = 0; hrow < 2; ++hrow) {
-        const int i = r0 + 8 * hrow;
-        const float hi = g.lh[i], li = g.ll[i];
-        const bool in0 = pass ? j <= i : j < i, in1 = pass ? j + 1 <= i : j + 1 < i;
-        const float v0 = in0 ? acc[nt][2 * hrow] * exp2f((hi - hj.x) + (li - lj.x)) * bj.x : 0.f;
-        const float v1 = in1 ? acc[nt][2 * hrow + 1] * exp2f((hi - hj.y) + (li - lj.y)) * bj.y : 0.f;
-        if (pass == 0) {
-          *reinterpret_cast<float2*>(M + i * AM + j) = make_float2(v0, v1);
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[i][e] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        uint32_t b[XS][4];
+#pragma unroll
+        for (int s = 0; s < XS; ++s) ldsm4(b[s], at_b<RB>(k + s * PB, 16 * J, 2 * kk, lane));
+        if constexpr (XS > 1)
+#pragma unroll
+          for (int s = 0; s < XS; ++s) ldsm4(a[0][s], at_a<RB>((pass ? q : k) + s * PB, 16 * I, 2 * kk, lane));
+        mma_planes<XS, XS, XS>(d[0], d[1], a[XS == 1 ? kk : 0], b);
+      }
+      const float cIJ = g.c[4 * I + J] * sc;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const int j = 16 * J + 8 * n + q2;
+        float v[4];
+        if (J < I) {
+          const float2 bb = *reinterpret_cast<const float2*>(g.bb + j);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = d[n][e] * (ra[e >> 1] * cIJ) * (e & 1 ? bb.y : bb.x);
         } else {
-          uint32_t p[NA];
-          split2<NA>(scale * v0, scale * v1, p);
 #pragma unroll
-          for (int s = 0; s < NA; ++s)
-            asm volatile("st.shared.b32 [%0], %1;" ::"r"(aq + s * SQ_BYTES + tile_off<SQ_RB>(i, nt) + 4 * (lane % 4)),
-                         "r"(p[s]) : "memory");
+          for (int e = 0; e < 4; ++e) {
+            const int i = r0 + 8 * (e >> 1), jj = j + (e & 1);
+            const float D = exp2f((g.lh[i] - g.lh[jj]) + (g.ll[i] - g.ll[jj])) * g.beta[jj];
+            v[e] = (pass ? jj <= i : jj < i) ? d[n][e] * D * sc : 0.f;
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const int i = r0 + 8 * r;
+          if (pass == 0) {
+            *reinterpret_cast<float2*>(M + i * AM + j) = make_float2(v[2 * r], v[2 * r + 1]);
+          } else {
+            uint32_t p[NA];
+            split2<NA>(v[2 * r], v[2 * r + 1], p);
+#pragma unroll
+            for (int s = 0; s < NA; ++s)
+              asm volatile("st.shared.b32 [%0], %1;" ::"r"(aq + s * SQ_BYTES + tile_off<SQ_RB>(i, 2 * J + n) + 2 * q2),
+                           "r"(p[s]) : "memory");
+          }
         }
       }
     }
   }
   bar_sync(bar, 128);
   invert_unit_lower(M, t, bar);
-#pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    const int idx = t + it * 128, i = idx / 8, c = idx % 8;
-    if (c / 2 > i / 16) continue;
+#pragma unroll 1
+  for (int idx = t; idx < 320; idx += 128) {   // 10 blocks x 16 rows x two 8-wide pieces
+    const int blk = idx / 32, bi = blk < 1 ? 0 : blk < 3 ? 1 : blk < 6 ? 2 : 3, bj = blk - bi * (bi + 1) / 2;
+    const int i = 16 * bi + (idx % 32) / 2, c = 2 * bj + idx % 2;
     const float4 x = *reinterpret_cast<const float4*>(M + i * AM + 8 * c);
     const float4 y = *reinterpret_cast<const float4*>(M + i * AM + 8 * c + 4);
     uint32_t r[4][NTP];
