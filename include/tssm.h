@@ -471,12 +471,17 @@ int tssm_gated_delta_step(const void* x, const void* dt, void* h, const void* A_
  * beta [Bt,L,H] f32; A_log [H] f32; h0, h_last [Bt,H,P,N] f32 (either may be
  * null); N <= 128; all contiguous.  states [Bt,H,ceil(L/64),P,N] f32 (the
  * state before every 64-token chunk) and errors [Bt,L,H,P] f32 (u - hd B) are
- * what the backward reads; both null when none follows.
+ * what the backward reads; both null when none follows.  workspace:
+ * tssm_gated_delta_rule_workspace_size bytes (0 for shapes that need none),
+ * 16-byte aligned.
  */
+int64_t tssm_gated_delta_rule_workspace_size(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P,
+                                             int64_t N, int dtype);
 int tssm_gated_delta_rule(const void* u, const void* A_log, const void* B, const void* C, const void* dt,
                           const void* beta, const void* h0, void* y, void* h_last, void* states,
-                          void* errors, int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N,
-                          double scale, int dtype, tssm_stream_t stream);
+                          void* errors, void* workspace, int64_t workspace_bytes, int64_t Bt, int64_t L,
+                          int64_t H, int64_t G, int64_t P, int64_t N, double scale, int dtype,
+                          tssm_stream_t stream);
 
 /*
  * Backward of tssm_gated_delta_rule: from the same inputs, dy (as y), the

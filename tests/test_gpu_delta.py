@@ -238,12 +238,13 @@ def test_rule_refusals_without_gpu():
     lib = _lib.load_library()
     one = 4096   # a non-null address that nothing reads
 
-    def rule(Bt=2, L=3, H=4, G=2, P=8, N=16, dtype=0, u=one, states=0, errors=0):
-        return lib.tssm_gated_delta_rule(u, one, one, one, one, one, 0, one, 0, states, errors, Bt, L, H, G, P, N, 1.0,
-                                         dtype, 0)
+    def rule(Bt=2, L=3, H=4, G=2, P=8, N=16, dtype=0, u=one, states=0, errors=0, ws=0, nbytes=0):
+        return lib.tssm_gated_delta_rule(u, one, one, one, one, one, 0, one, 0, states, errors, ws, nbytes, Bt, L, H, G,
+                                         P, N, 1.0, dtype, 0)
 
     for kw in (dict(Bt=-1), dict(G=3), dict(G=0), dict(N=0), dict(N=129), dict(dtype=2), dict(u=0), dict(L=1 << 31),
-               dict(states=one), dict(errors=one)):
+               dict(states=one), dict(errors=one), dict(dtype=1, P=64, N=64),
+               dict(dtype=1, P=64, N=64, ws=one, nbytes=1000), dict(dtype=1, P=64, N=64, ws=one + 4, nbytes=1 << 30)):
         assert rule(**kw) == 1, kw
     assert rule(Bt=0) == 0
 

@@ -346,7 +346,7 @@ constexpr int SQ_RB = 128, SQ_BYTES = Q * SQ_RB;
 // above the diagonal are not written: nobody reads them.
 template <int XS, int KN, int NA, int NTP>
 __device__ __forceinline__ void chunk_matrices(uint32_t k, uint32_t q, const Gates& g, float scale, float* M,
-                                               uint32_t aq, uint32_t tp, int t, int bar) {
+                                               uint8_t* aq, uint8_t* tp, int t, int bar) {
   constexpr int RB = KN * 2, PB = Q * RB, KK = KN / 16;
   const int w = t / 32, lane = t % 32, gr = lane / 4, q2 = 2 * (lane % 4);
 #pragma unroll
@@ -402,8 +402,7 @@ __device__ __forceinline__ void chunk_matrices(uint32_t k, uint32_t q, const Gat
             split2<NA>(v[2 * r], v[2 * r + 1], p);
 #pragma unroll
             for (int s = 0; s < NA; ++s)
-              asm volatile("st.shared.b32 [%0], %1;" ::"r"(aq + s * SQ_BYTES + tile_off<SQ_RB>(i, 2 * J + n) + 2 * q2),
-                           "r"(p[s]) : "memory");
+              *reinterpret_cast<uint32_t*>(aq + s * SQ_BYTES + tile_off<SQ_RB>(i, 2 * J + n) + 2 * q2) = p[s];
           }
         }
       }
@@ -424,8 +423,8 @@ __device__ __forceinline__ void chunk_matrices(uint32_t k, uint32_t q, const Gat
     split2<NTP>(y.z, y.w, r[3]);
 #pragma unroll
     for (int s = 0; s < NTP; ++s)
-      asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(tp + s * SQ_BYTES + tile_off<SQ_RB>(i, c)),
-                   "r"(r[0][s]), "r"(r[1][s]), "r"(r[2][s]), "r"(r[3][s]) : "memory");
+      *reinterpret_cast<uint4*>(tp + s * SQ_BYTES + tile_off<SQ_RB>(i, c)) =
+          make_uint4(r[0][s], r[1][s], r[2][s], r[3][s]);
   }
 }
 

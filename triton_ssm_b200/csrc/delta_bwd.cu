@@ -81,7 +81,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(cons
     cp_async_wait_all();
     bar_sync(1, 128);
     chunk_matrices<XS, KN, 3, 3>(s + SM::K, s + SM::QQ, gt, a.scale, reinterpret_cast<float*>(smem + SM::M),
-                                 s + SM::AQ, s + SM::T, t, 1);
+                                 buf + SM::AQ, buf + SM::T, t, 1);
   };
 
   const int p0 = 16 * warp;

@@ -11,6 +11,7 @@
 // Aq are shared by the warps as right operands.  Four more warps load the next
 // chunk and build its A, T and Aq meanwhile (BUFS = 2), one barrier a chunk.
 #include "delta.cuh"
+#include "delta_tc.h"
 
 namespace tssm {
 namespace delta {
@@ -82,7 +83,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
     cp_async_wait_all();
     bar_sync(1, 128);
     chunk_matrices<XS, KN, SM::NAQ, 3>(s + SM::K, s + SM::QQ, gt, a.scale, reinterpret_cast<float*>(smem + SM::M),
-                                       s + SM::AQ, s + SM::T, t, 1);
+                                       buf + SM::AQ, buf + SM::T, t, 1);
   };
 
   // ---- chain state
@@ -333,10 +334,18 @@ int by_block(const FwdArgs& a, int64_t Bt, cudaStream_t st) {
 }  // namespace delta
 }  // namespace tssm
 
+extern "C" int64_t tssm_gated_delta_rule_workspace_size(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P,
+                                                        int64_t N, int dtype) {
+  using namespace tssm::delta;
+  if (Bt <= 0 || L <= 0 || H <= 0 || G <= 0 || P <= 0 || !tc_takes(P, N, dtype)) return 0;
+  return tc_workspace(Bt, L, H, P, N);
+}
+
 extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const void* B, const void* C, const void* dt,
                                      const void* beta, const void* h0, void* y, void* h_last, void* states,
-                                     void* errors, int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N,
-                                     double scale, int dtype, tssm_stream_t stream) {
+                                     void* errors, void* workspace, int64_t workspace_bytes, int64_t Bt, int64_t L,
+                                     int64_t H, int64_t G, int64_t P, int64_t N, double scale, int dtype,
+                                     tssm_stream_t stream) {
   using namespace tssm;
   using namespace tssm::delta;
   TSSM_REQUIRE(Bt >= 0 && L >= 0 && H >= 0 && G >= 0 && P >= 0 && N >= 0, "gated_delta_rule: negative size");
@@ -349,6 +358,20 @@ extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const voi
   TSSM_REQUIRE(dtype == TSSM_F32 || dtype == TSSM_BF16, "gated_delta_rule: dtype must be f32 or bf16 (got %d)", dtype);
   TSSM_REQUIRE(L < (int64_t(1) << 31) && Bt < (int64_t(1) << 31) && H <= 1 << 20 && P <= 1 << 20,
                "gated_delta_rule: size out of range");
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(B) |
+                          reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(y) |
+                          reinterpret_cast<uintptr_t>(h0) | reinterpret_cast<uintptr_t>(h_last) |
+                          reinterpret_cast<uintptr_t>(states) | reinterpret_cast<uintptr_t>(errors);
+  const int64_t need = tssm_gated_delta_rule_workspace_size(Bt, L, H, G, P, N, dtype);
+  TSSM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
+               "gated_delta_rule: workspace of %lld bytes (16-byte aligned) needed, %lld given", (long long)need,
+               (long long)workspace_bytes);
+  if (need && (bases & 15u) == 0) {
+    const TcCall t{u, B, C, (const float*)A_log, (const float*)dt, (const float*)beta, (const float*)h0, y,
+                   (float*)h_last, (float*)states, (float*)errors, workspace, Bt, L, H, G, P, N, (float)scale};
+    return tc_run(t, st);
+  }
   FwdArgs a{};
   a.u = u; a.B = B; a.C = C;
   a.A_log = (const float*)A_log; a.dt = (const float*)dt; a.beta = (const float*)beta; a.h0 = (const float*)h0;
@@ -359,7 +382,6 @@ extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const voi
   const int per = dtype == TSSM_F32 ? 4 : 8;   // elements of 16 bytes
   a.vec_kq = N % per == 0 && aligned16(B) && aligned16(C);
   a.vec_v = P % per == 0 && aligned16(u) && aligned16(y);
-  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   if (dtype == TSSM_F32) return N <= 64 ? by_block<3, 64, 3>(a, Bt, st) : by_block<3, 128, 3>(a, Bt, st);
   // f32 results (the state, what the backward reads) want three planes; y alone is bf16: two
   if (h_last || states) return N <= 64 ? by_block<1, 64, 3>(a, Bt, st) : by_block<1, 128, 3>(a, Bt, st);

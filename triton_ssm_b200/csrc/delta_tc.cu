@@ -1,0 +1,537 @@
+// Chunked gated delta rule, forward, on tcgen05 (bf16, N = 64 or 128, P a
+// multiple of 64; formulas and precision: delta.cuh).
+//
+// Two kernels per segment of the sequence.  The chunk matrices T and
+// Aq diag(beta) depend on no state, so delta_prep_kernel builds them for every
+// (chunk, head) of the segment at once and leaves them in HBM as the shared-memory
+// images that the scan copies.  A segment's images take about IMAGE_BYTES and are
+// written and read while they are in L2.
+//
+// delta_scan_kernel: a block carries one (batch row, head) and 128 value channels,
+// transposed: TMEM lane = value channel p, so every step of the chain stays in its
+// thread.  Per chunk
+//   KS^T = S^T K^T              A: S planes (TMEM), B: K (shared memory)
+//   X^T  = V^T - exp(l) KS^T    threads: TMEM -> registers -> X planes (TMEM)
+//   E^T  = X^T T^T              A: X planes, B: T planes, 16-column steps of the triangle
+//   S^T  = exp(l_last) S^T + (E diag(w beta))^T K   (S in f32 registers, the sum from TMEM)
+//   O^T  = scale exp(l) S^T Q^T + E^T (Aq diag(beta))^T
+// Warps: 0-7 the chain (two per 32 lanes, each half of the columns: S 64 f32 a
+// thread), 8-11 the outputs, 12 copies, 13 issues KS, E and the state update,
+// 14 issues the products of O.  The chain is serial (three products a chunk with
+// TMEM round trips between them); everything else runs beside it.
+//
+// TMEM columns: S planes [0, 192) as 96 per half (32 per plane); the state
+// update's sum lies over planes 0, 1 of its half (N = 64: over KS), the E planes for
+// O over plane 2; KS, then E [192, 256); X planes, then E diag(w beta) planes [256, 352) as 48 per
+// half; O's two sums [352, 480).  A thread overwrites only columns of its own lane
+// and half, so only the products need waiting for.
+#include <cudaTypedefs.h>
+
+#include "delta.cuh"
+#include "delta_tc.h"
+#include "tcgen05.cuh"
+#include "tmap.cuh"
+
+namespace tssm {
+namespace delta {
+namespace {
+using namespace sm100;
+
+constexpr int TILE = 8192;                       // [64 x 64] bf16
+constexpr int IMG_T = 0, IMG_AQ = 3 * SQ_BYTES, IMG_G = IMG_AQ + 2 * SQ_BYTES, IMG = IMG_G + 2 * Q * 4;
+constexpr int64_t IMAGE_BYTES = 64ll << 20;
+
+// ------------------------------------------------------------------ chunk images
+struct PrepArgs {
+  const __nv_bfloat16 *B, *C;
+  const float *A_log, *dt, *beta;
+  uint8_t* img;
+  int64_t L, c0, nseg;   // first chunk and chunks of the segment
+  int H, G, N;
+  float scale;
+};
+
+template <int KN>
+struct PrepSmem {
+  static constexpr int PLANE = Q * KN * 2;
+  static constexpr int K = 0, QQ = PLANE, M = 2 * PLANE, G = M + Q * AM * 4, BYTES = G + (int)sizeof(Gates) + 128;
+};
+
+template <int KN>
+__global__ void __launch_bounds__(128, 4) delta_prep_kernel(const PrepArgs a) {
+  using SM = PrepSmem<KN>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((128u - (smem_addr(smem_raw) & 127u)) & 127u);
+  const uint32_t s = smem_addr(smem);
+  const int t = threadIdx.x;
+  const int64_t bh = blockIdx.x / a.nseg, ci = blockIdx.x - bh * a.nseg, b = bh / a.H;
+  const int h = (int)(bh - b * a.H), g = h / (a.H / a.G);
+  const int64_t t0 = (a.c0 + ci) * Q, sk = (int64_t)a.G * a.N;
+  const int rows = (int)min((int64_t)Q, a.L - t0);
+  const int64_t at = (b * a.L + t0) * sk + (int64_t)g * a.N;
+  load_planes<1, KN, 128>(s + SM::K, 0, a.B + at, sk, rows, a.N, true, t);
+  load_planes<1, KN, 128>(s + SM::QQ, 0, a.C + at, sk, rows, a.N, true, t);
+  Gates& gt = *reinterpret_cast<Gates*>(smem + SM::G);
+  if (t < 32) gates_warp(gt, a.dt + b * a.L * a.H + h, a.beta + b * a.L * a.H + h, a.H, a.A_log[h], t0, a.L, t);
+  cp_async_wait_all();
+  __syncthreads();
+  uint8_t* img = a.img + (bh * a.nseg + ci) * IMG;
+  float* go = reinterpret_cast<float*>(img + IMG_G);
+  go[t] = t < Q ? gt.eg[t] : gt.wb[t - Q];
+  chunk_matrices<1, KN, 2, 3>(s + SM::K, s + SM::QQ, gt, a.scale, reinterpret_cast<float*>(smem + SM::M), img + IMG_AQ,
+                              img + IMG_T, t, 1);
+}
+
+// ------------------------------------------------------------------ the scan
+struct ScanArgs {
+  const uint8_t* img;
+  const float* h_in;
+  float *h_out, *states, *errs;
+  int* status;
+  int64_t L, c0, nseg, nc;
+  int H, G, P, N, npb;
+  float scale;
+};
+
+template <int KN>
+struct ScanSmem {
+  static constexpr int NB = KN / 64;   // 64-wide blocks of K, Q
+  static constexpr int K = 0, QQ = K + NB * TILE, V = QQ + NB * TILE, IM = V + 2 * TILE,
+                       STAGE = (IM + IMG + 1023) / 1024 * 1024;
+  static constexpr int Y = 2 * STAGE, BAR = Y + 2 * TILE, BYTES = BAR + 256 + 1024;
+  static_assert(BYTES <= 232448, "shared-memory layout exceeds the per-block limit");
+};
+
+constexpr uint32_t C_KE = 192, C_XP = 256, C_O1 = 352, C_O2 = 416;
+
+// D (+)= A B with A in TMEM: row m in lane m, 16 bf16 of k in 8 columns.
+__device__ __forceinline__ void umma_bf16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+      "r"((uint32_t)acc)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st8u(uint32_t taddr, const uint32_t (&u)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(u[0]),
+               "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
+               : "memory");
+}
+// 16 values as NS planes of 8 columns, plane s at taddr + s * step (r is used up).
+template <int NS>
+__device__ __forceinline__ void store_planes(uint32_t taddr, uint32_t step, float (&r)[16]) {
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    uint32_t u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      u[i] = pack2(r[2 * i], r[2 * i + 1]);
+      if (s + 1 < NS) {
+        r[2 * i] -= lo2(u[i]);
+        r[2 * i + 1] -= hi2(u[i]);
+      }
+    }
+    tmem_st8u(taddr + s * step, u);
+  }
+}
+
+// NS: planes of the state and of X, E (3 when an f32 result is asked for, else 2).
+template <int KN, int NS>
+__global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constant__ CUtensorMap tm_k,
+                                                            const __grid_constant__ CUtensorMap tm_q,
+                                                            const __grid_constant__ CUtensorMap tm_u,
+                                                            const __grid_constant__ CUtensorMap tm_y, const ScanArgs a) {
+  using SM = ScanSmem<KN>;
+  constexpr int NB = SM::NB, HN = KN / 2;   // HN: state columns of a thread
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t bh = blockIdx.x / a.npb;
+  const int pb = (int)(blockIdx.x - bh * a.npb) * 128;
+  const int b = (int)(bh / a.H), h = (int)(bh - (int64_t)b * a.H), g = h / (a.H / a.G);
+  const int boxes = min(2, (a.P - pb) / 64);   // 64-channel boxes of this block
+  const int n = (int)a.nseg;
+
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + SM::BAR);
+  uint64_t *full = bar, *empty = bar + 2;      // [2] stage loaded / released
+  uint64_t *sready = bar + 4, *ksdone = bar + 5, *xready = bar + 6, *edone = bar + 7, *eready = bar + 8,
+           *dsdone = bar + 9, *qdone = bar + 10, *odone = bar + 11, *ofree = bar + 12, *drain = bar + 13;   // drain [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::BAR + 128);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + SM::BAR + 132);
+  int* issued = reinterpret_cast<int*>(smem + SM::BAR + 136);
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 2 + 8 + 4);   // two issuers' commits, chain and output warps
+      mbar_init(&drain[i], 1);
+    }
+    mbar_init(sready, 8);
+    mbar_init(xready, 8);
+    mbar_init(eready, 8);
+    mbar_init(ofree, 4);
+    mbar_init(ksdone, 1);
+    mbar_init(edone, 1);
+    mbar_init(dsdone, 1);
+    mbar_init(qdone, 1);
+    mbar_init(odone, 1);
+    *abort_flag = 0;
+    *issued = 0;
+    fence_mbar_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  auto stage = [&](int c) { return smem + (c & 1) * SM::STAGE; };
+  auto fail = [&](int code) {
+    *abort_flag = 1;
+    atomicExch(a.status, code);
+  };
+  // A wait by one thread (issuers, copies); false: give up.
+  auto wait1 = [&](uint64_t* m, int phase, int code) {
+    if (mbar_wait(m, phase & 1, abort_flag)) return true;
+    if (!*abort_flag) fail(code);
+    return false;
+  };
+  // A wait by a whole warp: every lane takes the same decision.
+  auto waitw = [&](uint64_t* m, int phase, int code) {
+    const bool ok = mbar_wait(m, phase & 1, abort_flag);
+    if (__all_sync(0xffffffffu, ok)) return true;
+    if (lane == 0 && !*abort_flag) fail(code);
+    return false;
+  };
+  auto arrive_warp = [&](uint64_t* m) {   // this warp's TMEM accesses before it are ordered before the arrival
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(m);
+  };
+
+  if (warp < 8) {
+    // ================================================================ the chain
+    const int half = warp >> 2, p = (warp & 3) * 32 + lane;   // value channel = TMEM lane
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const bool live = p < boxes * 64;
+    const int64_t row = (bh * a.P + pb + p) * (int64_t)a.N + half * HN;   // of h_in, h_out
+    float S[HN];
+#pragma unroll
+    for (int j = 0; j < HN; j += 4) {
+      const float4 v = live && a.h_in ? *reinterpret_cast<const float4*>(a.h_in + row + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+      S[j] = v.x; S[j + 1] = v.y; S[j + 2] = v.z; S[j + 3] = v.w;
+    }
+    bool ok = true;
+    for (int c = 0; c < n; ++c) {
+      if (a.states && live) {
+        float* dst = a.states + ((bh * a.nc + a.c0 + c) * a.P + pb + p) * (int64_t)a.N + half * HN;
+#pragma unroll
+        for (int j = 0; j < HN; j += 4) *reinterpret_cast<float4*>(dst + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+      }
+      // O's product of the chunk before has read the E planes that lie over plane 2
+      if (c > 0 && !waitw(odone, c - 1, 2001)) { ok = false; break; }
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < HN / 16; ++i) {
+        float r[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = S[16 * i + j];
+        store_planes<NS>(tl + 96 * half + 8 * i, 32, r);
+      }
+      tmem_wait_st();
+      arrive_warp(sready);
+      // X^T = V^T - exp(l) KS^T, 32 tokens of this half
+      const uint8_t* st = stage(c);
+      if (!waitw(&full[c & 1], c >> 1, 2002) || !waitw(ksdone, c, 2003)) { ok = false; break; }
+      tc_fence_after();
+      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_G);
+      const float* wb = eg + Q;
+      const __nv_bfloat16* vs = reinterpret_cast<const __nv_bfloat16*>(st + SM::V + (p >> 6) * TILE) + (p & 63) + half * 32 * 64;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x[16];
+        tmem_ld16(tl + C_KE + 32 * half + 16 * i, x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 e4 = *reinterpret_cast<const float4*>(eg + 32 * half + 16 * i + j);
+          const __nv_bfloat16* v = vs + (16 * i + j) * 64;
+          x[j] = __bfloat162float(v[0]) - e4.x * x[j];
+          x[j + 1] = __bfloat162float(v[64]) - e4.y * x[j + 1];
+          x[j + 2] = __bfloat162float(v[128]) - e4.z * x[j + 2];
+          x[j + 3] = __bfloat162float(v[192]) - e4.w * x[j + 3];
+        }
+        store_planes<NS>(tl + C_XP + 48 * half + 8 * i, 16, x);
+      }
+      tmem_wait_st();
+      arrive_warp(xready);
+      // E^T: planes of E for O, of E diag(w beta) for the state
+      if (!waitw(edone, c, 2004)) { ok = false; break; }
+      tc_fence_after();
+      const float el = eg[Q - 1];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x[16], r[16];
+        tmem_ld16(tl + C_KE + 32 * half + 16 * i, x);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 w4 = *reinterpret_cast<const float4*>(wb + 32 * half + 16 * i + j);
+          r[j] = x[j] * w4.x;
+          r[j + 1] = x[j + 1] * w4.y;
+          r[j + 2] = x[j + 2] * w4.z;
+          r[j + 3] = x[j + 3] * w4.w;
+        }
+        store_planes<NS>(tl + C_XP + 48 * half + 8 * i, 16, r);
+        if (a.errs && live) {
+          const int64_t tk = (a.c0 + c) * Q + 32 * half + 16 * i;
+          float* ep = a.errs + ((b * a.L + tk) * a.H + h) * (int64_t)a.P + pb + p;
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            if (tk + j < a.L) ep[(int64_t)j * a.H * a.P] = x[j];
+        }
+        store_planes<2>(tl + 96 * half + 64 + 8 * i, 16, x);
+      }
+      tmem_wait_st();
+      arrive_warp(eready);
+      if (lane == 0) mbar_arrive(&empty[c & 1]);   // V and the gates are read (arrive_warp synchronised the warp)
+      // S^T
+      if (!waitw(dsdone, c, 2005)) { ok = false; break; }
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < HN / 16; ++i) {
+        float d[16];
+        tmem_ld16(tl + (NB == 2 ? 96 * half : C_KE + 32 * half) + 16 * i, d);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) S[16 * i + j] = el * S[16 * i + j] + d[j];
+      }
+    }
+    if (ok && a.h_out && live) {
+#pragma unroll
+      for (int j = 0; j < HN; j += 4)
+        *reinterpret_cast<float4*>(a.h_out + row + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+    }
+  } else if (warp < 12) {
+    // ================================================================ outputs
+    const int w = warp - 8, p = w * 32 + lane;
+    const uint32_t tl = tmem + ((uint32_t)(w * 32) << 16);
+    for (int c = 0; c < n; ++c) {
+      const uint8_t* st = stage(c);
+      const bool bad = !waitw(&full[c & 1], c >> 1, 2006) || !waitw(odone, c, 2007);   // odone: both products
+      if (tid == 256 && c > 0) bulk_wait_read<0>();   // the last chunk's store has left the tile
+      if (named_bar_or(1, 128, bad)) break;
+      tc_fence_after();
+      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_G);
+      __nv_bfloat16* ys = reinterpret_cast<__nv_bfloat16*>(smem + SM::Y + (p >> 6) * TILE) + (p & 63);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float o1[16], o2[16];
+        tmem_ld16(tl + C_O1 + 16 * i, o1);
+        tmem_ld16(tl + C_O2 + 16 * i, o2);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          ys[(16 * i + j) * 64] = __float2bfloat16_rn(a.scale * eg[16 * i + j] * o1[j] + o2[j]);
+      }
+      arrive_warp(ofree);
+      if (lane == 0) mbar_arrive(&empty[c & 1]);
+      fence_proxy_async_smem();
+      named_bar_sync(1, 128);
+      if (tid == 256) {
+        for (int x = 0; x < boxes; ++x)   // rows past L are clipped by the map
+          tma_store_3d(&tm_y, smem + SM::Y + x * TILE, h * a.P + pb + 64 * x, (int)(a.c0 + c) * Q, b);
+        bulk_commit();
+      }
+    }
+    if (tid == 256) bulk_wait<0>();
+  } else {
+    if (warp == 12 && lane == 0) {
+      // ============================================================== copies
+      int c = 0;
+      const uint32_t bytes = 2 * NB * TILE + boxes * TILE + IMG;
+      for (; c < n; ++c) {
+        if (c >= 2 && !wait1(&empty[c & 1], (c >> 1) - 1, 2008)) break;
+        uint8_t* st = stage(c);
+        uint64_t* f = &full[c & 1];
+        const int t0 = (int)(a.c0 + c) * Q;
+        mbar_arrive_expect_tx(f, bytes);
+        for (int x = 0; x < NB; ++x) {
+          tma_load_3d(st + SM::K + x * TILE, &tm_k, g * a.N + 64 * x, t0, b, f);
+          tma_load_3d(st + SM::QQ + x * TILE, &tm_q, g * a.N + 64 * x, t0, b, f);
+        }
+        for (int x = 0; x < boxes; ++x) tma_load_3d(st + SM::V + x * TILE, &tm_u, h * a.P + pb + 64 * x, t0, b, f);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                         smem_u32(st + SM::IM)),
+                     "l"(a.img + (bh * a.nseg + c) * IMG), "r"(IMG), "r"(smem_u32(f))
+                     : "memory");
+        *issued = c + 1;
+      }
+    } else if (warp == 13 && lane == 0) {
+      // ============================================================== KS, E, state update
+      constexpr uint32_t ID_K = make_idesc_bf16(128, 64, false, false), ID_MN = make_idesc_bf16(128, 64, false, true);
+      for (int c = 0; c < n; ++c) {
+        const uint32_t st = smem_u32(stage(c));
+        if (!wait1(&full[c & 1], c >> 1, 2009) || !wait1(sready, c, 2010)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int s = NS - 1; s >= 0; --s)
+#pragma unroll
+          for (int kk = 0; kk < KN / 16; ++kk) {
+            const int hf = kk / (HN / 16), ko = kk % (HN / 16);
+            umma_bf16_ta(tmem + C_KE, tmem + 96 * hf + 32 * s + 8 * ko,
+                         make_desc_sw128(st + SM::K + (kk / 4) * TILE, 16) + 2 * (kk & 3), ID_K, s != NS - 1 || kk);
+          }
+        umma_commit(ksdone);
+        if (!wait1(xready, c, 2011)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint32_t id = make_idesc_bf16(128, 64 - 16 * t, false, false);
+#pragma unroll
+          for (int o = NS - 1; o >= 0; --o)
+#pragma unroll
+            for (int s = 0; s <= o; ++s)
+              umma_bf16_ta(tmem + C_KE + 16 * t, tmem + C_XP + 48 * (t >> 1) + 16 * s + 8 * (t & 1),
+                           make_desc_sw128(st + SM::IM + IMG_T + (o - s) * SQ_BYTES, 16) + 128 * t + 2 * t, id,
+                           t || o != NS - 1 || s);
+        }
+        umma_commit(edone);
+        if (!wait1(eready, c, 2012) || !wait1(qdone, c, 2013)) break;   // O's first product has read S planes 0, 1
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < NB; ++x)
+#pragma unroll
+          for (int s = NS - 1; s >= 0; --s)
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              umma_bf16_ta(tmem + (NB == 2 ? 96 * x : C_KE), tmem + C_XP + 48 * (t >> 1) + 16 * s + 8 * (t & 1),
+                           make_desc_sw128(st + SM::K + x * TILE, TILE) + 128 * t, ID_MN, s != NS - 1 || t);
+        umma_commit(dsdone);
+        umma_commit(&empty[c & 1]);
+      }
+      umma_commit(&drain[0]);
+      mbar_wait(&drain[0], 0, nullptr, 100000000ull);
+    } else if (warp == 14 && lane == 0) {
+      // ============================================================== O
+      constexpr uint32_t ID_K = make_idesc_bf16(128, 64, false, false);
+      for (int c = 0; c < n; ++c) {
+        const uint32_t st = smem_u32(stage(c));
+        if (!wait1(&full[c & 1], c >> 1, 2014) || !wait1(sready, c, 2015) || (c > 0 && !wait1(ofree, c - 1, 2016))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int s = 1; s >= 0; --s)
+#pragma unroll
+          for (int kk = 0; kk < KN / 16; ++kk) {
+            const int hf = kk / (HN / 16), ko = kk % (HN / 16);
+            umma_bf16_ta(tmem + C_O1, tmem + 96 * hf + 32 * s + 8 * ko,
+                         make_desc_sw128(st + SM::QQ + (kk / 4) * TILE, 16) + 2 * (kk & 3), ID_K, s != 1 || kk);
+          }
+        umma_commit(qdone);
+        if (!wait1(eready, c, 2017)) break;
+        tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint32_t id = make_idesc_bf16(128, 64 - 16 * t, false, false);
+#pragma unroll
+          for (int o = 1; o >= 0; --o)
+#pragma unroll
+            for (int s = 0; s <= o; ++s)
+              umma_bf16_ta(tmem + C_O2 + 16 * t, tmem + 96 * (t >> 1) + 64 + 16 * s + 8 * (t & 1),
+                           make_desc_sw128(st + SM::IM + IMG_AQ + (o - s) * SQ_BYTES, 16) + 128 * t + 2 * t, id,
+                           t || o != 1 || s);
+        }
+        umma_commit(odone);
+        umma_commit(&empty[c & 1]);
+      }
+      umma_commit(&drain[1]);
+      mbar_wait(&drain[1], 0, nullptr, 100000000ull);
+    }
+  }
+  // ================================================================ teardown
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort_flag)   // copies that were started land before the block leaves
+    for (int c = max(0, *issued - 2); c < *issued; ++c) mbar_wait(&full[c & 1], (c >> 1) & 1, nullptr, 100000000ull);
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+bool map_bf16(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, bool swizzle) {
+  auto fn = tmap_encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[3] = {d0, d1, d2};
+  cuuint64_t strides[2] = {d0 * 2, d0 * d1 * 2};
+  cuuint32_t box[3] = {64, 64, 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int64_t segment_chunks(int64_t streams, int64_t nc) {
+  return std::max<int64_t>(1, std::min(nc, IMAGE_BYTES / (streams * IMG)));
+}
+
+template <int KN, int NS>
+int run(const TcCall& a, cudaStream_t st) {
+  const int64_t streams = a.Bt * a.H, nc = cdiv(a.L, Q), seg = segment_chunks(streams, nc);
+  CUtensorMap mk, mq, mu, my;
+  if (!map_bf16(&mk, a.B, a.G * a.N, a.L, a.Bt, true) || !map_bf16(&mq, a.C, a.G * a.N, a.L, a.Bt, true) ||
+      !map_bf16(&mu, a.u, a.H * a.P, a.L, a.Bt, false) || !map_bf16(&my, a.y, a.H * a.P, a.L, a.Bt, false)) {
+    set_error("gated_delta_rule: cuTensorMapEncodeTiled failed");
+    return TSSM_ERR_CUDA;
+  }
+  int* status = device_status_ptr();
+  if (!status) {
+    set_error("gated_delta_rule: device status word unavailable");
+    return TSSM_ERR_CUDA;
+  }
+  auto prep = delta_prep_kernel<KN>;
+  auto scan = delta_scan_kernel<KN, NS>;
+  if (cudaFuncSetAttribute(prep, cudaFuncAttributeMaxDynamicSharedMemorySize, PrepSmem<KN>::BYTES) != cudaSuccess ||
+      cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem<KN>::BYTES) != cudaSuccess)
+    return check_launch("gated_delta_rule: set smem attribute");
+  uint8_t* img = (uint8_t*)a.ws;
+  float* carry = a.h_last ? a.h_last : (float*)(img + streams * seg * IMG);
+  for (int64_t c0 = 0; c0 < nc; c0 += seg) {
+    const int64_t m = std::min(seg, nc - c0);
+    const PrepArgs p{(const __nv_bfloat16*)a.B, (const __nv_bfloat16*)a.C, a.A_log, a.dt, a.beta, img, a.L, c0, m,
+                     (int)a.H, (int)a.G, (int)a.N, a.scale};
+    prep<<<(unsigned)(streams * m), 128, PrepSmem<KN>::BYTES, st>>>(p);
+    const bool last = c0 + m == nc;
+    const ScanArgs s{img, c0 ? carry : a.h0, last && !a.h_last ? nullptr : carry, a.states, a.errs, status, a.L, c0, m,
+                     nc, (int)a.H, (int)a.G, (int)a.P, (int)a.N, (int)cdiv(a.P, 128), a.scale};
+    scan<<<(unsigned)(streams * s.npb), 512, ScanSmem<KN>::BYTES, st>>>(mk, mq, mu, my, s);
+  }
+  return check_launch("gated_delta_rule");
+}
+
+}  // namespace
+
+bool tc_takes(int64_t P, int64_t N, int dtype) {
+  return dtype == TSSM_BF16 && (N == 64 || N == 128) && P % 64 == 0;
+}
+
+int64_t tc_workspace(int64_t Bt, int64_t L, int64_t H, int64_t P, int64_t N) {
+  const int64_t streams = Bt * H, nc = cdiv(L, Q), seg = segment_chunks(streams, nc);
+  return streams * seg * IMG + (seg < nc ? streams * P * N * 4 : 0);
+}
+
+int tc_run(const TcCall& a, cudaStream_t st) {
+  TSSM_REQUIRE(a.Bt * a.H * std::max(cdiv(a.P, 128), segment_chunks(a.Bt * a.H, cdiv(a.L, Q))) < (int64_t(1) << 31) &&
+                   a.H * a.P < (int64_t(1) << 31) && a.G * a.N < (int64_t(1) << 31),
+               "gated_delta_rule: size out of range");
+  const bool f32_out = a.h_last || a.states;
+  if (a.N == 64) return f32_out ? run<64, 3>(a, st) : run<64, 2>(a, st);
+  return f32_out ? run<128, 3>(a, st) : run<128, 2>(a, st);
+}
+
+}  // namespace delta
+}  // namespace tssm

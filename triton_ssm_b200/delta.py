@@ -43,6 +43,13 @@ def _rule_args(name, u, A_log, B, C, dt, beta, h0):
     return Bt, L, H, G, P, N
 
 
+def _dense(t):
+    """t contiguous and on a 16-byte boundary (a view at an odd offset is copied: the copies
+    that the kernels make by hardware start there)."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def gated_delta_rule(u, A_log, B, C, dt, beta, scale=1.0, h0=None, return_state=False, save=False, y=None):
     """The gated delta rule over whole sequences.
 
@@ -57,9 +64,9 @@ def gated_delta_rule(u, A_log, B, C, dt, beta, scale=1.0, h0=None, return_state=
     """
     _cuda(u, A_log, B, C, dt, beta, h0, y)
     Bt, L, H, G, P, N = _rule_args("gated_delta_rule", u, A_log, B, C, dt, beta, h0)
-    u, B, C = u.contiguous(), B.contiguous(), C.contiguous()
+    u, B, C = _dense(u), _dense(B), _dense(C)
     A_log, dt, beta = (t.float().contiguous() for t in (A_log, dt, beta))
-    h0 = h0.float().contiguous() if h0 is not None else None
+    h0 = _dense(h0.float()) if h0 is not None else None
     if y is None:
         y = torch.empty_like(u)
     elif y.shape != u.shape or y.dtype != u.dtype or not y.is_contiguous():
@@ -68,9 +75,11 @@ def gated_delta_rule(u, A_log, B, C, dt, beta, scale=1.0, h0=None, return_state=
     hl = torch.empty(Bt, H, P, N, **f32) if return_state else None
     states = torch.empty(Bt, H, -(-L // CHUNK), P, N, **f32) if save else None
     errors = torch.empty(Bt, L, H, P, **f32) if save else None
+    need = int(_lib.load_library().tssm_gated_delta_rule_workspace_size(Bt, L, H, G, P, N, dtype_code(u)))
+    ws = torch.empty(need, dtype=torch.uint8, device=u.device) if need else None
     with device_of(u):
         call("tssm_gated_delta_rule", ptr(u), ptr(A_log), ptr(B), ptr(C), ptr(dt), ptr(beta), ptr(h0), ptr(y), ptr(hl),
-             ptr(states), ptr(errors), Bt, L, H, G, P, N, float(scale), dtype_code(u), stream_of(u))
+             ptr(states), ptr(errors), ptr(ws), need, Bt, L, H, G, P, N, float(scale), dtype_code(u), stream_of(u))
     out = [y]
     if return_state:
         out.append(hl)
@@ -96,9 +105,9 @@ def gated_delta_rule_bwd(u, A_log, B, C, dt, beta, dy, saved, scale=1.0, dh_last
     for t, shape in ((states, (Bt, H, -(-L // CHUNK), P, N)), (errors, (Bt, L, H, P))):
         if tuple(t.shape) != shape or t.dtype != torch.float32 or not t.is_contiguous():
             raise ValueError("gated_delta_rule_bwd: saved must be what gated_delta_rule(..., save=True) returned")
-    u, B, C, dy = u.contiguous(), B.contiguous(), C.contiguous(), dy.contiguous()
+    u, B, C, dy = _dense(u), _dense(B), _dense(C), _dense(dy)
     A_log, dt, beta = (t.float().contiguous() for t in (A_log, dt, beta))
-    dh_last = dh_last.float().contiguous() if dh_last is not None else None
+    dh_last = _dense(dh_last.float()) if dh_last is not None else None
     f32 = dict(device=u.device, dtype=torch.float32)
     du, dB, dC, dA_log = torch.empty_like(u), torch.empty_like(B), torch.empty_like(C), torch.empty_like(A_log)
     ddt, dbeta, dh0 = torch.empty_like(dt), torch.empty_like(beta), torch.empty(Bt, H, P, N, **f32)
