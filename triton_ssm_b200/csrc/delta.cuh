@@ -51,16 +51,21 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
 __device__ __forceinline__ float lo2(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float hi2(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// x, y -= the bf16 pair h (exactly: the mixed-precision FMA reads bf16 operands, which saves
+// the shifts and masks; 13 instead of 16 cycles per pair split into three planes).
+__device__ __forceinline__ void sub2(float& x, float& y, uint32_t h) {
+  asm("{\n\t.reg .b16 l, u, m;\n\tmov.b32 {l, u}, %2;\n\tmov.b16 m, 0xBF80;\n\t"
+      "fma.rn.f32.bf16 %0, l, m, %0;\n\tfma.rn.f32.bf16 %1, u, m, %1;\n\t}"
+      : "+f"(x), "+f"(y) : "r"(h));
+}
+
 // (x, y) as NS bf16 pairs whose sum is exact to 8 NS bits.
 template <int NS>
 __device__ __forceinline__ void split2(float x, float y, uint32_t (&r)[NS]) {
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     r[s] = pack2(x, y);
-    if (s + 1 < NS) {
-      x -= lo2(r[s]);
-      y -= hi2(r[s]);
-    }
+    if (s + 1 < NS) sub2(x, y, r[s]);
   }
 }
 // The A operand (16 rows x 16 k) of two adjacent 16 x 8 result tiles: results feed the

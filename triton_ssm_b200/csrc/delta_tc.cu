@@ -14,17 +14,22 @@
 //   X^T  = V^T - exp(l) KS^T    threads: TMEM -> registers -> X planes (TMEM)
 //   E^T  = X^T T^T              A: X planes, B: T planes, 16-column steps of the triangle
 //   S^T  = exp(l_last) S^T + (E diag(w beta))^T K   (S in f32 registers, the sum from TMEM)
-//   O^T  = scale exp(l) S^T Q^T + E^T (Aq diag(beta))^T
-// Warps: 0-7 the chain (two per 32 lanes, each half of the columns: S 64 f32 a
-// thread), 8-11 the outputs, 12 copies, 13 issues KS, E and the state update,
-// 14 issues the products of O.  The chain is serial (three products a chunk with
-// TMEM round trips between them); everything else runs beside it.
+//   O^T  = scale exp(l) S^T Q^T + E^T (Aq diag(beta))^T   (two planes: y is bf16)
+// Warps: 0 issues the chain's products, 2 those of O, 1 copies, 4-11 are the chain (two
+// per 32 lanes, each half of the columns: S 64 f32 a thread), 12-15 the outputs.  The
+// chain is serial, so its latency counts: pieces of its operands are handed over as
+// they are written, by named barriers (a hand-over through an mbarrier measured 136
+// cycles, through a barrier 25), and a product runs while the next piece is split.
+// tcgen05 takes 32 cycles per 128 x 64 x 16 and 190 from issue to a thread that waits.
 //
-// TMEM columns: S planes [0, 192) as 96 per half (32 per plane); the state
-// update's sum lies over planes 0, 1 of its half (N = 64: over KS), the E planes for
-// O over plane 2; KS, then E [192, 256); X planes, then E diag(w beta) planes [256, 352) as 48 per
-// half; O's two sums [352, 480).  A thread overwrites only columns of its own lane
-// and half, so only the products need waiting for.
+// TMEM columns: [0, 192) S planes (planes 0, 1 of a half side by side, then both plane
+// 2s), later the state update's sum over planes 0, 1.  [192, 256) KS, then E.
+// [256, 352) X planes, then E diag(w beta) planes, 48 per half.  [352, 416) E's two
+// planes for O.  [416, 480) QS, then Aq diag(beta) E.  A thread overwrites columns of
+// its own lane and half only, so only products are waited for.
+//
+// Every wait on an mbarrier is bounded.  A warp that gives up sets the abort flag and
+// goes on without waiting, storing nothing: the named barriers' counts stay whole.
 #include <cudaTypedefs.h>
 
 #include "delta.cuh"
@@ -96,14 +101,21 @@ struct ScanArgs {
 template <int KN>
 struct ScanSmem {
   static constexpr int NB = KN / 64;   // 64-wide blocks of K, Q
-  static constexpr int K = 0, QQ = K + NB * TILE, V = QQ + NB * TILE, IM = V + 2 * TILE,
-                       STAGE = (IM + IMG + 1023) / 1024 * 1024;
+  static constexpr int K = 0, QQ = K + NB * TILE, V = QQ + NB * TILE, IM = V + 2 * TILE, STAGE = (IM + IMG + 1023) / 1024 * 1024;
   static constexpr int Y = 2 * STAGE, BAR = Y + 2 * TILE, BYTES = BAR + 256 + 1024;
   static_assert(BYTES <= 232448, "shared-memory layout exceeds the per-block limit");
 };
 
-constexpr uint32_t C_KE = 192, C_XP = 256, C_O1 = 352, C_O2 = 416;
+constexpr uint32_t C_KE = 192, C_XP = 256, C_EO = 352, C_O = 416;
+// named barriers (0: __syncthreads): outputs; pieces of S, X, E diag(w beta), E for their issuers
+constexpr uint32_t B_OUT = 1, B_S = 2, B_X = 6, B_W = 8, B_E = 10, B_ISSUE = 256 + 32;
 
+// One lane of a converged warp (always the same one).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
+  return e != 0;
+}
 // D (+)= A B with A in TMEM: row m in lane m, 16 bf16 of k in 8 columns.
 __device__ __forceinline__ void umma_bf16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
@@ -113,27 +125,40 @@ __device__ __forceinline__ void umma_bf16_ta(uint32_t d, uint32_t a, uint64_t b,
       "r"((uint32_t)acc)
       : "memory");
 }
+// A wait on the chain's path: a few short hardware-timed waits (a round trip through a
+// test_wait loop measured 272 cycles, through try_wait 237, and a waiting warp takes no
+// issue slots from the working ones), then as mbar_wait.
+__device__ __forceinline__ bool mbar_wait_hot(uint64_t* m, uint32_t parity, const volatile int* abort_flag) {
+  for (int i = 0; i < 64; ++i)
+    if (mbar_try_wait(m, parity, 20000u)) return true;
+  if (*abort_flag) return false;
+  return mbar_wait_slow(m, parity, abort_flag, 2000000000ull);
+}
 __device__ __forceinline__ void tmem_st8u(uint32_t taddr, const uint32_t (&u)[8]) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(u[0]),
                "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
                : "memory");
 }
-// 16 values as NS planes of 8 columns, plane s at taddr + s * step (r is used up).
+// 16 values as NS planes of 8 columns, plane s at taddr[s] (r is used up).
 template <int NS>
-__device__ __forceinline__ void store_planes(uint32_t taddr, uint32_t step, float (&r)[16]) {
+__device__ __forceinline__ void store_planes(const uint32_t (&taddr)[NS], float (&r)[16]) {
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     uint32_t u[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       u[i] = pack2(r[2 * i], r[2 * i + 1]);
-      if (s + 1 < NS) {
-        r[2 * i] -= lo2(u[i]);
-        r[2 * i + 1] -= hi2(u[i]);
-      }
+      if (s + 1 < NS) sub2(r[2 * i], r[2 * i + 1], u[i]);
     }
-    tmem_st8u(taddr + s * step, u);
+    tmem_st8u(taddr[s], u);
   }
+}
+template <int NS>
+__device__ __forceinline__ void store_planes(uint32_t taddr, uint32_t step, float (&r)[16]) {
+  uint32_t at[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) at[s] = taddr + s * step;
+  store_planes<NS>(at, r);
 }
 
 // NS: planes of the state and of X, E (3 when an f32 result is asked for, else 2).
@@ -155,21 +180,19 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
 
   uint64_t* bar = reinterpret_cast<uint64_t*>(smem + SM::BAR);
   uint64_t *full = bar, *empty = bar + 2;      // [2] stage loaded / released
-  uint64_t *sready = bar + 4, *ksdone = bar + 5, *xready = bar + 6, *edone = bar + 7, *eready = bar + 8,
-           *dsdone = bar + 9, *qdone = bar + 10, *odone = bar + 11, *ofree = bar + 12, *drain = bar + 13;   // drain [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::BAR + 128);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + SM::BAR + 132);
-  int* issued = reinterpret_cast<int*>(smem + SM::BAR + 136);
+  uint64_t *ksdone = bar + 4, *edone = bar + 5, *dsdone = bar + 6, *qdone = bar + 7, *odone = bar + 8, *qread = bar + 9,
+           *oread = bar + 10, *drain = bar + 11;   // drain [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::BAR + 192);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + SM::BAR + 196);
+  int* issued = reinterpret_cast<int*>(smem + SM::BAR + 200);
   if (tid == 0) {
     for (int i = 0; i < 2; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 2 + 8 + 4);   // two issuers' commits, chain and output warps
       mbar_init(&drain[i], 1);
     }
-    mbar_init(sready, 8);
-    mbar_init(xready, 8);
-    mbar_init(eready, 8);
-    mbar_init(ofree, 4);
+    mbar_init(qread, 4);
+    mbar_init(oread, 4);
     mbar_init(ksdone, 1);
     mbar_init(edone, 1);
     mbar_init(dsdone, 1);
@@ -179,7 +202,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
     *issued = 0;
     fence_mbar_init();
   }
-  if (warp == 0) {
+  if (warp == 1) {
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
@@ -193,15 +216,10 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
     *abort_flag = 1;
     atomicExch(a.status, code);
   };
-  // A wait by one thread (issuers, copies); false: give up.
-  auto wait1 = [&](uint64_t* m, int phase, int code) {
-    if (mbar_wait(m, phase & 1, abort_flag)) return true;
-    if (!*abort_flag) fail(code);
-    return false;
-  };
-  // A wait by a whole warp: every lane takes the same decision.
+  // A wait by a whole warp: every lane takes the same decision; false: give up.
   auto waitw = [&](uint64_t* m, int phase, int code) {
-    const bool ok = mbar_wait(m, phase & 1, abort_flag);
+    const bool ok = mbar_wait_hot(m, phase & 1, abort_flag);
+    tc_fence_after();
     if (__all_sync(0xffffffffu, ok)) return true;
     if (lane == 0 && !*abort_flag) fail(code);
     return false;
@@ -211,10 +229,21 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
     __syncwarp();
     if (lane == 0) mbar_arrive(m);
   };
+  auto hand_over = [&](uint32_t b) {      // TMEM stores of a piece -> its issuer
+    tmem_wait_st();
+    tc_fence_before();
+    named_bar_arrive(b, B_ISSUE);
+  };
+  auto take = [&](uint32_t b) {
+    named_bar_sync(b, B_ISSUE);
+    tc_fence_after();
+  };
+  // first column of plane s of a half of the state
+  auto plane = [](int s, int hf) { return (uint32_t)(s < 2 ? HN * hf + (HN / 2) * s : KN + (HN / 2) * hf); };
 
-  if (warp < 8) {
+  if (warp >= 4 && warp < 12) {
     // ================================================================ the chain
-    const int half = warp >> 2, p = (warp & 3) * 32 + lane;   // value channel = TMEM lane
+    const int half = (warp >> 2) - 1, p = (warp & 3) * 32 + lane;   // value channel = TMEM lane
     const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const bool live = p < boxes * 64;
     const int64_t row = (bh * a.P + pb + p) * (int64_t)a.N + half * HN;   // of h_in, h_out
@@ -226,30 +255,35 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
     }
     bool ok = true;
     for (int c = 0; c < n; ++c) {
-      if (a.states && live) {
-        float* dst = a.states + ((bh * a.nc + a.c0 + c) * a.P + pb + p) * (int64_t)a.N + half * HN;
-#pragma unroll
-        for (int j = 0; j < HN; j += 4) *reinterpret_cast<float4*>(dst + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
-      }
-      // O's product of the chunk before has read the E planes that lie over plane 2
-      if (c > 0 && !waitw(odone, c - 1, 2001)) { ok = false; break; }
-      tc_fence_after();
+      // S planes, 16 columns of the half at a time
 #pragma unroll
       for (int i = 0; i < HN / 16; ++i) {
         float r[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) r[j] = S[16 * i + j];
-        store_planes<NS>(tl + 96 * half + 8 * i, 32, r);
+        uint32_t at[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) at[s] = tl + plane(s, half) + 8 * i;
+        store_planes<NS>(at, r);
+        hand_over(B_S + i);
       }
-      tmem_wait_st();
-      arrive_warp(sready);
-      // X^T = V^T - exp(l) KS^T, 32 tokens of this half
+      if (a.states && live && ok) {
+        float* dst = a.states + ((bh * a.nc + a.c0 + c) * a.P + pb + p) * (int64_t)a.N + half * HN;
+#pragma unroll
+        for (int j = 0; j < HN; j += 4) *reinterpret_cast<float4*>(dst + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+      }
+      // X^T = V^T - exp(l) KS^T, 32 tokens of this half; V is fetched while KS runs
       const uint8_t* st = stage(c);
-      if (!waitw(&full[c & 1], c >> 1, 2002) || !waitw(ksdone, c, 2003)) { ok = false; break; }
-      tc_fence_after();
-      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_G);
+      ok = ok && waitw(&full[c & 1], c >> 1, 2002);
+      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_G) + 32 * half;
       const float* wb = eg + Q;
-      const __nv_bfloat16* vs = reinterpret_cast<const __nv_bfloat16*>(st + SM::V + (p >> 6) * TILE) + (p & 63) + half * 32 * 64;
+      uint32_t v[16];
+      {
+        const uint16_t* vs = reinterpret_cast<const uint16_t*>(st + SM::V + (p >> 6) * TILE) + (p & 63) + half * 32 * 64;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = __byte_perm(vs[(2 * j) * 64], vs[(2 * j + 1) * 64], 0x5410);
+      }
+      ok = ok && waitw(ksdone, c, 2003);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         float x[16];
@@ -257,54 +291,59 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
         tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
-          const float4 e4 = *reinterpret_cast<const float4*>(eg + 32 * half + 16 * i + j);
-          const __nv_bfloat16* v = vs + (16 * i + j) * 64;
-          x[j] = __bfloat162float(v[0]) - e4.x * x[j];
-          x[j + 1] = __bfloat162float(v[64]) - e4.y * x[j + 1];
-          x[j + 2] = __bfloat162float(v[128]) - e4.z * x[j + 2];
-          x[j + 3] = __bfloat162float(v[192]) - e4.w * x[j + 3];
+          const float4 e4 = *reinterpret_cast<const float4*>(eg + 16 * i + j);
+          x[j] = lo2(v[8 * i + j / 2]) - e4.x * x[j];
+          x[j + 1] = hi2(v[8 * i + j / 2]) - e4.y * x[j + 1];
+          x[j + 2] = lo2(v[8 * i + j / 2 + 1]) - e4.z * x[j + 2];
+          x[j + 3] = hi2(v[8 * i + j / 2 + 1]) - e4.w * x[j + 3];
         }
         store_planes<NS>(tl + C_XP + 48 * half + 8 * i, 16, x);
+        hand_over(B_X + i);
       }
-      tmem_wait_st();
-      arrive_warp(xready);
-      // E^T: planes of E for O, of E diag(w beta) for the state
-      if (!waitw(edone, c, 2004)) { ok = false; break; }
-      tc_fence_after();
-      const float el = eg[Q - 1];
+      // E^T: planes of E diag(w beta) for the state
+      const float el = (eg - 32 * half)[Q - 1];
+      ok = ok && waitw(edone, c, 2004);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float x[16], r[16];
+        float x[16];
         tmem_ld16(tl + C_KE + 32 * half + 16 * i, x);
         tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
-          const float4 w4 = *reinterpret_cast<const float4*>(wb + 32 * half + 16 * i + j);
-          r[j] = x[j] * w4.x;
-          r[j + 1] = x[j + 1] * w4.y;
-          r[j + 2] = x[j + 2] * w4.z;
-          r[j + 3] = x[j + 3] * w4.w;
+          const float4 w4 = *reinterpret_cast<const float4*>(wb + 16 * i + j);
+          x[j] *= w4.x;
+          x[j + 1] *= w4.y;
+          x[j + 2] *= w4.z;
+          x[j + 3] *= w4.w;
         }
-        store_planes<NS>(tl + C_XP + 48 * half + 8 * i, 16, r);
-        if (a.errs && live) {
+        store_planes<NS>(tl + C_XP + 48 * half + 8 * i, 16, x);
+        hand_over(B_W + i);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[c & 1]);   // V and the gates are read
+      // E's planes for O (whose product of the chunk before has read the last ones)
+      ok = ok && (c == 0 || waitw(odone, c - 1, 2001));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float x[16];
+        tmem_ld16(tl + C_KE + 32 * half + 16 * i, x);
+        tmem_wait_ld();
+        if (a.errs && live && ok) {
           const int64_t tk = (a.c0 + c) * Q + 32 * half + 16 * i;
           float* ep = a.errs + ((b * a.L + tk) * a.H + h) * (int64_t)a.P + pb + p;
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             if (tk + j < a.L) ep[(int64_t)j * a.H * a.P] = x[j];
         }
-        store_planes<2>(tl + 96 * half + 64 + 8 * i, 16, x);
+        store_planes<2>(tl + C_EO + 32 * half + 8 * i, 16, x);
       }
-      tmem_wait_st();
-      arrive_warp(eready);
-      if (lane == 0) mbar_arrive(&empty[c & 1]);   // V and the gates are read (arrive_warp synchronised the warp)
+      hand_over(B_E);
       // S^T
-      if (!waitw(dsdone, c, 2005)) { ok = false; break; }
-      tc_fence_after();
+      ok = ok && waitw(dsdone, c, 2005);
 #pragma unroll
       for (int i = 0; i < HN / 16; ++i) {
         float d[16];
-        tmem_ld16(tl + (NB == 2 ? 96 * half : C_KE + 32 * half) + 16 * i, d);
+        tmem_ld16(tl + HN * half + 16 * i, d);
         tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 16; ++j) S[16 * i + j] = el * S[16 * i + j] + d[j];
@@ -315,46 +354,66 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       for (int j = 0; j < HN; j += 4)
         *reinterpret_cast<float4*>(a.h_out + row + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
     }
-  } else if (warp < 12) {
+  } else if (warp >= 12) {
     // ================================================================ outputs
-    const int w = warp - 8, p = w * 32 + lane;
+    const int w = warp - 12, p = w * 32 + lane;
     const uint32_t tl = tmem + ((uint32_t)(w * 32) << 16);
     for (int c = 0; c < n; ++c) {
       const uint8_t* st = stage(c);
-      const bool bad = !waitw(&full[c & 1], c >> 1, 2006) || !waitw(odone, c, 2007);   // odone: both products
-      if (tid == 256 && c > 0) bulk_wait_read<0>();   // the last chunk's store has left the tile
-      if (named_bar_or(1, 128, bad)) break;
-      tc_fence_after();
-      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_G);
+      float o[Q];   // QS^T waits in registers, so that O's second product may take its columns
+      bool bad = !waitw(&full[c & 1], c >> 1, 2006) || !waitw(qdone, c, 2007);
+      if (!bad) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float t[16];
+          tmem_ld16(tl + C_O + 16 * i, t);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[16 * i + j] = t[j];
+        }
+        arrive_warp(qread);
+        const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_G);
+#pragma unroll
+        for (int j = 0; j < Q; j += 4) {
+          const float4 e4 = *reinterpret_cast<const float4*>(eg + j);
+          o[j] *= a.scale * e4.x;
+          o[j + 1] *= a.scale * e4.y;
+          o[j + 2] *= a.scale * e4.z;
+          o[j + 3] *= a.scale * e4.w;
+        }
+        bad = !waitw(odone, c, 2008);
+      }
+      if (tid == 384 && c > 0) bulk_wait_read<0>();   // the last chunk's store has left the tile
+      if (named_bar_or(B_OUT, 128, bad)) break;
       __nv_bfloat16* ys = reinterpret_cast<__nv_bfloat16*>(smem + SM::Y + (p >> 6) * TILE) + (p & 63);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float o1[16], o2[16];
-        tmem_ld16(tl + C_O1 + 16 * i, o1);
-        tmem_ld16(tl + C_O2 + 16 * i, o2);
+        float t[16];
+        tmem_ld16(tl + C_O + 16 * i, t);
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          ys[(16 * i + j) * 64] = __float2bfloat16_rn(a.scale * eg[16 * i + j] * o1[j] + o2[j]);
+        for (int j = 0; j < 16; ++j) ys[(16 * i + j) * 64] = __float2bfloat16_rn(o[16 * i + j] + t[j]);
       }
-      arrive_warp(ofree);
+      arrive_warp(oread);
       if (lane == 0) mbar_arrive(&empty[c & 1]);
       fence_proxy_async_smem();
-      named_bar_sync(1, 128);
-      if (tid == 256) {
+      named_bar_sync(B_OUT, 128);
+      if (tid == 384) {
         for (int x = 0; x < boxes; ++x)   // rows past L are clipped by the map
           tma_store_3d(&tm_y, smem + SM::Y + x * TILE, h * a.P + pb + 64 * x, (int)(a.c0 + c) * Q, b);
         bulk_commit();
       }
     }
-    if (tid == 256) bulk_wait<0>();
-  } else {
-    if (warp == 12 && lane == 0) {
-      // ============================================================== copies
-      int c = 0;
+    if (tid == 384) bulk_wait<0>();
+  } else if (warp == 1) {
+    // ================================================================ copies
+    if (lane == 0) {
       const uint32_t bytes = 2 * NB * TILE + boxes * TILE + IMG;
-      for (; c < n; ++c) {
-        if (c >= 2 && !wait1(&empty[c & 1], (c >> 1) - 1, 2008)) break;
+      for (int c = 0; c < n; ++c) {
+        if (c >= 2 && !mbar_wait(&empty[c & 1], ((c >> 1) - 1) & 1, abort_flag)) {
+          if (!*abort_flag) fail(2009);
+          break;
+        }
         uint8_t* st = stage(c);
         uint64_t* f = &full[c & 1];
         const int t0 = (int)(a.c0 + c) * Q;
@@ -370,86 +429,99 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
                      : "memory");
         *issued = c + 1;
       }
-    } else if (warp == 13 && lane == 0) {
-      // ============================================================== KS, E, state update
-      constexpr uint32_t ID_K = make_idesc_bf16(128, 64, false, false), ID_MN = make_idesc_bf16(128, 64, false, true);
-      for (int c = 0; c < n; ++c) {
-        const uint32_t st = smem_u32(stage(c));
-        if (!wait1(&full[c & 1], c >> 1, 2009) || !wait1(sready, c, 2010)) break;
-        tc_fence_after();
+    }
+  } else if (warp == 0) {
+    // ================================================================ the chain's products
+    bool ok = true;
+    for (int c = 0; c < n; ++c) {
+      const uint32_t st = smem_u32(stage(c));
+      ok = ok && waitw(&full[c & 1], c >> 1, 2010);
+      // KS
 #pragma unroll
-        for (int s = NS - 1; s >= 0; --s)
+      for (int i = 0; i < HN / 16; ++i) {
+        take(B_S + i);
+        if (ok && elect_one())
 #pragma unroll
-          for (int kk = 0; kk < KN / 16; ++kk) {
-            const int hf = kk / (HN / 16), ko = kk % (HN / 16);
-            umma_bf16_ta(tmem + C_KE, tmem + 96 * hf + 32 * s + 8 * ko,
-                         make_desc_sw128(st + SM::K + (kk / 4) * TILE, 16) + 2 * (kk & 3), ID_K, s != NS - 1 || kk);
-          }
-        umma_commit(ksdone);
-        if (!wait1(xready, c, 2011)) break;
-        tc_fence_after();
+          for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const uint32_t id = make_idesc_bf16(128, 64 - 16 * t, false, false);
-#pragma unroll
-          for (int o = NS - 1; o >= 0; --o)
-#pragma unroll
-            for (int s = 0; s <= o; ++s)
-              umma_bf16_ta(tmem + C_KE + 16 * t, tmem + C_XP + 48 * (t >> 1) + 16 * s + 8 * (t & 1),
-                           make_desc_sw128(st + SM::IM + IMG_T + (o - s) * SQ_BYTES, 16) + 128 * t + 2 * t, id,
-                           t || o != NS - 1 || s);
-        }
-        umma_commit(edone);
-        if (!wait1(eready, c, 2012) || !wait1(qdone, c, 2013)) break;   // O's first product has read S planes 0, 1
-        tc_fence_after();
-#pragma unroll
-        for (int x = 0; x < NB; ++x)
-#pragma unroll
-          for (int s = NS - 1; s >= 0; --s)
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-              umma_bf16_ta(tmem + (NB == 2 ? 96 * x : C_KE), tmem + C_XP + 48 * (t >> 1) + 16 * s + 8 * (t & 1),
-                           make_desc_sw128(st + SM::K + x * TILE, TILE) + 128 * t, ID_MN, s != NS - 1 || t);
-        umma_commit(dsdone);
-        umma_commit(&empty[c & 1]);
+            for (int s = NS - 1; s >= 0; --s) {
+              const int kk = hf * (HN / 16) + i;
+              umma_bf16_ta(tmem + C_KE, tmem + plane(s, hf) + 8 * i,
+                           make_desc_sw128(st + SM::K + (kk / 4) * TILE, 16) + 2 * (kk & 3),
+                           make_idesc_bf16(128, 64, false, false), i || hf || s != NS - 1);
+            }
       }
-      umma_commit(&drain[0]);
-      mbar_wait(&drain[0], 0, nullptr, 100000000ull);
-    } else if (warp == 14 && lane == 0) {
-      // ============================================================== O
-      constexpr uint32_t ID_K = make_idesc_bf16(128, 64, false, false);
-      for (int c = 0; c < n; ++c) {
-        const uint32_t st = smem_u32(stage(c));
-        if (!wait1(&full[c & 1], c >> 1, 2014) || !wait1(sready, c, 2015) || (c > 0 && !wait1(ofree, c - 1, 2016))) break;
-        tc_fence_after();
+      umma_commit_warp(ksdone);
+      // E, over KS
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        take(B_X + i);
+        if (ok && elect_one())
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int o = NS - 1; o >= 0; --o)
+#pragma unroll
+              for (int s = 0; s <= o; ++s) {
+                const int t = 2 * hf + i;   // tokens 16 t .. reach the columns from 16 t
+                umma_bf16_ta(tmem + C_KE + 16 * t, tmem + C_XP + 48 * hf + 16 * s + 8 * i,
+                             make_desc_sw128(st + SM::IM + IMG_T + (o - s) * SQ_BYTES, 16) + 130 * t,
+                             make_idesc_bf16(128, 64 - 16 * t, false, false), t || o != NS - 1 || s);
+              }
+      }
+      umma_commit_warp(edone);
+      // state update, over S planes 0 and 1, which QS has read by now
+      ok = ok && waitw(qdone, c, 2011);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        take(B_W + i);
+        if (ok && elect_one())
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int s = NS - 1; s >= 0; --s)
+              umma_bf16_ta(tmem, tmem + C_XP + 48 * hf + 16 * s + 8 * i,
+                           make_desc_sw128(st + SM::K, TILE) + 128 * (2 * hf + i),
+                           make_idesc_bf16(128, KN, false, true), i || hf || s != NS - 1);
+      }
+      umma_commit_warp(dsdone);
+      umma_commit_warp(&empty[c & 1]);
+    }
+    umma_commit_warp(&drain[0]);
+    mbar_wait(&drain[0], 0, nullptr, 100000000ull);
+  } else if (warp == 2) {
+    // ================================================================ O's products
+    bool ok = true;
+    for (int c = 0; c < n; ++c) {
+      const uint32_t st = smem_u32(stage(c));
+      // QS behind KS (it runs while X is made), once the columns of the last output are read
+      ok = ok && waitw(&full[c & 1], c >> 1, 2012) && waitw(ksdone, c, 2013) && (c == 0 || waitw(oread, c - 1, 2014));
+      if (ok && elect_one())
 #pragma unroll
         for (int s = 1; s >= 0; --s)
 #pragma unroll
-          for (int kk = 0; kk < KN / 16; ++kk) {
-            const int hf = kk / (HN / 16), ko = kk % (HN / 16);
-            umma_bf16_ta(tmem + C_O1, tmem + 96 * hf + 32 * s + 8 * ko,
-                         make_desc_sw128(st + SM::QQ + (kk / 4) * TILE, 16) + 2 * (kk & 3), ID_K, s != 1 || kk);
-          }
-        umma_commit(qdone);
-        if (!wait1(eready, c, 2017)) break;
-        tc_fence_after();
+          for (int kk = 0; kk < KN / 16; ++kk)
+            umma_bf16_ta(tmem + C_O, tmem + plane(s, kk / (HN / 16)) + 8 * (kk % (HN / 16)),
+                         make_desc_sw128(st + SM::QQ + (kk / 4) * TILE, 16) + 2 * (kk & 3),
+                         make_idesc_bf16(128, 64, false, false), s != 1 || kk);
+      umma_commit_warp(qdone);
+      take(B_E);
+      ok = ok && waitw(qread, c, 2015);
+      if (ok && elect_one())
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const uint32_t id = make_idesc_bf16(128, 64 - 16 * t, false, false);
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int o = 1; o >= 0; --o)
 #pragma unroll
             for (int s = 0; s <= o; ++s)
-              umma_bf16_ta(tmem + C_O2 + 16 * t, tmem + 96 * (t >> 1) + 64 + 16 * s + 8 * (t & 1),
-                           make_desc_sw128(st + SM::IM + IMG_AQ + (o - s) * SQ_BYTES, 16) + 128 * t + 2 * t, id,
-                           t || o != 1 || s);
-        }
-        umma_commit(odone);
-        umma_commit(&empty[c & 1]);
-      }
-      umma_commit(&drain[1]);
-      mbar_wait(&drain[1], 0, nullptr, 100000000ull);
+              umma_bf16_ta(tmem + C_O + 16 * t, tmem + C_EO + 32 * (t >> 1) + 16 * s + 8 * (t & 1),
+                           make_desc_sw128(st + SM::IM + IMG_AQ + (o - s) * SQ_BYTES, 16) + 130 * t,
+                           make_idesc_bf16(128, 64 - 16 * t, false, false), t || o != 1 || s);
+      umma_commit_warp(odone);
+      umma_commit_warp(&empty[c & 1]);
     }
+    umma_commit_warp(&drain[1]);
+    mbar_wait(&drain[1], 0, nullptr, 100000000ull);
   }
   // ================================================================ teardown
   tc_fence_before();
@@ -457,7 +529,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
   if (tid == 0 && *abort_flag)   // copies that were started land before the block leaves
     for (int c = max(0, *issued - 2); c < *issued; ++c) mbar_wait(&full[c & 1], (c >> 1) & 1, nullptr, 100000000ull);
   __syncthreads();
-  if (warp == 0) {
+  if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
