@@ -349,13 +349,15 @@ constexpr int SQ_RB = 128, SQ_BYTES = Q * SQ_RB;
 // 128 threads (t = 0..127): from the loaded K, Q planes and the gates, the planes of
 // Aq diag(beta) (NA of them) and of T (NTP).  M is the f32 work matrix.  Entries of 16-blocks
 // above the diagonal are not written: nobody reads them.
-template <int XS, int KN, int NA, int NTP>
+// If ALIAS, M may lie over the Q planes (their product comes first).
+template <int XS, int KN, int NA, int NTP, bool ALIAS = false>
 __device__ __forceinline__ void chunk_matrices(uint32_t k, uint32_t q, const Gates& g, float scale, float* M,
                                                uint8_t* aq, uint8_t* tp, int t, int bar) {
   constexpr int RB = KN * 2, PB = Q * RB, KK = KN / 16;
   const int w = t / 32, lane = t % 32, gr = lane / 4, q2 = 2 * (lane % 4);
 #pragma unroll
-  for (int pass = 0; pass < 2; ++pass) {   // K K^T, then Q K^T with the rows dealt the other way round
+  for (int pass = 1; pass >= 0; --pass) {   // Q K^T, then K K^T with the rows dealt the other way round
+    if (ALIAS && pass == 0) bar_sync(bar, 128);
     const int I = pass ? 3 - w : w, r0 = 16 * I + gr;
     uint32_t a[XS == 1 ? KK : 1][XS][4];   // this row block's operand (bf16: kept for all column blocks)
     if constexpr (XS == 1)

@@ -23,10 +23,13 @@
 // tcgen05 takes 32 cycles per 128 x 64 x 16 and 190 from issue to a thread that waits.
 //
 // TMEM columns: [0, 192) S planes (planes 0, 1 of a half side by side, then both plane
-// 2s), later the state update's sum over planes 0, 1.  [192, 256) KS, then E.
-// [256, 352) X planes, then E diag(w beta) planes, 48 per half.  [352, 416) E's two
-// planes for O.  [416, 480) QS, then Aq diag(beta) E.  A thread overwrites columns of
+// 2s), later the state update's sum over planes 0, 1.  [192, 256) KS.  [256, 352) X
+// planes, then E diag(w beta) planes, 48 per half.  [352, 416) E, then its two planes
+// for O.  [416, 480) QS, then O.  A thread overwrites columns of
 // its own lane and half only, so only products are waited for.
+//
+// Loops are left rolled where registers allow: unrolled (130 KB of code) the warps
+// waited for instructions, the more so with both SMs of a pair at work.
 //
 // Every wait on an mbarrier is bounded.  A warp that gives up sets the abort flag and
 // goes on without waiting, storing nothing: the named barriers' counts stay whole.
@@ -44,7 +47,7 @@ using namespace sm100;
 
 constexpr int TILE = 8192;                       // [64 x 64] bf16
 constexpr int IMG_T = 0, IMG_AQ = 3 * SQ_BYTES, IMG_G = IMG_AQ + 2 * SQ_BYTES, IMG = IMG_G + 2 * Q * 4;
-constexpr int64_t IMAGE_BYTES = 64ll << 20;
+constexpr int64_t IMAGE_BYTES = 256ll << 20;
 
 // ------------------------------------------------------------------ chunk images
 struct PrepArgs {
@@ -59,11 +62,12 @@ struct PrepArgs {
 template <int KN>
 struct PrepSmem {
   static constexpr int PLANE = Q * KN * 2;
-  static constexpr int K = 0, QQ = PLANE, M = 2 * PLANE, G = M + Q * AM * 4, BYTES = G + (int)sizeof(Gates) + 128;
+  static constexpr int MB = Q * AM * 4;   // the work matrix lies over the Q tile
+  static constexpr int K = 0, QQ = PLANE, M = QQ, G = QQ + (MB > PLANE ? MB : PLANE), BYTES = G + (int)sizeof(Gates) + 128;
 };
 
 template <int KN>
-__global__ void __launch_bounds__(128, 4) delta_prep_kernel(const PrepArgs a) {
+__global__ void __launch_bounds__(128, 6) delta_prep_kernel(const PrepArgs a) {
   using SM = PrepSmem<KN>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((128u - (smem_addr(smem_raw) & 127u)) & 127u);
@@ -83,7 +87,7 @@ __global__ void __launch_bounds__(128, 4) delta_prep_kernel(const PrepArgs a) {
   uint8_t* img = a.img + (bh * a.nseg + ci) * IMG;
   float* go = reinterpret_cast<float*>(img + IMG_G);
   go[t] = t < Q ? gt.eg[t] : gt.wb[t - Q];
-  chunk_matrices<1, KN, 2, 3>(s + SM::K, s + SM::QQ, gt, a.scale, reinterpret_cast<float*>(smem + SM::M), img + IMG_AQ,
+  chunk_matrices<1, KN, 2, 3, true>(s + SM::K, s + SM::QQ, gt, a.scale, reinterpret_cast<float*>(smem + SM::M), img + IMG_AQ,
                               img + IMG_T, t, 1);
 }
 
@@ -106,7 +110,7 @@ struct ScanSmem {
   static_assert(BYTES <= 232448, "shared-memory layout exceeds the per-block limit");
 };
 
-constexpr uint32_t C_KE = 192, C_XP = 256, C_EO = 352, C_O = 416;
+constexpr uint32_t C_KS = 192, C_XP = 256, C_E = 352, C_O = 416;
 // named barriers (0: __syncthreads): outputs; pieces of S, X, E diag(w beta), E for their issuers
 constexpr uint32_t B_OUT = 1, B_S = 2, B_X = 6, B_W = 8, B_E = 10, B_ISSUE = 256 + 32;
 
@@ -129,6 +133,7 @@ __device__ __forceinline__ void umma_bf16_ta(uint32_t d, uint32_t a, uint64_t b,
 // test_wait loop measured 272 cycles, through try_wait 237, and a waiting warp takes no
 // issue slots from the working ones), then as mbar_wait.
 __device__ __forceinline__ bool mbar_wait_hot(uint64_t* m, uint32_t parity, const volatile int* abort_flag) {
+#pragma unroll 1
   for (int i = 0; i < 64; ++i)
     if (mbar_try_wait(m, parity, 20000u)) return true;
   if (*abort_flag) return false;
@@ -138,6 +143,19 @@ __device__ __forceinline__ void tmem_st8u(uint32_t taddr, const uint32_t (&u)[8]
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(u[0]),
                "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
                : "memory");
+}
+// 16 columns of TMEM into registers.  The wait is part of the statement, so that no use of
+// the values can be scheduled before it.
+__device__ __forceinline__ void tmem_get16(uint32_t taddr, float (&r)[16]) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(taddr)
+      : "memory");
 }
 // 16 values as NS planes of 8 columns, plane s at taddr[s] (r is used up).
 template <int NS>
@@ -272,42 +290,38 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
 #pragma unroll
         for (int j = 0; j < HN; j += 4) *reinterpret_cast<float4*>(dst + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
       }
-      // X^T = V^T - exp(l) KS^T, 32 tokens of this half; V is fetched while KS runs
+      // X^T = V^T - exp(l) KS^T, 32 tokens of this half
       const uint8_t* st = stage(c);
       ok = ok && waitw(&full[c & 1], c >> 1, 2002);
       const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_G) + 32 * half;
       const float* wb = eg + Q;
-      uint32_t v[16];
-      {
-        const uint16_t* vs = reinterpret_cast<const uint16_t*>(st + SM::V + (p >> 6) * TILE) + (p & 63) + half * 32 * 64;
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = __byte_perm(vs[(2 * j) * 64], vs[(2 * j + 1) * 64], 0x5410);
-      }
+      const float el = (eg - 32 * half)[Q - 1];
+      const uint16_t* vs = reinterpret_cast<const uint16_t*>(st + SM::V + (p >> 6) * TILE) + (p & 63) + half * 32 * 64;
       ok = ok && waitw(ksdone, c, 2003);
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         float x[16];
-        tmem_ld16(tl + C_KE + 32 * half + 16 * i, x);
-        tmem_wait_ld();
+        uint32_t v[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = vs[(16 * i + j) * 64];
+        tmem_get16(tl + C_KS + 32 * half + 16 * i, x);
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
           const float4 e4 = *reinterpret_cast<const float4*>(eg + 16 * i + j);
-          x[j] = lo2(v[8 * i + j / 2]) - e4.x * x[j];
-          x[j + 1] = hi2(v[8 * i + j / 2]) - e4.y * x[j + 1];
-          x[j + 2] = lo2(v[8 * i + j / 2 + 1]) - e4.z * x[j + 2];
-          x[j + 3] = hi2(v[8 * i + j / 2 + 1]) - e4.w * x[j + 3];
+          x[j] = lo2(v[j]) - e4.x * x[j];
+          x[j + 1] = lo2(v[j + 1]) - e4.y * x[j + 1];
+          x[j + 2] = lo2(v[j + 2]) - e4.z * x[j + 2];
+          x[j + 3] = lo2(v[j + 3]) - e4.w * x[j + 3];
         }
         store_planes<NS>(tl + C_XP + 48 * half + 8 * i, 16, x);
         hand_over(B_X + i);
       }
       // E^T: planes of E diag(w beta) for the state
-      const float el = (eg - 32 * half)[Q - 1];
       ok = ok && waitw(edone, c, 2004);
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         float x[16];
-        tmem_ld16(tl + C_KE + 32 * half + 16 * i, x);
-        tmem_wait_ld();
+        tmem_get16(tl + C_E + 32 * half + 16 * i, x);
 #pragma unroll
         for (int j = 0; j < 16; j += 4) {
           const float4 w4 = *reinterpret_cast<const float4*>(wb + 16 * i + j);
@@ -321,21 +335,21 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[c & 1]);   // V and the gates are read
-      // E's planes for O (whose product of the chunk before has read the last ones)
-      ok = ok && (c == 0 || waitw(odone, c - 1, 2001));
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float x[16];
-        tmem_ld16(tl + C_KE + 32 * half + 16 * i, x);
-        tmem_wait_ld();
+      // E's planes for O, over E (both pieces are read before either is written)
+      {
+        float x[2][16];
+        tmem_get16(tl + C_E + 32 * half, x[0]);
+        tmem_get16(tl + C_E + 32 * half + 16, x[1]);
         if (a.errs && live && ok) {
-          const int64_t tk = (a.c0 + c) * Q + 32 * half + 16 * i;
+          const int64_t tk = (a.c0 + c) * Q + 32 * half;
           float* ep = a.errs + ((b * a.L + tk) * a.H + h) * (int64_t)a.P + pb + p;
+          const int left = (int)min((int64_t)32, a.L - tk);
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (tk + j < a.L) ep[(int64_t)j * a.H * a.P] = x[j];
+          for (int j = 0; j < 32; ++j)
+            if (j < left) ep[(int64_t)j * a.H * a.P] = x[j >> 4][j & 15];
         }
-        store_planes<2>(tl + C_EO + 32 * half + 8 * i, 16, x);
+        store_planes<2>(tl + C_E + 32 * half, 16, x[0]);
+        store_planes<2>(tl + C_E + 32 * half + 8, 16, x[1]);
       }
       hand_over(B_E);
       // S^T
@@ -343,8 +357,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
 #pragma unroll
       for (int i = 0; i < HN / 16; ++i) {
         float d[16];
-        tmem_ld16(tl + HN * half + 16 * i, d);
-        tmem_wait_ld();
+        tmem_get16(tl + HN * half + 16 * i, d);
 #pragma unroll
         for (int j = 0; j < 16; ++j) S[16 * i + j] = el * S[16 * i + j] + d[j];
       }
@@ -360,39 +373,37 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
     const uint32_t tl = tmem + ((uint32_t)(w * 32) << 16);
     for (int c = 0; c < n; ++c) {
       const uint8_t* st = stage(c);
-      float o[Q];   // QS^T waits in registers, so that O's second product may take its columns
+      // scale exp(l) QS^T goes back to its columns, where Aq diag(beta) E is added
       bool bad = !waitw(&full[c & 1], c >> 1, 2006) || !waitw(qdone, c, 2007);
+      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_G);
       if (!bad) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
+#pragma unroll 1
+        for (int i = 0; i < Q; i += 16) {
           float t[16];
-          tmem_ld16(tl + C_O + 16 * i, t);
-          tmem_wait_ld();
+          tmem_get16(tl + C_O + i, t);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) o[16 * i + j] = t[j];
+          for (int j = 0; j < 16; j += 4) {
+            const float4 e4 = *reinterpret_cast<const float4*>(eg + i + j);
+            t[j] *= a.scale * e4.x;
+            t[j + 1] *= a.scale * e4.y;
+            t[j + 2] *= a.scale * e4.z;
+            t[j + 3] *= a.scale * e4.w;
+          }
+          tmem_st16(tl + C_O + i, t);
         }
+        tmem_wait_st();
         arrive_warp(qread);
-        const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_G);
-#pragma unroll
-        for (int j = 0; j < Q; j += 4) {
-          const float4 e4 = *reinterpret_cast<const float4*>(eg + j);
-          o[j] *= a.scale * e4.x;
-          o[j + 1] *= a.scale * e4.y;
-          o[j + 2] *= a.scale * e4.z;
-          o[j + 3] *= a.scale * e4.w;
-        }
         bad = !waitw(odone, c, 2008);
       }
       if (tid == 384 && c > 0) bulk_wait_read<0>();   // the last chunk's store has left the tile
       if (named_bar_or(B_OUT, 128, bad)) break;
       __nv_bfloat16* ys = reinterpret_cast<__nv_bfloat16*>(smem + SM::Y + (p >> 6) * TILE) + (p & 63);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
+#pragma unroll 1
+      for (int i = 0; i < Q; i += 16) {
         float t[16];
-        tmem_ld16(tl + C_O + 16 * i, t);
-        tmem_wait_ld();
+        tmem_get16(tl + C_O + i, t);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) ys[(16 * i + j) * 64] = __float2bfloat16_rn(o[16 * i + j] + t[j]);
+        for (int j = 0; j < 16; ++j) ys[(i + j) * 64] = __float2bfloat16_rn(t[j]);
       }
       arrive_warp(oread);
       if (lane == 0) mbar_arrive(&empty[c & 1]);
@@ -437,7 +448,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       const uint32_t st = smem_u32(stage(c));
       ok = ok && waitw(&full[c & 1], c >> 1, 2010);
       // KS
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < HN / 16; ++i) {
         take(B_S + i);
         if (ok && elect_one())
@@ -446,14 +457,15 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
 #pragma unroll
             for (int s = NS - 1; s >= 0; --s) {
               const int kk = hf * (HN / 16) + i;
-              umma_bf16_ta(tmem + C_KE, tmem + plane(s, hf) + 8 * i,
+              umma_bf16_ta(tmem + C_KS, tmem + plane(s, hf) + 8 * i,
                            make_desc_sw128(st + SM::K + (kk / 4) * TILE, 16) + 2 * (kk & 3),
                            make_idesc_bf16(128, 64, false, false), i || hf || s != NS - 1);
             }
       }
       umma_commit_warp(ksdone);
-      // E, over KS
-#pragma unroll
+      // E, where O's product of the chunk before has read its planes
+      ok = ok && (c == 0 || waitw(odone, c - 1, 2018));
+#pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         take(B_X + i);
         if (ok && elect_one())
@@ -464,7 +476,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
 #pragma unroll
               for (int s = 0; s <= o; ++s) {
                 const int t = 2 * hf + i;   // tokens 16 t .. reach the columns from 16 t
-                umma_bf16_ta(tmem + C_KE + 16 * t, tmem + C_XP + 48 * hf + 16 * s + 8 * i,
+                umma_bf16_ta(tmem + C_E + 16 * t, tmem + C_XP + 48 * hf + 16 * s + 8 * i,
                              make_desc_sw128(st + SM::IM + IMG_T + (o - s) * SQ_BYTES, 16) + 130 * t,
                              make_idesc_bf16(128, 64 - 16 * t, false, false), t || o != NS - 1 || s);
               }
@@ -472,7 +484,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       umma_commit_warp(edone);
       // state update, over S planes 0 and 1, which QS has read by now
       ok = ok && waitw(qdone, c, 2011);
-#pragma unroll
+#pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         take(B_W + i);
         if (ok && elect_one())
@@ -497,10 +509,10 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       // QS behind KS (it runs while X is made), once the columns of the last output are read
       ok = ok && waitw(&full[c & 1], c >> 1, 2012) && waitw(ksdone, c, 2013) && (c == 0 || waitw(oread, c - 1, 2014));
       if (ok && elect_one())
+#pragma unroll 1
+        for (int kk = 0; kk < KN / 16; ++kk)
 #pragma unroll
-        for (int s = 1; s >= 0; --s)
-#pragma unroll
-          for (int kk = 0; kk < KN / 16; ++kk)
+          for (int s = 1; s >= 0; --s)
             umma_bf16_ta(tmem + C_O, tmem + plane(s, kk / (HN / 16)) + 8 * (kk % (HN / 16)),
                          make_desc_sw128(st + SM::QQ + (kk / 4) * TILE, 16) + 2 * (kk & 3),
                          make_idesc_bf16(128, 64, false, false), s != 1 || kk);
@@ -508,15 +520,15 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       take(B_E);
       ok = ok && waitw(qread, c, 2015);
       if (ok && elect_one())
-#pragma unroll
+#pragma unroll 1
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int o = 1; o >= 0; --o)
 #pragma unroll
             for (int s = 0; s <= o; ++s)
-              umma_bf16_ta(tmem + C_O + 16 * t, tmem + C_EO + 32 * (t >> 1) + 16 * s + 8 * (t & 1),
+              umma_bf16_ta(tmem + C_O + 16 * t, tmem + C_E + 32 * (t >> 1) + 16 * s + 8 * (t & 1),
                            make_desc_sw128(st + SM::IM + IMG_AQ + (o - s) * SQ_BYTES, 16) + 130 * t,
-                           make_idesc_bf16(128, 64 - 16 * t, false, false), t || o != 1 || s);
+                           make_idesc_bf16(128, 64 - 16 * t, false, false), true);   // onto scale exp(l) QS
       umma_commit_warp(odone);
       umma_commit_warp(&empty[c & 1]);
     }
