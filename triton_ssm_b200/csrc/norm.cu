@@ -22,19 +22,18 @@ namespace {
 constexpr int NT = 256;
 constexpr int64_t L2_BYTES = 64ll << 20;   // of 126 MB: room for the outputs written meanwhile
 
-template <typename T, int V> struct vec;   // V elements moved as one access
+// V elements moved as one access: R as they lie in memory, cvt to f32.
+template <typename T, int V> struct vec;
 template <> struct vec<float, 4> {
-  __device__ static void ld(const float* p, float (&f)[4]) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
+  using R = float4;
+  __device__ static void cvt(const R& v, float (&f)[4]) {
     f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
   }
-  __device__ static void st(float* p, const float (&f)[4]) {
-    *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-  }
+  __device__ static R pack(const float (&f)[4]) { return make_float4(f[0], f[1], f[2], f[3]); }
 };
 template <> struct vec<__nv_bfloat16, 8> {
-  __device__ static void ld(const __nv_bfloat16* p, float (&f)[8]) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
+  using R = uint4;
+  __device__ static void cvt(const R& v, float (&f)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -42,38 +41,56 @@ template <> struct vec<__nv_bfloat16, 8> {
       f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
     }
   }
-  __device__ static void st(__nv_bfloat16* p, const float (&f)[8]) {
+  __device__ static R pack(const float (&f)[8]) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const __nv_bfloat162 b = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
       w[i] = *reinterpret_cast<const uint32_t*>(&b);
     }
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    return make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 template <> struct vec<__nv_bfloat16, 4> {
-  __device__ static void ld(const __nv_bfloat16* p, float (&f)[4]) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
+  using R = uint2;
+  __device__ static void cvt(const R& v, float (&f)[4]) {
     f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
     f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
   }
-  __device__ static void st(__nv_bfloat16* p, const float (&f)[4]) {
+  __device__ static R pack(const float (&f)[4]) {
     const __nv_bfloat162 a = __floats2bfloat162_rn(f[0], f[1]), b = __floats2bfloat162_rn(f[2], f[3]);
-    *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
   }
 };
-template <typename T> struct vec<T, 1> {
-  __device__ static void ld(const T* p, float (&f)[1]) { f[0] = ldf(p); }
-  __device__ static void st(T* p, const float (&f)[1]) { stf(p, f[0]); }
+template <> struct vec<float, 1> {
+  using R = float;
+  __device__ static void cvt(const R& v, float (&f)[1]) { f[0] = v; }
+  __device__ static R pack(const float (&f)[1]) { return f[0]; }
 };
+template <> struct vec<__nv_bfloat16, 1> {
+  using R = uint16_t;
+  __device__ static void cvt(const R& v, float (&f)[1]) { f[0] = __uint_as_float((uint32_t)v << 16); }
+  __device__ static R pack(const float (&f)[1]) { return __bfloat16_as_ushort(__float2bfloat16_rn(f[0])); }
+};
+template <typename T, int V> using raw = typename vec<T, V>::R;
+template <typename T, int V>
+__device__ __forceinline__ raw<T, V> ldr(const T* p) { return *reinterpret_cast<const raw<T, V>*>(p); }
+template <typename T, int V>
+__device__ __forceinline__ void stv(T* p, const float (&f)[V]) { *reinterpret_cast<raw<T, V>*>(p) = vec<T, V>::pack(f); }
 
-// sigmoid(z).  A bf16 result takes the hardware exponential and division (relative
-// error near 2^-21, far below bf16's 2^-9); f32 takes the accurate ones.
+// sigmoid(z).  A bf16 result takes the hardware exponential and reciprocal (relative
+// error near 2^-21, far below bf16's 2^-9); f32 takes the accurate ones.  z far below 0
+// gives 1 / inf = 0.
 template <typename T>
 __device__ __forceinline__ float sigmoid(float z) {
-  if constexpr (std::is_same<T, float>::value) return 1.f / (1.f + expf(-z));
-  else return __fdividef(1.f, 1.f + __expf(fminf(-z, 80.f)));
+  if constexpr (std::is_same<T, float>::value) {
+    return 1.f / (1.f + expf(-z));
+  } else {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * z));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return r;
+  }
 }
 template <typename T, bool SILU>
 __device__ __forceinline__ float act(float z) {
@@ -86,8 +103,103 @@ __device__ __forceinline__ float dact(float z) {
   return s * (1.f + z * (1.f - s));
 }
 
+// Element-wise arithmetic on V values, two lanes an instruction where V is even: a bf16
+// pass at the HBM rate leaves about 20 instructions per value.
+template <int V>
+__device__ __forceinline__ float vsum(const float (&v)[V]) {
+  if constexpr (V % 2 == 0) {
+    float2 s = make_float2(v[0], v[1]);
+#pragma unroll
+    for (int i = 2; i < V; i += 2) s = fadd2(s, make_float2(v[i], v[i + 1]));
+    return s.x + s.y;
+  } else {
+    float s = v[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i) s += v[i];
+    return s;
+  }
+}
+// v += c
+template <int V>
+__device__ __forceinline__ void vadd(float (&v)[V], float c) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 r = fadd2(make_float2(v[i], v[i + 1]), make_float2(c, c));
+      v[i] = r.x;
+      v[i + 1] = r.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] += c;
+  }
+}
+// d = a * b + c (any of b, c broadcast by the caller's arrays)
+template <int V>
+__device__ __forceinline__ void vfma(float (&d)[V], const float (&a)[V], const float (&b)[V], const float (&c)[V]) {
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 r = ffma2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), make_float2(c[i], c[i + 1]));
+      d[i] = r.x;
+      d[i + 1] = r.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) d[i] = a[i] * b[i] + c[i];
+  }
+}
+template <int V>
+__device__ __forceinline__ void vscale(float (&d)[V], const float (&a)[V], float c) {   // d = a * c
+  if constexpr (V % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+      const float2 r = fmul2(make_float2(a[i], a[i + 1]), make_float2(c, c));
+      d[i] = r.x;
+      d[i + 1] = r.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) d[i] = a[i] * c;
+  }
+}
+template <int V>
+__device__ __forceinline__ float vdot(const float (&a)[V], const float (&b)[V]) {
+  if constexpr (V % 2 == 0) {
+    float2 s = fmul2(make_float2(a[0], a[1]), make_float2(b[0], b[1]));
+#pragma unroll
+    for (int i = 2; i < V; i += 2) s = ffma2(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), s);
+    return s.x + s.y;
+  } else {
+    float s = a[0] * b[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i) s += a[i] * b[i];
+    return s;
+  }
+}
+// What the backward needs of V values x with their dy: n = (x - mean) rstd into x, and
+// dz = dy act'(n w + b) into d.  sh = -mean rstd.
+template <typename T, int V, bool SILU>
+__device__ __forceinline__ void to_dz(float (&x)[V], float (&d)[V], const float (&w)[V], const float (&b)[V], float r,
+                                      float sh) {
+  float rr[V], ss[V], z[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    rr[i] = r;
+    ss[i] = sh;
+  }
+  vfma<V>(x, x, rr, ss);
+  if (SILU) {
+    vfma<V>(z, x, w, b);
+#pragma unroll
+    for (int i = 0; i < V; ++i) d[i] *= dact<T, true>(z[i]);
+  }
+}
+
 __device__ __forceinline__ float lane_sum(float v, int w) {
-  for (int o = w >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    if (o < w) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
 
@@ -98,11 +210,11 @@ struct TokenGeom {
 };
 
 template <typename T, int V, int NV, bool SILU>
-__global__ void __launch_bounds__(NT) gn_token_kernel(const T* __restrict__ x, const float* __restrict__ w,
+__global__ void __launch_bounds__(NT, NV == 1 ? 4 : NV == 2 ? 3 : 2) gn_token_kernel(const T* __restrict__ x, const float* __restrict__ w,
                                                       const float* __restrict__ b, T* __restrict__ y,
                                                       float* __restrict__ mean_o, float* __restrict__ rstd_o,
                                                       int64_t rows, int groups, int Cg, float eps, TokenGeom ge) {
-  constexpr int U = NV == 1 ? 4 : NV == 2 ? 2 : 1;   // rows in flight per thread
+  constexpr int U = NV == 1 ? 2 : 1;   // rows in flight per thread (more resident warps beat more rows)
   const int slot = threadIdx.x / ge.tl, lane = threadIdx.x % ge.tl;
   const int g = blockIdx.y * ge.gpb + slot % ge.gpb, rr = slot / ge.gpb;
   const bool live = rr < ge.rpb && g < groups;
@@ -122,46 +234,58 @@ __global__ void __launch_bounds__(NT) gn_token_kernel(const T* __restrict__ x, c
     }
   }
   const int64_t step = (int64_t)gridDim.x * ge.rpb;
-  // the loop bound is the block's, so that every lane of a warp takes part in the shuffles
-  for (int64_t r0 = (int64_t)blockIdx.x * ge.rpb; r0 < rows; r0 += step * U) {
-    float v[U][NV][V];
+  const int64_t off = (int64_t)g * Cg + lane * V;
+  // The next rows' loads go out before this row's arithmetic (as they lie in memory: half
+  // the registers of f32).  The loop bound is the block's, so that every lane of a warp
+  // takes part in the shuffles.
+  raw<T, V> nx[U][NV];
+  auto fetch = [&](int64_t r0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int64_t r = r0 + rr + u * step;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (has[j] && r < rows) vec<T, V>::ld(x + r * C + (int64_t)g * Cg + (lane + j * ge.tl) * V, v[u][j]);
-        else
-#pragma unroll
-          for (int i = 0; i < V; ++i) v[u][j][i] = 0.f;
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t r = r0 + rr + u * step;
-      float s = 0.f;
 #pragma unroll
       for (int j = 0; j < NV; ++j)
+        nx[u][j] = has[j] && r < rows ? ldr<T, V>(x + r * C + off + j * ge.tl * V) : raw<T, V>{};
+    }
+  };
+  int64_t r0 = (int64_t)blockIdx.x * ge.rpb;
+  fetch(r0);
+  for (; r0 < rows; r0 += step * U) {
+    raw<T, V> cur[U][NV];
 #pragma unroll
-        for (int i = 0; i < V; ++i) s += v[u][j][i];
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < NV; ++j) cur[u][j] = nx[u][j];
+    fetch(r0 + step * U);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t r = r0 + rr + u * step;
+      float v[NV][V];
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < NV; ++j) {
+        vec<T, V>::cvt(cur[u][j], v[j]);
+        s += vsum<V>(v[j]);
+      }
       const float mean = lane_sum(s, ge.tl) * inv;
       float m2 = 0.f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          v[u][j][i] -= mean;
-          m2 += has[j] ? v[u][j][i] * v[u][j][i] : 0.f;
-        }
-      const float rstd = 1.f / sqrtf(lane_sum(m2, ge.tl) * inv + eps);
+      for (int j = 0; j < NV; ++j) {
+        vadd<V>(v[j], -mean);
+        const float q = vdot<V>(v[j], v[j]);
+        m2 += has[j] ? q : 0.f;
+      }
+      const float rstd = rsqrtf(lane_sum(m2, ge.tl) * inv + eps);
       if (r >= rows) continue;   // after the shuffles
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
         if (!has[j]) continue;
         float o[V];
+        vscale<V>(o, v[j], rstd);
+        vfma<V>(o, o, wr[j], br[j]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = act<T, SILU>(v[u][j][i] * rstd * wr[j][i] + br[j][i]);
-        vec<T, V>::st(y + r * C + (int64_t)g * Cg + (lane + j * ge.tl) * V, o);
+        for (int i = 0; i < V; ++i) o[i] = act<T, SILU>(o[i]);
+        stv<T, V>(y + r * C + off + j * ge.tl * V, o);
       }
       if (mean_o && live && lane == 0) {
         mean_o[r * groups + g] = mean;
@@ -173,13 +297,12 @@ __global__ void __launch_bounds__(NT) gn_token_kernel(const T* __restrict__ x, c
 
 // Backward: dx, and per (block, row slot) partial sums of dw and db: part [2][parts][C].
 template <typename T, int V, int NV, bool SILU>
-__global__ void __launch_bounds__(NT) gn_token_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+__global__ void __launch_bounds__(NT, NV == 1 ? 3 : NV == 2 ? 2 : 1) gn_token_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                           const float* __restrict__ w, const float* __restrict__ b,
                                                           const float* __restrict__ mean_i,
                                                           const float* __restrict__ rstd_i, T* __restrict__ dx,
                                                           float* __restrict__ part, int64_t rows, int groups, int Cg,
                                                           TokenGeom ge) {
-  constexpr int U = NV == 1 ? 2 : 1;
   const int slot = threadIdx.x / ge.tl, lane = threadIdx.x % ge.tl;
   const int g = blockIdx.y * ge.gpb + slot % ge.gpb, rr = slot / ge.gpb;
   const bool live = rr < ge.rpb && g < groups;
@@ -200,54 +323,57 @@ __global__ void __launch_bounds__(NT) gn_token_bwd_kernel(const T* __restrict__ 
     }
   }
   const int64_t step = (int64_t)gridDim.x * ge.rpb;
-  for (int64_t r0 = (int64_t)blockIdx.x * ge.rpb; r0 < rows; r0 += step * U) {
-    float v[U][NV][V], d[U][NV][V], mean[U], rstd[U];
+  const int64_t off = (int64_t)g * Cg + lane * V;
+  raw<T, V> nx[NV], nd[NV];
+  float nm, nr;
+  auto fetch = [&](int64_t r0) {   // the next row, before this one's arithmetic
+    const int64_t r = r0 + rr;
+    const bool in = live && r < rows;
+    nm = in ? mean_i[r * groups + g] : 0.f;
+    nr = in ? rstd_i[r * groups + g] : 0.f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t r = r0 + rr + u * step;
-      const bool in = live && r < rows;
-      mean[u] = in ? mean_i[r * groups + g] : 0.f;
-      rstd[u] = in ? rstd_i[r * groups + g] : 0.f;
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int64_t at = r * C + (int64_t)g * Cg + (lane + j * ge.tl) * V;
-        if (has[j] && in) {
-          vec<T, V>::ld(x + at, v[u][j]);
-          vec<T, V>::ld(dy + at, d[u][j]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) v[u][j][i] = d[u][j][i] = 0.f;
-        }
-      }
+    for (int j = 0; j < NV; ++j) {
+      const bool ok = has[j] && in;
+      const int64_t at = r * C + off + j * ge.tl * V;
+      nx[j] = ok ? ldr<T, V>(x + at) : raw<T, V>{};
+      nd[j] = ok ? ldr<T, V>(dy + at) : raw<T, V>{};
     }
+  };
+  int64_t r0 = (int64_t)blockIdx.x * ge.rpb;
+  fetch(r0);
+  for (; r0 < rows; r0 += step) {
+    float v[NV][V], d[NV][V];
+    const float mean = nm, rstd = nr;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t r = r0 + rr + u * step;
-      float s0 = 0.f, s1 = 0.f;
+    for (int j = 0; j < NV; ++j) {
+      vec<T, V>::cvt(nx[j], v[j]);
+      vec<T, V>::cvt(nd[j], d[j]);
+    }
+    fetch(r0 + step);
+    const int64_t r = r0 + rr;
+    float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) {   // lanes without values have w = dy = 0
+      to_dz<T, V, SILU>(v[j], d[j], wr[j], br[j], rstd, -mean * rstd);
+      vfma<V>(aw[j], d[j], v[j], aw[j]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float n = (v[u][j][i] - mean[u]) * rstd[u];
-          const float dz = d[u][j][i] * dact<T, SILU>(n * wr[j][i] + br[j][i]);
-          aw[j][i] += dz * n;
-          ab[j][i] += dz;
-          v[u][j][i] = n;
-          d[u][j][i] = dz * wr[j][i];
-          s0 += d[u][j][i];
-          s1 += d[u][j][i] * n;
-        }
-      s0 = lane_sum(s0, ge.tl) * inv;
-      s1 = lane_sum(s1, ge.tl) * inv;
-      if (r >= rows) continue;   // after the shuffles
-#pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        if (!has[j]) continue;
-        float o[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = rstd[u] * (d[u][j][i] - s0 - v[u][j][i] * s1);
-        vec<T, V>::st(dx + r * C + (int64_t)g * Cg + (lane + j * ge.tl) * V, o);
+      for (int i = 0; i < V; ++i) {
+        ab[j][i] += d[j][i];
+        d[j][i] *= wr[j][i];
       }
+      s0 += vsum<V>(d[j]);
+      s1 += vdot<V>(d[j], v[j]);
+    }
+    s0 = lane_sum(s0, ge.tl) * inv;
+    s1 = lane_sum(s1, ge.tl) * inv;
+    if (r >= rows) continue;   // after the shuffles
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      if (!has[j]) continue;
+      float o[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = rstd * (d[j][i] - s0 - v[j][i] * s1);
+      stv<T, V>(dx + r * C + off + j * ge.tl * V, o);
     }
   }
   const int64_t parts = (int64_t)gridDim.x * ge.rpb;
@@ -300,7 +426,7 @@ constexpr int UR = 4;   // rows in flight per thread
 // (n, m, q) += (n2, m2, q2): counts, means, sums of squared deviations.
 __device__ __forceinline__ void chan(float& n, float& m, float& q, float n2, float m2, float q2) {
   if (n2 == 0.f) return;
-  const float t = n + n2, d = m2 - m, f = n2 / t;
+  const float t = n + n2, d = m2 - m, f = __fdividef(n2, t);
   m += d * f;
   q += q2 + d * d * n * f;
   n = t;
@@ -308,7 +434,7 @@ __device__ __forceinline__ void chan(float& n, float& m, float& q, float n2, flo
 
 // st [b][chunk][C / V] x (mean, squared deviations) of each thread column.
 template <typename T, int V>
-__global__ void __launch_bounds__(NT) gn_stats_kernel(const T* __restrict__ x, float2* __restrict__ st, int64_t L,
+__global__ void __launch_bounds__(NT, 4) gn_stats_kernel(const T* __restrict__ x, float2* __restrict__ st, int64_t L,
                                                       int64_t C, MapGeom ge) {
   __shared__ float sn[NT], sm[NT], sq[NT];
   const int tx = threadIdx.x % ge.cols, ty = threadIdx.x / ge.cols;
@@ -317,28 +443,35 @@ __global__ void __launch_bounds__(NT) gn_stats_kernel(const T* __restrict__ x, f
   float n = 0.f, m = 0.f, q = 0.f;
   if (ty < ge.rows_y && cv < ncv) {
     const T* p = x + ((int64_t)blockIdx.z * L) * C + cv * V;
+    raw<T, V> nx[UR];
+    auto fetch = [&](int64_t l) {
+#pragma unroll
+      for (int u = 0; u < UR; ++u) {
+        const int64_t lu = l + (int64_t)u * ge.rows_y;
+        nx[u] = lu < l1 ? ldr<T, V>(p + lu * C) : raw<T, V>{};
+      }
+    };
+    fetch(l0 + ty);
     for (int64_t l = l0 + ty; l < l1; l += (int64_t)ge.rows_y * UR) {
       float v[UR][V];
       float cnt = 0.f, s = 0.f;
 #pragma unroll
-      for (int u = 0; u < UR; ++u) {
-        const int64_t lu = l + (int64_t)u * ge.rows_y;
-        if (lu < l1) vec<T, V>::ld(p + lu * C, v[u]);
-      }
+      for (int u = 0; u < UR; ++u) vec<T, V>::cvt(nx[u], v[u]);
+      fetch(l + (int64_t)ge.rows_y * UR);
 #pragma unroll
       for (int u = 0; u < UR; ++u)
         if (l + (int64_t)u * ge.rows_y < l1) {
           cnt += V;
-#pragma unroll
-          for (int i = 0; i < V; ++i) s += v[u][i];
+          s += vsum<V>(v[u]);
         }
-      const float mu = s / cnt;
+      const float mu = __fdividef(s, cnt);
       float d2 = 0.f;
 #pragma unroll
       for (int u = 0; u < UR; ++u)
-        if (l + (int64_t)u * ge.rows_y < l1)
-#pragma unroll
-          for (int i = 0; i < V; ++i) d2 += (v[u][i] - mu) * (v[u][i] - mu);
+        if (l + (int64_t)u * ge.rows_y < l1) {
+          vadd<V>(v[u], -mu);
+          d2 += vdot<V>(v[u], v[u]);
+        }
       chan(n, m, q, cnt, mu, d2);
     }
   }
@@ -353,38 +486,50 @@ __global__ void __launch_bounds__(NT) gn_stats_kernel(const T* __restrict__ x, f
   }
 }
 
-// mean, rstd of one (b, g) per block, from the partial statistics.
+__device__ __forceinline__ float block_sum(float v, float* sm) {   // every thread gets the sum
+  v = lane_sum(v, 32);
+  if (threadIdx.x % 32 == 0) sm[threadIdx.x / 32] = v;
+  __syncthreads();
+  float t = 0.f;
+  for (int k = 0; k < (int)blockDim.x / 32; ++k) t += sm[k];
+  __syncthreads();
+  return t;
+}
+
+// mean, rstd of one (b, g) per block, from the partial statistics: their weighted mean,
+// then the squared deviations about it (two passes over values that stay in L1).
 __global__ void __launch_bounds__(NT) gn_merge_kernel(const float2* __restrict__ st, float* __restrict__ mean_o,
                                                       float* __restrict__ rstd_o, int64_t L, int64_t ncv, int per,
                                                       int V, int groups, int64_t chunk, int64_t nchunks, float eps) {
-  __shared__ float sn[NT], sm[NT], sq[NT];
+  __shared__ float sm[NT / 32];
   const int64_t b = blockIdx.y;
   const int g = blockIdx.x;
-  float n = 0.f, m = 0.f, q = 0.f;
-  for (int64_t i = threadIdx.x; i < nchunks * per; i += NT) {
-    const int64_t ck = i / per, c = (int64_t)g * per + (i - ck * per);
-    const float2 e = st[(b * nchunks + ck) * ncv + c];
-    chan(n, m, q, (float)(min(L, (ck + 1) * chunk) - ck * chunk) * V, e.x, e.y);
+  const float2* p = st + b * nchunks * ncv + (int64_t)g * per;
+  const int n = (int)(nchunks * per);
+  const float inv = 1.f / ((float)L * (float)(per * V)), last = (float)(L - (nchunks - 1) * chunk) * V;
+  float s = 0.f;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const int ck = i / per;
+    s += (ck == nchunks - 1 ? last : (float)chunk * V) * p[(int64_t)ck * ncv + (i - ck * per)].x;
   }
-  sn[threadIdx.x] = n;
-  sm[threadIdx.x] = m;
-  sq[threadIdx.x] = q;
-  __syncthreads();
-  for (int o = NT / 2; o > 0; o >>= 1) {
-    if (threadIdx.x < o) {
-      const int k = threadIdx.x + o;
-      chan(sn[threadIdx.x], sm[threadIdx.x], sq[threadIdx.x], sn[k], sm[k], sq[k]);
-    }
-    __syncthreads();
+  const float mean = block_sum(s, sm) * inv;
+  float q = 0.f;
+#pragma unroll 4
+  for (int i = threadIdx.x; i < n; i += NT) {
+    const int ck = i / per;
+    const float2 e = p[(int64_t)ck * ncv + (i - ck * per)];
+    q += e.y + (ck == nchunks - 1 ? last : (float)chunk * V) * (e.x - mean) * (e.x - mean);
   }
+  q = block_sum(q, sm);
   if (threadIdx.x == 0) {
-    mean_o[b * groups + g] = sm[0];
-    rstd_o[b * groups + g] = 1.f / sqrtf(sq[0] / sn[0] + eps);
+    mean_o[b * groups + g] = mean;
+    rstd_o[b * groups + g] = rsqrtf(q * inv + eps);
   }
 }
 
 template <typename T, int V, bool SILU>
-__global__ void __launch_bounds__(NT) gn_apply_kernel(const T* __restrict__ x, const float* __restrict__ w,
+__global__ void __launch_bounds__(NT, 4) gn_apply_kernel(const T* __restrict__ x, const float* __restrict__ w,
                                                       const float* __restrict__ b, const float* __restrict__ mean,
                                                       const float* __restrict__ rstd, T* __restrict__ y, int64_t L,
                                                       int64_t C, int groups, int Cg, MapGeom ge) {
@@ -402,27 +547,38 @@ __global__ void __launch_bounds__(NT) gn_apply_kernel(const T* __restrict__ x, c
   const int64_t l0 = (int64_t)blockIdx.x * ge.chunk, l1 = min(L, l0 + ge.chunk);
   const T* px = x + bz * L * C + c;
   T* py = y + bz * L * C + c;
-  for (int64_t l = l0 + ty; l < l1; l += (int64_t)ge.rows_y * UR) {
-    float v[UR][V];
+  raw<T, V> nx[UR];
+  auto fetch = [&](int64_t l) {
 #pragma unroll
     for (int u = 0; u < UR; ++u) {
       const int64_t lu = l + (int64_t)u * ge.rows_y;
-      if (lu < l1) vec<T, V>::ld(px + lu * C, v[u]);
+      nx[u] = lu < l1 ? ldr<T, V>(px + lu * C) : raw<T, V>{};
     }
+  };
+  fetch(l0 + ty);
+  for (int64_t l = l0 + ty; l < l1; l += (int64_t)ge.rows_y * UR) {
+    raw<T, V> cur[UR];
+#pragma unroll
+    for (int u = 0; u < UR; ++u) cur[u] = nx[u];
+    fetch(l + (int64_t)ge.rows_y * UR);
 #pragma unroll
     for (int u = 0; u < UR; ++u) {
       const int64_t lu = l + (int64_t)u * ge.rows_y;
       if (lu >= l1) break;
+      float v[V];
+      vec<T, V>::cvt(cur[u], v);
+      vadd<V>(v, -m);
+      vfma<V>(v, v, a, o);
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[u][i] = act<T, SILU>((v[u][i] - m) * a[i] + o[i]);
-      vec<T, V>::st(py + lu * C, v[u]);
+      for (int i = 0; i < V; ++i) v[i] = act<T, SILU>(v[i]);
+      stv<T, V>(py + lu * C, v);
     }
   }
 }
 
 // part [b][chunk][2][C]: sums of dz n and dz over the chunk's rows.
 template <typename T, int V, bool SILU>
-__global__ void __launch_bounds__(NT) gn_bwd_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+__global__ void __launch_bounds__(NT, 2) gn_bwd_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                          const float* __restrict__ w, const float* __restrict__ b,
                                                          const float* __restrict__ mean,
                                                          const float* __restrict__ rstd, float* __restrict__ part,
@@ -444,26 +600,33 @@ __global__ void __launch_bounds__(NT) gn_bwd_sums_kernel(const T* __restrict__ d
     }
     const int64_t l0 = (int64_t)blockIdx.x * ge.chunk, l1 = min(L, l0 + ge.chunk);
     const int64_t base = bz * L * C + c;
-    for (int64_t l = l0 + ty; l < l1; l += (int64_t)ge.rows_y * UR) {
-      float v[UR][V], d[UR][V];
+    raw<T, V> nx[UR], nd[UR];
+    auto fetch = [&](int64_t l) {
 #pragma unroll
       for (int u = 0; u < UR; ++u) {
         const int64_t lu = l + (int64_t)u * ge.rows_y;
-        if (lu < l1) {
-          vec<T, V>::ld(x + base + lu * C, v[u]);
-          vec<T, V>::ld(dy + base + lu * C, d[u]);
-        }
+        nx[u] = lu < l1 ? ldr<T, V>(x + base + lu * C) : raw<T, V>{};
+        nd[u] = lu < l1 ? ldr<T, V>(dy + base + lu * C) : raw<T, V>{};
       }
+    };
+    fetch(l0 + ty);
+    for (int64_t l = l0 + ty; l < l1; l += (int64_t)ge.rows_y * UR) {
+      raw<T, V> cx[UR], cd[UR];
 #pragma unroll
       for (int u = 0; u < UR; ++u) {
-        if (l + (int64_t)u * ge.rows_y >= l1) break;
+        cx[u] = nx[u];
+        cd[u] = nd[u];
+      }
+      fetch(l + (int64_t)ge.rows_y * UR);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float n = (v[u][i] - m) * r;
-          const float dz = d[u][i] * dact<T, SILU>(n * wr[i] + br[i]);
-          aw[i] += dz * n;
-          ab[i] += dz;
-        }
+      for (int u = 0; u < UR; ++u) {   // rows behind the chunk have dy = 0
+        float v[V], d[V];
+        vec<T, V>::cvt(cx[u], v);
+        vec<T, V>::cvt(cd[u], d);
+        to_dz<T, V, SILU>(v, d, wr, br, r, -m * r);
+        vfma<V>(aw, d, v, aw);
+#pragma unroll
+        for (int i = 0; i < V; ++i) ab[i] += d[i];
       }
     }
   }
@@ -489,49 +652,59 @@ __global__ void __launch_bounds__(NT) gn_bwd_sums_kernel(const T* __restrict__ d
   }
 }
 
-// One (b, g) per block: per-channel sums over the chunks into chan_sum [2][Bt][C], and the
-// group means of gr and gr n into gm [Bt][groups] (x: mean gr, y: mean gr n).
-__global__ void __launch_bounds__(NT) gn_bwd_merge_kernel(const float* __restrict__ part, const float* __restrict__ w,
-                                                          float* __restrict__ chan_sum, float2* __restrict__ gm,
-                                                          int64_t L, int64_t C, int groups, int Cg, int64_t nchunks,
-                                                          int64_t Bt, int64_t b0) {
-  __shared__ float sa[NT / 32], sb[NT / 32];
+// One (b, g) per block of 1024: per-channel sums over the chunks into chan_sum [2][Bt][C], and
+// the group means of gr and gr n into gm [Bt][groups] (x: mean gr, y: mean gr n).  A warp per
+// 32 channels and every 32nd chunk.
+__global__ void __launch_bounds__(1024) gn_bwd_merge_kernel(const float* __restrict__ part, const float* __restrict__ w,
+                                                            float* __restrict__ chan_sum, float2* __restrict__ gm,
+                                                            int64_t L, int64_t C, int groups, int Cg, int64_t nchunks,
+                                                            int64_t Bt, int64_t b0) {
+  __shared__ float sa[32][33], sb[32][33];
   const int64_t b = blockIdx.y;
-  const int g = blockIdx.x;
+  const int g = blockIdx.x, tx = threadIdx.x % 32, ty = threadIdx.x / 32;
   float ga = 0.f, gb = 0.f;
-  for (int i = threadIdx.x; i < Cg; i += NT) {
-    const int64_t c = (int64_t)g * Cg + i;
+  for (int i0 = 0; i0 < Cg; i0 += 32) {
+    const int64_t c = (int64_t)g * Cg + i0 + tx;
+    const bool in = i0 + tx < Cg;
     float a = 0.f, d = 0.f;
+    if (in) {
 #pragma unroll 4
-    for (int64_t k = 0; k < nchunks; ++k) {
-      const float* p = part + (b * nchunks + k) * 2 * C + c;
-      a += p[0];
-      d += p[C];
+      for (int64_t k = ty; k < nchunks; k += 32) {
+        const float* p = part + (b * nchunks + k) * 2 * C + c;
+        a += p[0];
+        d += p[C];
+      }
     }
-    chan_sum[(b0 + b) * C + c] = a;
-    chan_sum[(Bt + b0 + b) * C + c] = d;
-    ga += a * w[c];
-    gb += d * w[c];
+    sa[ty][tx] = a;
+    sb[ty][tx] = d;
+    __syncthreads();
+    // the 32 partial sums of a channel: a warp per channel, chunks across its lanes
+    a = lane_sum(sa[tx][ty], 32);
+    d = lane_sum(sb[tx][ty], 32);
+    if (tx == 0 && i0 + ty < Cg) {
+      const int64_t cc = (int64_t)g * Cg + i0 + ty;
+      chan_sum[(b0 + b) * C + cc] = a;
+      chan_sum[(Bt + b0 + b) * C + cc] = d;
+      ga += a * w[cc];
+      gb += d * w[cc];
+    }
+    __syncthreads();
   }
-  ga = lane_sum(ga, 32);
-  gb = lane_sum(gb, 32);
-  if (threadIdx.x % 32 == 0) {
-    sa[threadIdx.x / 32] = ga;
-    sb[threadIdx.x / 32] = gb;
+  if (tx == 0) {
+    sa[0][ty] = ga;
+    sb[0][ty] = gb;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int k = 1; k < NT / 32; ++k) {
-      sa[0] += sa[k];
-      sb[0] += sb[k];
-    }
+  if (ty == 0) {
+    ga = lane_sum(sa[0][tx], 32);
+    gb = lane_sum(sb[0][tx], 32);
     const float inv = 1.f / ((float)L * (float)Cg);
-    gm[b * groups + g] = make_float2(sb[0] * inv, sa[0] * inv);
+    if (tx == 0) gm[b * groups + g] = make_float2(gb * inv, ga * inv);
   }
 }
 
 template <typename T, int V, bool SILU>
-__global__ void __launch_bounds__(NT) gn_bwd_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x,
+__global__ void __launch_bounds__(NT, 2) gn_bwd_apply_kernel(const T* __restrict__ dy, const T* __restrict__ x,
                                                           const float* __restrict__ w, const float* __restrict__ b,
                                                           const float* __restrict__ mean,
                                                           const float* __restrict__ rstd,
@@ -551,27 +724,35 @@ __global__ void __launch_bounds__(NT) gn_bwd_apply_kernel(const T* __restrict__ 
   }
   const int64_t l0 = (int64_t)blockIdx.x * ge.chunk, l1 = min(L, l0 + ge.chunk);
   const int64_t base = bz * L * C + c;
-  for (int64_t l = l0 + ty; l < l1; l += (int64_t)ge.rows_y * UR) {
-    float v[UR][V], d[UR][V];
+  raw<T, V> nx[UR], nd[UR];
+  auto fetch = [&](int64_t l) {
 #pragma unroll
     for (int u = 0; u < UR; ++u) {
       const int64_t lu = l + (int64_t)u * ge.rows_y;
-      if (lu < l1) {
-        vec<T, V>::ld(x + base + lu * C, v[u]);
-        vec<T, V>::ld(dy + base + lu * C, d[u]);
-      }
+      nx[u] = lu < l1 ? ldr<T, V>(x + base + lu * C) : raw<T, V>{};
+      nd[u] = lu < l1 ? ldr<T, V>(dy + base + lu * C) : raw<T, V>{};
     }
+  };
+  fetch(l0 + ty);
+  for (int64_t l = l0 + ty; l < l1; l += (int64_t)ge.rows_y * UR) {
+    raw<T, V> cx[UR], cd[UR];
+#pragma unroll
+    for (int u = 0; u < UR; ++u) {
+      cx[u] = nx[u];
+      cd[u] = nd[u];
+    }
+    fetch(l + (int64_t)ge.rows_y * UR);
 #pragma unroll
     for (int u = 0; u < UR; ++u) {
       const int64_t lu = l + (int64_t)u * ge.rows_y;
       if (lu >= l1) break;
+      float v[V], d[V];
+      vec<T, V>::cvt(cx[u], v);
+      vec<T, V>::cvt(cd[u], d);
+      to_dz<T, V, SILU>(v, d, wr, br, r, -m * r);
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float n = (v[u][i] - m) * r;
-        const float gr = d[u][i] * dact<T, SILU>(n * wr[i] + br[i]) * wr[i];
-        v[u][i] = r * (gr - mm.x - n * mm.y);
-      }
-      vec<T, V>::st(dx + base + lu * C, v[u]);
+      for (int i = 0; i < V; ++i) v[i] = r * (d[i] * wr[i] - mm.x - v[i] * mm.y);
+      stv<T, V>(dx + base + lu * C, v);
     }
   }
 }
@@ -615,16 +796,17 @@ int64_t token_blocks(const TokenGeom& ge, int64_t rows, int per_sm) {
   const int64_t want = cdiv((int64_t)num_sms() * per_sm, ge.cblocks);
   return std::max<int64_t>(1, std::min(want, cdiv(rows, ge.rpb)));
 }
-constexpr int TOKEN_BWD_PER_SM = 4;
+constexpr int TOKEN_BWD_PER_SM = 3;
 
-MapGeom map_geom(int64_t Bt, int64_t L, int64_t C, int V) {
+MapGeom map_geom(int64_t Bt, int64_t L, int64_t C, int V, bool bwd) {
   MapGeom ge;
   const int64_t ncv = C / V;
   ge.cblocks = (int)cdiv(ncv, NT);
   ge.cols = (int)cdiv(ncv, ge.cblocks);
   ge.rows_y = NT / ge.cols;
-  // about eight blocks per SM over the batch, and no chunk below one unrolled pass
-  const int64_t want = std::max<int64_t>(1, cdiv((int64_t)num_sms() * 8, Bt * ge.cblocks));
+  // one set of resident blocks over the batch (launch bounds: 4 per SM forward, 2 backward),
+  // and no chunk below one unrolled pass
+  const int64_t want = std::max<int64_t>(1, (int64_t)num_sms() * (bwd ? 2 : 4) / (Bt * ge.cblocks));
   ge.chunk = std::max<int64_t>(cdiv(L, want), (int64_t)ge.rows_y * UR);
   ge.nchunks = cdiv(L, ge.chunk);
   return ge;
@@ -637,7 +819,7 @@ int64_t batch_piece(int64_t Bt, int64_t bytes_per_row) {
 
 // Workspace of the L > 1 passes: partial sums of one piece, group means, per-row channel sums.
 int64_t map_part_floats(int64_t piece, int64_t L, int64_t C, int V, bool train) {
-  const MapGeom ge = map_geom(piece, L, C, V);
+  const MapGeom ge = map_geom(piece, L, C, V, train);
   return piece * ge.nchunks * 2 * (train ? C : C / V);
 }
 
@@ -671,7 +853,7 @@ void token_bwd(const Norm& a, const TokenGeom& ge, int nv) {
 template <typename T, int V, bool SILU>
 void map_fwd(const Norm& a) {
   const int64_t row = a.L * a.C, piece = batch_piece(a.Bt, row * sizeof(T));
-  const MapGeom ge = map_geom(piece, a.L, a.C, V);
+  const MapGeom ge = map_geom(piece, a.L, a.C, V, false);
   float2* st = (float2*)a.ws;
   for (int64_t b0 = 0; b0 < a.Bt; b0 += piece) {
     const int64_t nb = std::min(piece, a.Bt - b0);
@@ -689,7 +871,7 @@ void map_fwd(const Norm& a) {
 template <typename T, int V, bool SILU>
 void map_bwd(const Norm& a) {
   const int64_t row = a.L * a.C, piece = batch_piece(a.Bt, 2 * row * sizeof(T));
-  const MapGeom ge = map_geom(piece, a.L, a.C, V);
+  const MapGeom ge = map_geom(piece, a.L, a.C, V, true);
   float* part = (float*)a.ws;
   float* chan_sum = part + map_part_floats(piece, a.L, a.C, V, true);
   float2* gm = (float2*)(chan_sum + 2 * a.Bt * a.C);
@@ -700,7 +882,7 @@ void map_bwd(const Norm& a) {
     const float *mean = (const float*)a.mean + b0 * a.groups, *rstd = (const float*)a.rstd + b0 * a.groups;
     gn_bwd_sums_kernel<T, V, SILU><<<grid, NT, 0, a.st>>>(dy, x, (const float*)a.w, (const float*)a.b, mean, rstd,
                                                           part, a.L, a.C, a.groups, a.Cg, ge);
-    gn_bwd_merge_kernel<<<dim3((unsigned)a.groups, (unsigned)nb), NT, 0, a.st>>>(
+    gn_bwd_merge_kernel<<<dim3((unsigned)a.groups, (unsigned)nb), 1024, 0, a.st>>>(
         part, (const float*)a.w, chan_sum, gm, a.L, a.C, a.groups, a.Cg, ge.nchunks, a.Bt, b0);
     gn_bwd_apply_kernel<T, V, SILU><<<grid, NT, 0, a.st>>>(dy, x, (const float*)a.w, (const float*)a.b, mean, rstd,
                                                            gm, (T*)a.y + b0 * row, a.L, a.C, a.groups, a.Cg, ge);
