@@ -120,13 +120,36 @@ class _Same:
 
 
 _SAME = _Same()
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def device_of(t):
-    """A context in which t's device is the current one (launches and the
-    device's status word follow the current device)."""
-    i = t.device.index
-    return _SAME if i is None or i == torch.cuda.current_device() else torch.cuda.device(t.device)
+def same_device(first, *rest):
+    """The index of the CUDA device that all the tensors (None is skipped) are on."""
+    d = first.get_device() if isinstance(first, torch.Tensor) else -1
+    if d < 0:
+        raise ValueError("tssm_b200 operators take CUDA tensors (no CPU fallback)")
+    for t in rest:
+        if t is not None and (not isinstance(t, torch.Tensor) or t.get_device() != d):
+            if not isinstance(t, torch.Tensor) or not t.is_cuda:
+                raise ValueError("tssm_b200 operators take CUDA tensors (no CPU fallback)")
+            raise ValueError("all tensors must be on the same device")
+    return d
+
+
+def on_device(index):
+    """A context in which that device is the current one (launches and the device's status
+    word follow the current device)."""
+    return _SAME if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def raw_stream(index):
+    """The device's current stream as an integer."""
+    return _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream
+
+
+def addr(t):
+    """A tensor's address as an integer (None: null)."""
+    return t.data_ptr() if t is not None else None
 
 
 def ptr(t):

@@ -9,8 +9,8 @@ of the inputs' device.
 import torch
 
 from . import _lib
-from ._lib import call, device_of, dtype_code, ptr, stream_of
-from .ops import _cuda, _need
+from ._lib import addr, call, dtype_code, on_device, raw_stream, same_device
+from .ops import _need
 
 __all__ = ["group_norm_act", "group_norm_act_bwd"]
 
@@ -24,7 +24,7 @@ def _norm_args(name, x, weight, bias, groups, act):
     if x.dim() not in (2, 3):
         raise ValueError("%s: expected x [Bt,L,C] or [rows,C]" % name)
     C = x.shape[-1]
-    if tuple(weight.shape) != (C,) or tuple(bias.shape) != (C,):
+    if weight.shape != (C,) or bias.shape != (C,):
         raise ValueError("%s: weight and bias must be [C]" % name)
     if groups < 1 or C % groups:
         raise ValueError("%s: C (%d) must be a multiple of groups (%d)" % (name, C, groups))
@@ -48,7 +48,7 @@ def group_norm_act(x, weight, bias, groups, eps=1e-5, act="silu", return_stats=F
     Returns y in x's dtype, or (y, mean, rstd) with the statistics
     [Bt,groups] f32 when ``return_stats`` (the backward takes them).
     """
-    _cuda(x, weight, bias, y)
+    dev = same_device(x, weight, bias, y)
     groups = int(groups)
     Bt, L, C = _norm_args("group_norm_act", x, weight, bias, groups, act)
     x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
@@ -56,16 +56,19 @@ def group_norm_act(x, weight, bias, groups, eps=1e-5, act="silu", return_stats=F
         y = torch.empty_like(x)
     elif y.shape != x.shape or y.dtype != x.dtype or not y.is_contiguous():
         raise ValueError("group_norm_act: y must be contiguous and match x")
-    mean = rstd = None
-    if return_stats or L != 1 or C // groups > 128:
+    mean = rstd = ws = None
+    need = 0
+    narrow = L == 1 and C // groups <= 128   # needs neither statistics nor workspace
+    if return_stats or not narrow:
         mean, rstd = torch.empty(2, Bt, groups, device=x.device, dtype=torch.float32)
         if L == 0:
             mean.zero_()
             rstd.fill_(float(eps) ** -0.5)
-    ws, need = _workspace(x, Bt, L, C, groups, False)
-    with device_of(x):
-        call("tssm_group_norm_act", ptr(x), ptr(weight), ptr(bias), ptr(y), ptr(mean), ptr(rstd), ptr(ws), need, Bt, L,
-             C, groups, float(eps), _ACT[act], dtype_code(x), stream_of(x))
+    if not narrow:
+        ws, need = _workspace(x, Bt, L, C, groups, False)
+    with on_device(dev):
+        call("tssm_group_norm_act", addr(x), addr(weight), addr(bias), addr(y), addr(mean), addr(rstd), addr(ws), need, Bt, L,
+             C, groups, float(eps), _ACT[act], dtype_code(x), raw_stream(dev))
     return (y, mean, rstd) if return_stats else y
 
 
@@ -76,7 +79,7 @@ def group_norm_act_bwd(dy, x, weight, bias, mean, rstd, act="silu"):
     [Bt,groups] f32 from the forward.  Returns (dx in x's dtype, dweight [C],
     dbias [C] f32); the sums over rows run in a fixed order.
     """
-    _cuda(dy, x, weight, bias, mean, rstd)
+    dev = same_device(x, dy, weight, bias, mean, rstd)
     if mean.dim() != 2 or mean.shape != rstd.shape or mean.dtype != torch.float32 or rstd.dtype != torch.float32:
         raise ValueError("group_norm_act_bwd: mean and rstd must be [Bt,groups] f32")
     groups = mean.shape[1]
@@ -87,7 +90,7 @@ def group_norm_act_bwd(dy, x, weight, bias, mean, rstd, act="silu"):
     dx = torch.empty_like(x)
     dw, db = torch.empty(2, C, device=x.device, dtype=torch.float32)
     ws, need = _workspace(x, Bt, L, C, groups, True)
-    with device_of(x):
-        call("tssm_group_norm_act_bwd", ptr(dy), ptr(x), ptr(weight), ptr(bias), ptr(mean), ptr(rstd), ptr(dx),
-             ptr(dw), ptr(db), ptr(ws), need, Bt, L, C, groups, _ACT[act], dtype_code(x), stream_of(x))
+    with on_device(dev):
+        call("tssm_group_norm_act_bwd", addr(dy), addr(x), addr(weight), addr(bias), addr(mean), addr(rstd), addr(dx),
+             addr(dw), addr(db), addr(ws), need, Bt, L, C, groups, _ACT[act], dtype_code(x), raw_stream(dev))
     return dx, dw, db
