@@ -261,38 +261,78 @@ struct GradSmem {
                        S = DE + 3 * SQ_BYTES, G = S + 3 * PLANE, VEC = G + (int)sizeof(Gates);
   static constexpr int M1 = E, M2 = DE;           // after the channel loop
   static constexpr int Y = S;                     // 64 x 65 floats, after it too
-  static constexpr int BYTES = VEC + (2 * Q * 3 + Q * 4 + 16) * 4 + 128;
+  static constexpr int BYTES = VEC + (4 * Q * 3 + Q * 8 + 16) * 4 + 128;
   static_assert(3 * PLANE >= Q * 65 * 4, "Y fits the state region");
 };
+constexpr int GT = 512;   // threads: warp = (16 tokens, a quarter of N)
+
+// Eight f32 of a tile's piece (row r, columns 8 c ..), zeros outside.
+__device__ __forceinline__ void fetch8(const float* src, int64_t stride, int rows, int valid, bool vec, int r, int c,
+                                       float (&f)[8]) {
+  if (vec) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float4 v = r < rows && 8 * c + 4 * q < valid
+                           ? *reinterpret_cast<const float4*>(src + (int64_t)r * stride + 8 * c + 4 * q)
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+      f[4 * q] = v.x; f[4 * q + 1] = v.y; f[4 * q + 2] = v.z; f[4 * q + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = r < rows && 8 * c + e < valid ? src[(int64_t)r * stride + 8 * c + e] : 0.f;
+  }
+}
+__device__ __forceinline__ void put8(uint8_t* dst, int plane, const float (&f)[8]) {
+  uint32_t w[4][3];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) split2<3>(f[2 * q], f[2 * q + 1], w[q]);
+#pragma unroll
+  for (int z = 0; z < 3; ++z)
+    *reinterpret_cast<uint4*>(dst + z * plane) = make_uint4(w[0][z], w[1][z], w[2][z], w[3][z]);
+}
 
 template <int XS, int KN>
-__global__ void __launch_bounds__(256, 1) delta_bwd_grad_kernel(const BwdArgs a) {
+__global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) {
   using T = typename std::conditional<XS == 1, __nv_bfloat16, float>::type;
   using SM = GradSmem<XS, KN>;
-  constexpr int RB = KN * 2, NTH = KN / 16;   // 8-wide tiles of a warp's half of N
+  constexpr int RB = KN * 2, NTQ = KN / 32;   // 8-wide tiles of a warp's quarter of N
+  constexpr int SP = KN / 64;                 // pieces of a 64 x KN state tile per thread
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((128u - (smem_addr(smem_raw) & 127u)) & 127u);
   const uint32_t s = smem_addr(smem);
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  const int mt = warp % 4, half = warp / 4, pr = lane / 4, q2 = 2 * (lane % 4);
+  const int mt = warp % 4, qt = warp / 4, pr = lane / 4, q2 = 2 * (lane % 4);
   const int64_t bh = blockIdx.x / a.nc, c = blockIdx.x - bh * a.nc, b = bh / a.H;
   const int h = (int)(bh - b * a.H), g = h / (a.H / a.G);
   const int64_t t0 = c * Q, su = (int64_t)a.H * a.P, sk = (int64_t)a.G * a.N;
   const int rows = (int)min((int64_t)Q, a.L - t0);
   Gates& gt = *reinterpret_cast<Gates*>(smem + SM::G);
   float* vec = reinterpret_cast<float*>(smem + SM::VEC);
-  float *va = vec, *vb = vec + 2 * Q, *vw = vec + 4 * Q;   // [2][Q] row dots of a, b, and w e.(K dS1)
-  float* seg = vec + 6 * Q;                                // [4][Q] column sums of Y by row quarter
-  float* red = seg + 4 * Q;                                // [8] <S0, dS1> by warp
+  float *va = vec, *vb = vec + 4 * Q, *vw = vec + 8 * Q;   // [4][Q] row dots of a, b, and w e.(K dS1), by quarter
+  float* seg = vec + 12 * Q;                               // [8][Q] column sums of Y by row eighth
+  float* red = seg + 8 * Q;                                // [16] <S0, dS1> by warp
 
-  load_planes<XS, KN, 256>(s + SM::K, SM::PLANE, (const T*)a.B + (b * a.L + t0) * sk + (int64_t)g * a.N, sk, rows, a.N,
-                           a.vec_kq, tid);
-  load_planes<XS, KN, 256>(s + SM::QQ, SM::PLANE, (const T*)a.C + (b * a.L + t0) * sk + (int64_t)g * a.N, sk, rows, a.N,
-                           a.vec_kq, tid);
+  const float* S0 = a.states + ((bh * a.nc + c) * a.P) * (int64_t)a.N;
+  const float* dS = a.dstates + ((bh * a.nc + c) * a.P) * (int64_t)a.N;
+  const int64_t tok = (b * a.L + t0) * su + (int64_t)h * a.P;
+  // A thread's pieces: row er, piece ec of the 64 x 64 tiles; rows sr, piece sc of the state's.
+  const int er = tid / 8, ec = tid % 8, sr = tid / (KN / 8), sc = tid % (KN / 8);
+  constexpr int SR = GT / (KN / 8);   // state rows between a thread's pieces
+  float fs[SP][8];                    // the next state pieces, in flight during the products
+  auto fetch_state = [&](const float* src, int p0) {
+#pragma unroll
+    for (int i = 0; i < SP; ++i)
+      fetch8(src + (int64_t)p0 * a.N, a.N, min(64, a.P - p0), a.N, a.vec_n4, sr + i * SR, sc, fs[i]);
+  };
+  fetch_state(S0, 0);
+  load_planes<XS, KN, GT>(s + SM::K, SM::PLANE, (const T*)a.B + (b * a.L + t0) * sk + (int64_t)g * a.N, sk, rows, a.N,
+                          a.vec_kq, tid);
+  load_planes<XS, KN, GT>(s + SM::QQ, SM::PLANE, (const T*)a.C + (b * a.L + t0) * sk + (int64_t)g * a.N, sk, rows, a.N,
+                          a.vec_kq, tid);
   if (warp == 0)
     gates_warp(gt, a.dt + b * a.L * a.H + h, a.beta + b * a.L * a.H + h, a.H, a.A_log[h], t0, a.L, lane);
 
-  float dq0[NTH][4], dk0[NTH][4], dk1[NTH][4], m1[4][4], m2[4][4];
+  float dq0[NTQ][4], dk0[NTQ][4], dk1[NTQ][4], m1[2][4], m2[2][4];
   auto zero = [](auto& m) {
     for (auto& r : m)
       for (float& v : r) v = 0.f;
@@ -303,18 +343,22 @@ __global__ void __launch_bounds__(256, 1) delta_bwd_grad_kernel(const BwdArgs a)
   zero(m1);
   zero(m2);
   float dot = 0.f;
-  const float* S0 = a.states + ((bh * a.nc + c) * a.P) * (int64_t)a.N;
-  const float* dS = a.dstates + ((bh * a.nc + c) * a.P) * (int64_t)a.N;
-  const int64_t tok = (b * a.L + t0) * su + (int64_t)h * a.P;
   for (int p0 = 0; p0 < a.P; p0 += 64) {
     const int pv = min(64, a.P - p0);
-    __syncthreads();
-    load_planes<XS, 64, 256>(s + SM::DO, SQ_BYTES, (const T*)a.dy + tok + p0, su, rows, pv, a.vec_v, tid);
-    load_planes<3, 64, 256>(s + SM::E, SQ_BYTES, a.errs + tok + p0, su, rows, pv, a.vec_p4, tid);
-    load_planes<3, 64, 256>(s + SM::DE, SQ_BYTES, a.derrs + tok + p0, su, rows, pv, a.vec_p4, tid);
-    load_planes<3, KN, 256>(s + SM::S, SM::PLANE, S0 + (int64_t)p0 * a.N, a.N, pv, a.N, a.vec_n4, tid);
+    if (p0) __syncthreads();
+    {
+      float fe[8], fd[8];
+      fetch8(a.errs + tok + p0, su, rows, pv, a.vec_p4, er, ec, fe);
+      fetch8(a.derrs + tok + p0, su, rows, pv, a.vec_p4, er, ec, fd);
+      load_planes<XS, 64, GT>(s + SM::DO, SQ_BYTES, (const T*)a.dy + tok + p0, su, rows, pv, a.vec_v, tid);
+#pragma unroll
+      for (int i = 0; i < SP; ++i) put8(smem + SM::S + tile_off<RB>(sr + i * SR, sc), SM::PLANE, fs[i]);
+      put8(smem + SM::E + tile_off<SQ_RB>(er, ec), SQ_BYTES, fe);
+      put8(smem + SM::DE + tile_off<SQ_RB>(er, ec), SQ_BYTES, fd);
+    }
     cp_async_wait_all();
     __syncthreads();
+    fetch_state(dS, p0);
 #pragma unroll 1
     for (int kk = 0; kk < 4; ++kk) {
       uint32_t fo[XS][4], fe[3][4], w[3][4];
@@ -322,86 +366,66 @@ __global__ void __launch_bounds__(256, 1) delta_bwd_grad_kernel(const BwdArgs a)
       for (int z = 0; z < XS; ++z) ldsm4(fo[z], at_a<SQ_RB>(s + SM::DO + z * SQ_BYTES, 16 * mt, 2 * kk, lane));
 #pragma unroll
       for (int z = 0; z < 3; ++z) ldsm4(fe[z], at_a<SQ_RB>(s + SM::DE + z * SQ_BYTES, 16 * mt, 2 * kk, lane));
+      if (qt <= mt) {
 #pragma unroll
-      for (int np = 0; np < 2; ++np) {
-        if (2 * half + np > mt) break;
-#pragma unroll
-        for (int z = 0; z < 3; ++z)
-          ldsm4(w[z], at_b<SQ_RB>(s + SM::E + z * SQ_BYTES, 32 * half + 16 * np, 2 * kk, lane));
-        mma_planes<XS, 3, 3>(m1[2 * np], m1[2 * np + 1], fo, w);
-        mma_planes<3, 3, 3>(m2[2 * np], m2[2 * np + 1], fe, w);
+        for (int z = 0; z < 3; ++z) ldsm4(w[z], at_b<SQ_RB>(s + SM::E + z * SQ_BYTES, 16 * qt, 2 * kk, lane));
+        mma_planes<XS, 3, 3>(m1[0], m1[1], fo, w);
+        mma_planes<3, 3, 3>(m2[0], m2[1], fe, w);
       }
 #pragma unroll
-      for (int nn = 0; nn < NTH / 2; ++nn) {
+      for (int nn = 0; nn < NTQ / 2; ++nn) {
 #pragma unroll
-        for (int z = 0; z < 3; ++z)
-          ldsm4t(w[z], at_a<RB>(s + SM::S + z * SM::PLANE, 16 * kk, half * NTH + 2 * nn, lane));
+        for (int z = 0; z < 3; ++z) ldsm4t(w[z], at_a<RB>(s + SM::S + z * SM::PLANE, 16 * kk, qt * NTQ + 2 * nn, lane));
         mma_planes<XS, 3, 3>(dq0[2 * nn], dq0[2 * nn + 1], fo, w);
         mma_planes<3, 3, 3>(dk0[2 * nn], dk0[2 * nn + 1], fe, w);
       }
     }
     __syncthreads();
     // dS1 takes S0's place; <S0, dS1> on the way (the planes of S0 add up to its f32 values)
-    for (int i = tid; i < 64 * (KN / 8); i += 256) {
-      const int r = i / (KN / 8), cc = i % (KN / 8);
-      float f[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = 0.f;
-      if (r < pv) {
-        const float* p = dS + (int64_t)(p0 + r) * a.N + cc * 8;
+    for (int i = 0; i < SP; ++i) {
+      uint8_t* at = smem + SM::S + tile_off<RB>(sr + i * SR, sc);
+      float o[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (cc * 8 + e < a.N) f[e] = p[e];
-      }
-      const uint32_t off = tile_off<RB>(r, cc);
-      uint4 old[3];
+      for (int e = 0; e < 8; ++e) o[e] = 0.f;
 #pragma unroll
-      for (int z = 0; z < 3; ++z) old[z] = *reinterpret_cast<const uint4*>(smem + SM::S + z * SM::PLANE + off);
-      uint32_t nw[4][3];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        float lo = 0.f, hi = 0.f;
-#pragma unroll
-        for (int z = 2; z >= 0; --z) {
-          const uint32_t o = q == 0 ? old[z].x : q == 1 ? old[z].y : q == 2 ? old[z].z : old[z].w;
-          lo += lo2(o);
-          hi += hi2(o);
-        }
-        dot += lo * f[2 * q] + hi * f[2 * q + 1];
-        split2<3>(f[2 * q], f[2 * q + 1], nw[q]);
+      for (int z = 2; z >= 0; --z) {
+        const uint4 v = *reinterpret_cast<const uint4*>(at + z * SM::PLANE);
+        o[0] += lo2(v.x); o[1] += hi2(v.x); o[2] += lo2(v.y); o[3] += hi2(v.y);
+        o[4] += lo2(v.z); o[5] += hi2(v.z); o[6] += lo2(v.w); o[7] += hi2(v.w);
       }
 #pragma unroll
-      for (int z = 0; z < 3; ++z)
-        *reinterpret_cast<uint4*>(smem + SM::S + z * SM::PLANE + off) = make_uint4(nw[0][z], nw[1][z], nw[2][z], nw[3][z]);
+      for (int e = 0; e < 8; ++e) dot += o[e] * fs[i][e];
+      put8(at, SM::PLANE, fs[i]);
     }
     __syncthreads();
+    if (p0 + 64 < a.P) fetch_state(S0, p0 + 64);
 #pragma unroll 1
     for (int kk = 0; kk < 4; ++kk) {
       uint32_t fe[3][4], w[3][4];
 #pragma unroll
       for (int z = 0; z < 3; ++z) ldsm4(fe[z], at_a<SQ_RB>(s + SM::E + z * SQ_BYTES, 16 * mt, 2 * kk, lane));
 #pragma unroll
-      for (int nn = 0; nn < NTH / 2; ++nn) {
+      for (int nn = 0; nn < NTQ / 2; ++nn) {
 #pragma unroll
-        for (int z = 0; z < 3; ++z)
-          ldsm4t(w[z], at_a<RB>(s + SM::S + z * SM::PLANE, 16 * kk, half * NTH + 2 * nn, lane));
+        for (int z = 0; z < 3; ++z) ldsm4t(w[z], at_a<RB>(s + SM::S + z * SM::PLANE, 16 * kk, qt * NTQ + 2 * nn, lane));
         mma_planes<3, 3, 3>(dk1[2 * nn], dk1[2 * nn + 1], fe, w);
       }
     }
   }
   __syncthreads();   // the regions of E, dE and the state are free; the gates were written long ago
 
-  // row dots over this warp's half of N, and the state parts of dQ, dK (in dq0, dk0)
+  // row dots over this warp's quarter of N, and the state parts of dQ, dK (in dq0, dk0)
   {
     float ra[2] = {0.f, 0.f}, rb[2] = {0.f, 0.f};
     const int i0 = 16 * mt + pr;
 #pragma unroll
-    for (int j = 0; j < NTH; ++j)
+    for (int j = 0; j < NTQ; ++j)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int i = i0 + 8 * r;
         const float eg = gt.eg[i], wb = gt.wb[i];
-        const uint32_t off = tile_off<RB>(i, half * NTH + j) + 2 * q2;
+        const uint32_t off = tile_off<RB>(i, qt * NTQ + j) + 2 * q2;
         float kl = 0.f, kh = 0.f, ql = 0.f, qh = 0.f;
 #pragma unroll
         for (int z = XS - 1; z >= 0; --z) {
@@ -427,42 +451,38 @@ __global__ void __launch_bounds__(256, 1) delta_bwd_grad_kernel(const BwdArgs a)
       }
       if (lane % 4 == 0) {
         const int i = i0 + 8 * r;
-        va[half * Q + i] = ra[r];
-        vb[half * Q + i] = gt.wb[i] * rb[r];
-        vw[half * Q + i] = gt.w[i] * rb[r];
+        va[qt * Q + i] = ra[r];
+        vb[qt * Q + i] = gt.wb[i] * rb[r];
+        vw[qt * Q + i] = gt.w[i] * rb[r];
       }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
     if (lane == 0) red[warp] = dot;
   }
-  // q.k and k.k of this warp's 16 x 32 block, then M1, M2 (planes) and Y
+  // q.k and k.k of this warp's 16 x 16 block, then M1, M2 (planes) and Y
   {
-    float gk[4][4], gq[4][4];
+    float gk[2][4], gq[2][4];
     zero(gk);
     zero(gq);
+    if (qt <= mt) {
 #pragma unroll 1
-    for (int kk = 0; kk < KN / 16; ++kk) {
-      uint32_t fk[XS][4], fq[XS][4], w[XS][4];
+      for (int kk = 0; kk < KN / 16; ++kk) {
+        uint32_t fk[XS][4], fq[XS][4], w[XS][4];
 #pragma unroll
-      for (int z = 0; z < XS; ++z) {
-        ldsm4(fk[z], at_a<RB>(s + SM::K + z * SM::PLANE, 16 * mt, 2 * kk, lane));
-        ldsm4(fq[z], at_a<RB>(s + SM::QQ + z * SM::PLANE, 16 * mt, 2 * kk, lane));
-      }
-#pragma unroll
-      for (int np = 0; np < 2; ++np) {
-        if (2 * half + np > mt) break;
-#pragma unroll
-        for (int z = 0; z < XS; ++z)
-          ldsm4(w[z], at_b<RB>(s + SM::K + z * SM::PLANE, 32 * half + 16 * np, 2 * kk, lane));
-        mma_planes<XS, XS, XS>(gk[2 * np], gk[2 * np + 1], fk, w);
-        mma_planes<XS, XS, XS>(gq[2 * np], gq[2 * np + 1], fq, w);
+        for (int z = 0; z < XS; ++z) {
+          ldsm4(fk[z], at_a<RB>(s + SM::K + z * SM::PLANE, 16 * mt, 2 * kk, lane));
+          ldsm4(fq[z], at_a<RB>(s + SM::QQ + z * SM::PLANE, 16 * mt, 2 * kk, lane));
+          ldsm4(w[z], at_b<RB>(s + SM::K + z * SM::PLANE, 16 * qt, 2 * kk, lane));
+        }
+        mma_planes<XS, XS, XS>(gk[0], gk[1], fk, w);
+        mma_planes<XS, XS, XS>(gq[0], gq[1], fq, w);
       }
     }
     float* Y = reinterpret_cast<float*>(smem + SM::Y);
 #pragma unroll
-    for (int nt = 0; nt < 4; ++nt) {
-      const int j = 32 * half + 8 * nt + q2;
+    for (int nt = 0; nt < 2; ++nt) {
+      const int j = 16 * qt + 8 * nt + q2;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         const int i = 16 * mt + pr + 8 * r;
@@ -481,7 +501,7 @@ __global__ void __launch_bounds__(256, 1) delta_bwd_grad_kernel(const BwdArgs a)
         uint32_t p1[SM::NMP], p2[SM::NMP];
         split2<SM::NMP>(u1[0], u1[1], p1);
         split2<SM::NMP>(u2[0], u2[1], p2);
-        const uint32_t off = tile_off<SQ_RB>(i, 4 * half + nt) + 2 * q2;
+        const uint32_t off = tile_off<SQ_RB>(i, 2 * qt + nt) + 2 * q2;
 #pragma unroll
         for (int z = 0; z < SM::NMP; ++z) {
           *reinterpret_cast<uint32_t*>(smem + SM::M1 + z * SQ_BYTES + off) = p1[z];
@@ -499,11 +519,11 @@ __global__ void __launch_bounds__(256, 1) delta_bwd_grad_kernel(const BwdArgs a)
   for (int t = 0; t < 4; ++t) {
     uint32_t f[NMP][4], w[XS][4], w2[XS][4];
 #pragma unroll
-    for (int nn = 0; nn < NTH / 2; ++nn) {
+    for (int nn = 0; nn < NTQ / 2; ++nn) {
 #pragma unroll
       for (int z = 0; z < XS; ++z) {
-        ldsm4t(w[z], at_a<RB>(s + SM::K + z * SM::PLANE, 16 * t, half * NTH + 2 * nn, lane));
-        ldsm4t(w2[z], at_a<RB>(s + SM::QQ + z * SM::PLANE, 16 * t, half * NTH + 2 * nn, lane));
+        ldsm4t(w[z], at_a<RB>(s + SM::K + z * SM::PLANE, 16 * t, qt * NTQ + 2 * nn, lane));
+        ldsm4t(w2[z], at_a<RB>(s + SM::QQ + z * SM::PLANE, 16 * t, qt * NTQ + 2 * nn, lane));
       }
       if (t <= mt) {   // rows i = 16 mt, k = j = 16 t
 #pragma unroll
@@ -525,10 +545,10 @@ __global__ void __launch_bounds__(256, 1) delta_bwd_grad_kernel(const BwdArgs a)
     }
   }
 #pragma unroll
-  for (int j = 0; j < NTH; ++j)
+  for (int j = 0; j < NTQ; ++j)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int i = 16 * mt + pr + 8 * (e >> 1), n = 8 * (half * NTH + j) + q2 + (e & 1);
+      const int i = 16 * mt + pr + 8 * (e >> 1), n = 8 * (qt * NTQ + j) + q2 + (e & 1);
       if (i >= rows || n >= a.N) continue;
       const float vq = dq0[j][e], vk = dk0[j][e] - dk1[j][e];
       if (a.dk_part) {
@@ -541,62 +561,64 @@ __global__ void __launch_bounds__(256, 1) delta_bwd_grad_kernel(const BwdArgs a)
         stf((T*)a.dB + at, vk);
       }
     }
-  // column sums of Y, row prefixes of Y diag(beta) within 16-column segments (in place)
+  // column sums of Y, row prefixes of Y diag(beta) within 8-column segments (in place)
   float* Y = reinterpret_cast<float*>(smem + SM::Y);
   {
-    const int j = tid % 64, qr = tid / 64;
+    const int j = tid % 64, o = tid / 64;
     float v = 0.f;
-#pragma unroll 4
-    for (int i = 16 * qr; i < 16 * qr + 16; ++i) v += Y[i * 65 + j];
-    seg[qr * Q + j] = v;
+#pragma unroll
+    for (int i = 8 * o; i < 8 * o + 8; ++i) v += Y[i * 65 + j];
+    seg[o * Q + j] = v;
   }
   __syncthreads();
   {
-    const int i = tid % 64, sg = tid / 64;
+    const int i = tid % 64, o = tid / 64;
     float v = 0.f;
-#pragma unroll 4
-    for (int j = 16 * sg; j < 16 * sg + 16; ++j) {
+#pragma unroll
+    for (int j = 8 * o; j < 8 * o + 8; ++j) {
       v += Y[i * 65 + j] * gt.beta[j];
       Y[i * 65 + j] = v;
     }
   }
   __syncthreads();
   {
-    const int t = tid / 4, qr = tid % 4;   // four threads a token
+    const int t = tid / 8, o = tid % 8;   // eight threads a token
     float v = 0.f;
-    for (int i = max(16 * qr, t); i < 16 * qr + 16; ++i) {
-      v += va[i] + va[Q + i];
+    for (int i = max(8 * o, t); i < 8 * o + 8; ++i) {
+      v += (va[i] + va[Q + i]) + (va[2 * Q + i] + va[3 * Q + i]);
       if (t > 0) {
         v += Y[i * 65 + t - 1];
-        for (int sg = 0; sg < (t - 1) / 16; ++sg) v += Y[i * 65 + 16 * sg + 15];
+        for (int sg = 0; sg < (t - 1) / 8; ++sg) v += Y[i * 65 + 8 * sg + 7];
       }
     }
-    for (int j = 16 * qr; j < min(16 * qr + 16, t); ++j) v += vb[j] + vb[Q + j];
-    v += __shfl_xor_sync(0xffffffffu, v, 1);
-    v += __shfl_xor_sync(0xffffffffu, v, 2);
+    for (int j = 8 * o; j < min(8 * o + 8, t); ++j) v += (vb[j] + vb[Q + j]) + (vb[2 * Q + j] + vb[3 * Q + j]);
+#pragma unroll
+    for (int x = 1; x < 8; x <<= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
     float da = 0.f;
-    if (qr == 0) {
+    if (o == 0) {
       float d = 0.f;
-      for (int k = 0; k < 8; ++k) d += red[k];
+      for (int k = 0; k < GT / 32; ++k) d += red[k];
       const float dl = t < rows ? v + gt.eg[Q - 1] * d : 0.f;
       const float ea = expf(a.A_log[h]);
       if (t < rows) {
         const int64_t at = (b * a.L + t0 + t) * a.H + h;
+        float db = (vw[t] + vw[Q + t]) + (vw[2 * Q + t] + vw[3 * Q + t]);
+        for (int k = 0; k < 8; ++k) db += seg[k * Q + t];
         a.ddt[at] = -ea * dl;
-        a.dbeta[at] = seg[t] + seg[Q + t] + seg[2 * Q + t] + seg[3 * Q + t] + vw[t] + vw[Q + t];
+        a.dbeta[at] = db;
         // dA_log: dl times the log-decay, which is bounded as the forward bounds it
         da = dl * fmaxf(-ea * a.dt[at], -139.f);
       }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) da += __shfl_xor_sync(0xffffffffu, da, o);
+    for (int x = 16; x > 0; x >>= 1) da += __shfl_xor_sync(0xffffffffu, da, x);
     __syncthreads();
     if (lane == 0) red[warp] = da;
   }
   __syncthreads();
   if (tid == 0) {
     float d = 0.f;
-    for (int k = 0; k < 8; ++k) d += red[k];
+    for (int k = 0; k < GT / 32; ++k) d += red[k];
     a.da_part[bh * a.nc + c] = d;
   }
 }
@@ -664,7 +686,7 @@ int launch_all(const BwdArgs& a, cudaStream_t st) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
       return check_launch("gated_delta_rule_bwd: set smem attribute");
     TSSM_REQUIRE(a.Bt * a.H * a.nc < (int64_t(1) << 31), "gated_delta_rule_bwd: size out of range");
-    kern<<<(unsigned)(a.Bt * a.H * a.nc), 256, bytes, st>>>(a);
+    kern<<<(unsigned)(a.Bt * a.H * a.nc), GT, bytes, st>>>(a);
     if (a.dk_part) {
       const int64_t n = a.Bt * a.L * a.G * a.N;
       TSSM_REQUIRE(cdiv(n, 256) < (int64_t(1) << 31), "gated_delta_rule_bwd: size out of range");
