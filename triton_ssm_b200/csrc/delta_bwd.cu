@@ -35,7 +35,7 @@ struct BwdArgs {
   int H, G, P, N, npb;
   int64_t nc;
   float scale;
-  int vec_kq, vec_v, vec_n4, vec_p4;
+  int vec_kq, vec_v, vec_p4;
 };
 
 // ------------------------------------------------------------------ the chain
@@ -110,7 +110,15 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(cons
     const Gates& gt = *reinterpret_cast<const Gates*>(buf + SM::G);
     const int64_t t0 = c * Q;
     const int rows = (int)min((int64_t)Q, a.L - t0);
-    state_io(a.dstates + ((bh * a.nc + c) * a.P + pb + p0 + pr) * a.N, nullptr);
+    {
+      float* dst = a.dstates + (bh * a.nc + c) * saved_floats(a.P, a.N);
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+          if (8 * j + q2 < (a.N + 3) / 4 * 4 && pb + p0 + pr + 8 * r < a.P)
+            *saved_pair(dst, a.P, pb + p0 + pr + 8 * r, 8 * j + q2) = make_float2(S[j][2 * r], S[j][2 * r + 1]);
+    }
     // dO^T fragments of 16 tokens from 16 t
     auto load_do = [&](int t, uint32_t (&f)[XS][4]) {
 #pragma unroll
@@ -312,17 +320,23 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
   float* seg = vec + 12 * Q;                               // [8][Q] column sums of Y by row eighth
   float* red = seg + 8 * Q;                                // [16] <S0, dS1> by warp
 
-  const float* S0 = a.states + ((bh * a.nc + c) * a.P) * (int64_t)a.N;
-  const float* dS = a.dstates + ((bh * a.nc + c) * a.P) * (int64_t)a.N;
+  const float* S0 = a.states + (bh * a.nc + c) * saved_floats(a.P, a.N);
+  const float* dS = a.dstates + (bh * a.nc + c) * saved_floats(a.P, a.N);
   const int64_t tok = (b * a.L + t0) * su + (int64_t)h * a.P;
   // A thread's pieces: row er, piece ec of the 64 x 64 tiles; rows sr, piece sc of the state's.
-  const int er = tid / 8, ec = tid % 8, sr = tid / (KN / 8), sc = tid % (KN / 8);
-  constexpr int SR = GT / (KN / 8);   // state rows between a thread's pieces
+  const int er = tid / 8, ec = tid % 8, sr = tid % 64, sc = tid / 64;   // state: lanes on neighbouring rows
   float fs[SP][8];                    // the next state pieces, in flight during the products
   auto fetch_state = [&](const float* src, int p0) {
 #pragma unroll
     for (int i = 0; i < SP; ++i)
-      fetch8(src + (int64_t)p0 * a.N, a.N, min(64, a.P - p0), a.N, a.vec_n4, sr + i * SR, sc, fs[i]);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int n4 = 2 * (sc + 8 * i) + q;
+        const float4 v = p0 + sr < a.P && 4 * n4 < a.N
+                             ? *reinterpret_cast<const float4*>(src + ((int64_t)n4 * a.P + p0 + sr) * 4)
+                             : make_float4(0.f, 0.f, 0.f, 0.f);
+        fs[i][4 * q] = v.x; fs[i][4 * q + 1] = v.y; fs[i][4 * q + 2] = v.z; fs[i][4 * q + 3] = v.w;
+      }
   };
   fetch_state(S0, 0);
   load_planes<XS, KN, GT>(s + SM::K, SM::PLANE, (const T*)a.B + (b * a.L + t0) * sk + (int64_t)g * a.N, sk, rows, a.N,
@@ -352,7 +366,7 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
       fetch8(a.derrs + tok + p0, su, rows, pv, a.vec_p4, er, ec, fd);
       load_planes<XS, 64, GT>(s + SM::DO, SQ_BYTES, (const T*)a.dy + tok + p0, su, rows, pv, a.vec_v, tid);
 #pragma unroll
-      for (int i = 0; i < SP; ++i) put8(smem + SM::S + tile_off<RB>(sr + i * SR, sc), SM::PLANE, fs[i]);
+      for (int i = 0; i < SP; ++i) put8(smem + SM::S + tile_off<RB>(sr, sc + 8 * i), SM::PLANE, fs[i]);
       put8(smem + SM::E + tile_off<SQ_RB>(er, ec), SQ_BYTES, fe);
       put8(smem + SM::DE + tile_off<SQ_RB>(er, ec), SQ_BYTES, fd);
     }
@@ -384,7 +398,7 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
     // dS1 takes S0's place; <S0, dS1> on the way (the planes of S0 add up to its f32 values)
 #pragma unroll
     for (int i = 0; i < SP; ++i) {
-      uint8_t* at = smem + SM::S + tile_off<RB>(sr + i * SR, sc);
+      uint8_t* at = smem + SM::S + tile_off<RB>(sr, sc + 8 * i);
       float o[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = 0.f;
@@ -544,24 +558,7 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
       }
     }
   }
-#pragma unroll
-  for (int j = 0; j < NTQ; ++j)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int i = 16 * mt + pr + 8 * (e >> 1), n = 8 * (qt * NTQ + j) + q2 + (e & 1);
-      if (i >= rows || n >= a.N) continue;
-      const float vq = dq0[j][e], vk = dk0[j][e] - dk1[j][e];
-      if (a.dk_part) {
-        const int64_t at = ((b * a.L + t0 + i) * a.H + h) * (int64_t)a.N + n;
-        a.dq_part[at] = vq;
-        a.dk_part[at] = vk;
-      } else {   // one value head a key head
-        const int64_t at = (b * a.L + t0 + i) * sk + (int64_t)g * a.N + n;
-        stf((T*)a.dC + at, vq);
-        stf((T*)a.dB + at, vk);
-      }
-    }
-  // column sums of Y, row prefixes of Y diag(beta) within 8-column segments (in place)
+  // column sums of Y, then its row prefixes with beta (in place, a row per warp and step)
   float* Y = reinterpret_cast<float*>(smem + SM::Y);
   {
     const int j = tid % 64, o = tid / 64;
@@ -572,26 +569,69 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
   }
   __syncthreads();
   {
-    const int i = tid % 64, o = tid / 64;
-    float v = 0.f;
+    const float b0 = gt.beta[2 * lane], b1 = gt.beta[2 * lane + 1];
+    float y0[4], y1[4], v[4];
 #pragma unroll
-    for (int j = 8 * o; j < 8 * o + 8; ++j) {
-      v += Y[i * 65 + j] * gt.beta[j];
-      Y[i * 65 + j] = v;
+    for (int k = 0; k < 4; ++k) {
+      const float* row = Y + (warp + 16 * k) * 65 + 2 * lane;
+      y0[k] = row[0] * b0;
+      y1[k] = row[1] * b1;
+      v[k] = y0[k] + y1[k];
+    }
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float u = __shfl_up_sync(0xffffffffu, v[k], x);
+        if (lane >= x) v[k] += u;
+      }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float before = __shfl_up_sync(0xffffffffu, v[k], 1);
+      float* row = Y + (warp + 16 * k) * 65 + 2 * lane;
+      row[0] = (lane ? before : 0.f) + y0[k];
+      row[1] = v[k];
     }
   }
+  // dQ, dK: two adjacent columns a store
+#pragma unroll
+  for (int j = 0; j < NTQ; ++j)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int i = 16 * mt + pr + 8 * r, n = 8 * (qt * NTQ + j) + q2;
+      if (i >= rows || n >= a.N) continue;
+      const float vq[2] = {dq0[j][2 * r], dq0[j][2 * r + 1]};
+      const float vk[2] = {dk0[j][2 * r] - dk1[j][2 * r], dk0[j][2 * r + 1] - dk1[j][2 * r + 1]};
+      const bool two = n + 1 < a.N;
+      if (a.dk_part) {
+        const int64_t at = ((b * a.L + t0 + i) * a.H + h) * (int64_t)a.N + n;
+        if (a.N % 2 == 0) {
+          *reinterpret_cast<float2*>(a.dq_part + at) = make_float2(vq[0], vq[1]);
+          *reinterpret_cast<float2*>(a.dk_part + at) = make_float2(vk[0], vk[1]);
+        } else {
+          for (int e = 0; e <= (int)two; ++e) {
+            a.dq_part[at + e] = vq[e];
+            a.dk_part[at + e] = vk[e];
+          }
+        }
+      } else {   // one value head a key head
+        const int64_t at = (b * a.L + t0 + i) * sk + (int64_t)g * a.N + n;
+        for (int e = 0; e <= (int)two; ++e) {
+          stf((T*)a.dC + at + e, vq[e]);
+          stf((T*)a.dB + at + e, vk[e]);
+        }
+      }
+    }
   __syncthreads();
   {
     const int t = tid / 8, o = tid % 8;   // eight threads a token
     float v = 0.f;
-    for (int i = max(8 * o, t); i < 8 * o + 8; ++i) {
-      v += (va[i] + va[Q + i]) + (va[2 * Q + i] + va[3 * Q + i]);
-      if (t > 0) {
-        v += Y[i * 65 + t - 1];
-        for (int sg = 0; sg < (t - 1) / 8; ++sg) v += Y[i * 65 + 8 * sg + 7];
-      }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = 8 * o + k;
+      if (i >= t) v += (va[i] + va[Q + i]) + (va[2 * Q + i] + va[3 * Q + i]) + (t > 0 ? Y[i * 65 + t - 1] : 0.f);
+      else v += (vb[i] + vb[Q + i]) + (vb[2 * Q + i] + vb[3 * Q + i]);
     }
-    for (int j = 8 * o; j < min(8 * o + 8, t); ++j) v += (vb[j] + vb[Q + j]) + (vb[2 * Q + j] + vb[3 * Q + j]);
 #pragma unroll
     for (int x = 1; x < 8; x <<= 1) v += __shfl_xor_sync(0xffffffffu, v, x);
     float da = 0.f;
@@ -706,7 +746,7 @@ BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N
   auto up = [](int64_t n) { return (n + 3) / 4 * 4; };
   const int64_t nc = cdiv(L, delta::Q);
   BwdSpace s;
-  s.dstates = up(Bt * H * nc * P * N);
+  s.dstates = Bt * H * nc * saved_floats(P, N);
   s.derrs = up(Bt * L * H * P);
   s.part = H == G ? 0 : up(Bt * L * H * N);
   s.da = up(Bt * H * nc);
@@ -752,6 +792,7 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
     if (cudaMemsetAsync(dA_log, 0, H * 4, st) != cudaSuccess) return check_launch("gated_delta_rule_bwd: clear");
     return TSSM_OK;
   }
+  TSSM_REQUIRE(Bt * L == 0 || aligned16(states), "gated_delta_rule_bwd: states must be 16-byte aligned");
   const BwdSpace sp = space(Bt, L, H, G, P, N);
   BwdArgs a{};
   a.u = u; a.B = B; a.C = C; a.dy = dy;
@@ -770,7 +811,6 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
   const int per = dtype == TSSM_F32 ? 4 : 8;
   a.vec_kq = N % per == 0 && aligned16(B) && aligned16(C);
   a.vec_v = P % per == 0 && aligned16(dy);
-  a.vec_n4 = N % 4 == 0 && aligned16(states);
   a.vec_p4 = P % 4 == 0 && aligned16(errors);
   if (dtype == TSSM_F32) return N <= 64 ? launch_all<3, 64>(a, st) : launch_all<3, 128>(a, st);
   return N <= 64 ? launch_all<1, 64>(a, st) : launch_all<1, 128>(a, st);

@@ -113,7 +113,15 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
     const Gates& gt = *reinterpret_cast<const Gates*>(buf + SM::G);
     const int64_t t0 = c * Q;
     const int rows = (int)min((int64_t)Q, a.L - t0);
-    if (a.states) state_io(a.states + ((bh * a.nc + c) * a.P + pb + p0 + pr) * a.N, nullptr);
+    if (a.states) {
+      float* dst = a.states + (bh * a.nc + c) * saved_floats(a.P, a.N);
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int r = 0; r < 2; ++r)   // columns beyond N are 0
+          if (8 * j + q2 < (a.N + 3) / 4 * 4 && pb + p0 + pr + 8 * r < a.P)
+            *saved_pair(dst, a.P, pb + p0 + pr + 8 * r, 8 * j + q2) = make_float2(S[j][2 * r], S[j][2 * r + 1]);
+    }
     // KS^T, then X^T
     float x[8][4];
 #pragma unroll

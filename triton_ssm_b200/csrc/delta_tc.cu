@@ -285,10 +285,11 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
         store_planes<NS>(at, r);
         hand_over(B_S + i);
       }
-      if (a.states && live && ok) {
-        float* dst = a.states + ((bh * a.nc + a.c0 + c) * a.P + pb + p) * (int64_t)a.N + half * HN;
+      if (a.states && live && ok) {   // [N / 4][P][4]: 512 bytes a warp and store
+        float4* dst = reinterpret_cast<float4*>(a.states) +
+                      ((bh * a.nc + a.c0 + c) * (a.N / 4) + half * (HN / 4)) * (int64_t)a.P + pb + p;
 #pragma unroll
-        for (int j = 0; j < HN; j += 4) *reinterpret_cast<float4*>(dst + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+        for (int j = 0; j < HN; j += 4) dst[(int64_t)(j / 4) * a.P] = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
       }
       // X^T = V^T - exp(l) KS^T, 32 tokens of this half
       const uint8_t* st = stage(c);
