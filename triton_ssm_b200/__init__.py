@@ -10,8 +10,8 @@ from .delta import *  # noqa: F401,F403
 from .delta import __all__ as _delta_all
 from .norm import *  # noqa: F401,F403
 from .norm import __all__ as _norm_all
-from .streaming import StreamingRing  # noqa: F401
+from .streaming import DeltaStream, StreamingRing  # noqa: F401
 
-__all__ = ["load_library", "LIB_PATH", "TSSMError", "StreamingRing"] + list(_ops_all) + \
+__all__ = ["load_library", "LIB_PATH", "TSSMError", "StreamingRing", "DeltaStream"] + list(_ops_all) + \
     list(_delta_all) + list(_norm_all)
 __version__ = "0.1.0"

@@ -9,9 +9,11 @@ a service can persist its streams and resume them bit for bit.
 """
 import torch
 
+from .delta import gated_delta_rule, gated_delta_step
+from .norm import group_norm_act
 from .ops import streaming_interp_then_ssm
 
-__all__ = ["StreamingRing"]
+__all__ = ["StreamingRing", "DeltaStream"]
 
 _STATE = ("ring_V", "ring_M", "ring_tau", "ring_head", "h")
 _PARAMS = ("Abar", "Bbar", "D")
@@ -89,3 +91,88 @@ class StreamingRing:
         ring = cls(Bt, H, KR - 1, ck["Abar"], ck["Bbar"], ck["D"], device=device, block_h=ck["block_h"])
         ring.restore(ck)
         return ring
+
+
+class DeltaStream:
+    """S independent streams of a gated-delta-rule layer: the state h [S,H,P,N]
+    f32 stays on the device, ``prefill`` advances every stream by a prompt,
+    ``step`` by one token.  Outputs are normalised per token and head (group
+    norm with H groups), then ``act``.
+
+    A_log [H]; weight, bias [H*P] (default 1 and 0), f32; scale defaults to
+    N ** -0.5.
+    """
+
+    _TENSORS = ("A_log", "weight", "bias", "h")
+
+    def __init__(self, S, H, P, N, A_log, weight=None, bias=None, scale=None, eps=1e-5, act="silu", device=None,
+                 h0=None):
+        device = torch.device(device) if device is not None else A_log.device
+        if device.type != "cuda":
+            raise ValueError("DeltaStream lives on a CUDA device (no CPU fallback)")
+        if tuple(A_log.shape) != (H,):
+            raise ValueError("DeltaStream: A_log must be [H]")
+        if act not in ("silu", "none"):
+            raise ValueError("DeltaStream: act must be 'silu' or 'none' (got %r)" % (act,))
+        f32 = dict(device=device, dtype=torch.float32)
+        self.A_log = A_log.to(**f32).contiguous()
+        self.weight = torch.ones(H * P, **f32) if weight is None else weight.to(**f32).contiguous()
+        self.bias = torch.zeros(H * P, **f32) if bias is None else bias.to(**f32).contiguous()
+        self.scale = float(N) ** -0.5 if scale is None else float(scale)
+        self.eps, self.act, self.tokens = float(eps), act, 0
+        self.h = torch.zeros(S, H, P, N, **f32)
+        if h0 is not None:
+            if tuple(h0.shape) != (S, H, P, N):
+                raise ValueError("DeltaStream: h0 must be [S,H,P,N]")
+            self.h.copy_(h0)
+
+    def _norm(self, y):
+        H = self.h.shape[1]
+        return group_norm_act(y.reshape(-1, y.shape[-1]), self.weight, self.bias, H, eps=self.eps,
+                              act=self.act).view(y.shape)
+
+    def prefill(self, u, B, C, dt, beta):
+        """L tokens of every stream: u [S,L,H*P], B, C [S,L,G,N], dt, beta [S,L,H]; streams that
+        are shorter are padded at their end with zeros (dt = beta = 0).  Returns [S,L,H*P]."""
+        if u.dim() != 3 or u.shape[0] != self.h.shape[0]:
+            raise ValueError("DeltaStream.prefill: u must be [S,L,H*P] with S = %d streams" % self.h.shape[0])
+        y, self.h = gated_delta_rule(u, self.A_log, B, C, dt, beta, scale=self.scale, h0=self.h, return_state=True)
+        self.tokens += u.shape[1]
+        return self._norm(y)
+
+    def step(self, x, B, C, dt, beta):
+        """One token of every stream: x [S,H*P], B, C [S,G,N], dt, beta [S,H].  Returns [S,H*P]."""
+        S, H, P, _ = self.h.shape
+        if tuple(x.shape) != (S, H * P):
+            raise ValueError("DeltaStream.step: x must be [S,H*P] = [%d,%d]" % (S, H * P))
+        y = gated_delta_step(x.reshape(S, H, P), dt, self.h, self.A_log, B, C, beta, scale=self.scale)
+        self.tokens += 1
+        return self._norm(y.view(S, H * P))
+
+    def checkpoint(self):
+        """A host copy of the streams' state and parameters, complete when this returns."""
+        ck = {"scale": self.scale, "eps": self.eps, "act": self.act, "tokens": self.tokens}
+        ck.update((k, getattr(self, k).cpu()) for k in self._TENSORS)
+        return ck
+
+    def restore(self, ck):
+        """Put a checkpoint of streams of the same shape back in place."""
+        for k in self._TENSORS:
+            if tuple(ck[k].shape) != tuple(getattr(self, k).shape):
+                raise ValueError("DeltaStream.restore: %s has shape %s, expected %s"
+                                 % (k, tuple(ck[k].shape), tuple(getattr(self, k).shape)))
+        for k in self._TENSORS:
+            getattr(self, k).copy_(ck[k])
+        self.scale, self.eps, self.act, self.tokens = (float(ck["scale"]), float(ck["eps"]), str(ck["act"]),
+                                                       int(ck["tokens"]))
+
+    def save(self, path):
+        torch.save(self.checkpoint(), path)
+
+    @classmethod
+    def load(cls, path, device="cuda"):
+        ck = torch.load(path, map_location="cpu", weights_only=True)
+        S, H, P, N = ck["h"].shape
+        st = cls(S, H, P, N, ck["A_log"], device=device)
+        st.restore(ck)
+        return st
