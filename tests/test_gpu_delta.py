@@ -366,6 +366,29 @@ def test_backward_graph_repeats_and_empty(cuda_ops):
     assert torch.equal(out[6], dhd) and not out[1].any()
 
 
+@pytest.mark.gpu
+def test_many_streams_go_through_in_segments(cuda_ops):
+    """So many streams that the sequence is cut into segments of single chunks: a row's results are
+    those of the row alone."""
+    Bt, L = 3300, 150
+    a, h0 = make(2, L, 2, 1, 64, 64, torch.bfloat16, seed=27)
+    d = {k: v.to(dev) for k, v in a.items()}
+    g = torch.Generator().manual_seed(7)
+    dy, dh = torch.randn(2, L, 128, generator=g).bfloat16().to(dev), torch.randn(2, 2, 64, 64, generator=g).to(dev)
+    many = {k: (v if k == "A_log" else v.repeat(Bt // 2, *[1] * (v.dim() - 1))) for k, v in d.items()}
+
+    def run(x, h, dy, dh):
+        args = (x["u"].flatten(2), x["A_log"], x["B"], x["C"], x["dt"], x["beta"])
+        y, hl, saved = cuda_ops.gated_delta_rule(*args, h0=h, return_state=True, save=True)
+        grads = cuda_ops.gated_delta_rule_bwd(*args, dy, saved, dh_last=dh)
+        return [y, hl] + [g for n, g in zip(NAMES, grads) if n != "dA_log"]
+
+    few = run(d, h0.to(dev), dy, dh)
+    out = run(many, h0.to(dev).repeat(Bt // 2, 1, 1, 1), dy.repeat(Bt // 2, 1, 1), dh.repeat(Bt // 2, 1, 1, 1))
+    for x, y in zip(few, out):
+        assert torch.equal(y[:2], x) and torch.equal(y[-2:], x)
+
+
 def test_backward_refusals_without_gpu():
     from triton_ssm_b200 import _lib
     lib = _lib.load_library()

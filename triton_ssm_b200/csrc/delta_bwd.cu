@@ -20,6 +20,7 @@
 // (chunk, head) pairs at once.  Shared key heads and dA_log are summed last, in a
 // fixed order.
 #include "delta.cuh"
+#include "delta_tc.h"
 
 namespace tssm {
 namespace delta {
@@ -31,6 +32,7 @@ struct BwdArgs {
   void *du, *dB, *dC;
   float *dA_log, *ddt, *dbeta, *dh0;
   float *dstates, *derrs, *dk_part, *dq_part, *da_part;   // workspace
+  void* img;   // the tcgen05 chain's workspace; null: the register chain
   int64_t Bt, L;
   int H, G, P, N, npb;
   int64_t nc;
@@ -717,8 +719,14 @@ int launch_chain(BwdArgs a, cudaStream_t st) {
 template <int XS, int KN>
 int launch_all(const BwdArgs& a, cudaStream_t st) {
   using T = typename std::conditional<XS == 1, __nv_bfloat16, float>::type;
-  const bool wide = a.P > 64 && a.Bt * a.H * cdiv(a.P, 128) >= num_sms();
-  if (int e = wide ? launch_chain<XS, KN, 8>(a, st) : launch_chain<XS, KN, 4>(a, st)) return e;
+  if (a.img) {
+    const TcBackCall t{a.B, a.C, a.dy, a.A_log, a.dt, a.beta, a.dh_last, a.du, a.dh0, a.dstates, a.derrs, a.img,
+                       a.Bt, a.L, a.H, a.G, a.P, a.N, a.scale};
+    if (int e = tc_back_run(t, st)) return e;
+  } else {
+    const bool wide = a.P > 64 && a.Bt * a.H * cdiv(a.P, 128) >= num_sms();
+    if (int e = wide ? launch_chain<XS, KN, 8>(a, st) : launch_chain<XS, KN, 4>(a, st)) return e;
+  }
   if (a.nc > 0) {
     constexpr int bytes = GradSmem<XS, KN>::BYTES;
     static_assert(bytes <= 232448, "shared-memory layout exceeds the per-block limit");
@@ -738,11 +746,12 @@ int launch_all(const BwdArgs& a, cudaStream_t st) {
   return check_launch("gated_delta_rule_bwd");
 }
 
-// Workspace in floats: dS1 of every chunk, dE, per-head dK and dQ (shared key heads), dA parts.
+// Workspace in floats: dS1 of every chunk, dE, per-head dK and dQ (shared key heads), dA parts,
+// the tcgen05 chain's images.
 struct BwdSpace {
-  int64_t dstates, derrs, part, da, total;
+  int64_t dstates, derrs, part, da, img, total;
 };
-BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N) {
+BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N, int dtype) {
   auto up = [](int64_t n) { return (n + 3) / 4 * 4; };
   const int64_t nc = cdiv(L, delta::Q);
   BwdSpace s;
@@ -750,7 +759,8 @@ BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N
   s.derrs = up(Bt * L * H * P);
   s.part = H == G ? 0 : up(Bt * L * H * N);
   s.da = up(Bt * H * nc);
-  s.total = s.dstates + s.derrs + 2 * s.part + s.da;
+  s.img = tc_takes(P, N, dtype) ? tc_back_workspace(Bt, L, H) / 4 : 0;
+  s.total = s.dstates + s.derrs + 2 * s.part + s.da + s.img;
   return s;
 }
 
@@ -759,9 +769,9 @@ BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N
 }  // namespace tssm
 
 extern "C" int64_t tssm_gated_delta_rule_bwd_workspace_size(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P,
-                                                            int64_t N) {
+                                                            int64_t N, int dtype) {
   if (Bt <= 0 || L <= 0 || H <= 0 || G <= 0 || P <= 0 || N <= 0) return 0;
-  return tssm::delta::space(Bt, L, H, G, P, N).total * 4;
+  return tssm::delta::space(Bt, L, H, G, P, N, dtype).total * 4;
 }
 
 extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const void* B, const void* C, const void* dt,
@@ -783,7 +793,7 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
   TSSM_REQUIRE(A_log && dA_log && (Bt == 0 || dh0), "gated_delta_rule_bwd: null pointer");
   TSSM_REQUIRE(Bt * L == 0 || (u && B && C && dt && beta && dy && states && errors && du && dB && dC && ddt && dbeta),
                "gated_delta_rule_bwd: null pointer");
-  const int64_t need = tssm_gated_delta_rule_bwd_workspace_size(Bt, L, H, G, P, N);
+  const int64_t need = tssm_gated_delta_rule_bwd_workspace_size(Bt, L, H, G, P, N, dtype);
   TSSM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
                "gated_delta_rule_bwd: workspace of %lld bytes (16-byte aligned) needed, %lld given", (long long)need,
                (long long)workspace_bytes);
@@ -793,7 +803,7 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
     return TSSM_OK;
   }
   TSSM_REQUIRE(Bt * L == 0 || aligned16(states), "gated_delta_rule_bwd: states must be 16-byte aligned");
-  const BwdSpace sp = space(Bt, L, H, G, P, N);
+  const BwdSpace sp = space(Bt, L, H, G, P, N, dtype);
   BwdArgs a{};
   a.u = u; a.B = B; a.C = C; a.dy = dy;
   a.A_log = (const float*)A_log; a.dt = (const float*)dt; a.beta = (const float*)beta;
@@ -805,6 +815,9 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
   a.dk_part = sp.part ? a.derrs + sp.derrs : nullptr;
   a.dq_part = sp.part ? a.dk_part + sp.part : nullptr;
   a.da_part = a.derrs + sp.derrs + 2 * sp.part;
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(dy) |
+                          reinterpret_cast<uintptr_t>(dh_last) | reinterpret_cast<uintptr_t>(dh0);
+  a.img = sp.img && L > 0 && (bases & 15u) == 0 ? a.da_part + sp.da : nullptr;
   a.Bt = Bt; a.L = L; a.H = (int)H; a.G = (int)G; a.P = (int)P; a.N = (int)N;
   a.nc = cdiv(L, delta::Q);
   a.scale = (float)scale;

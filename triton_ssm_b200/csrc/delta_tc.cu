@@ -46,7 +46,12 @@ namespace {
 using namespace sm100;
 
 constexpr int TILE = 8192;                       // [64 x 64] bf16
-constexpr int IMG_T = 0, IMG_AQ = 3 * SQ_BYTES, IMG_G = IMG_AQ + 2 * SQ_BYTES, IMG = IMG_G + 2 * Q * 4;
+// A chunk's image: T planes, NA planes of Aq diag(beta), exp(l) and w beta.
+constexpr int IMG_T = 0, IMG_AQ = 3 * SQ_BYTES;
+__host__ __device__ constexpr int img_gates(int na) { return IMG_AQ + na * SQ_BYTES; }
+__host__ __device__ constexpr int img_bytes(int na) { return img_gates(na) + 2 * Q * 4; }
+constexpr int IMG_G = img_gates(2), IMG = img_bytes(2);           // forward
+constexpr int IMG_G3 = img_gates(3), IMG3 = img_bytes(3);         // backward: f32 gradients want all of Aq
 constexpr int64_t IMAGE_BYTES = 256ll << 20;
 
 // ------------------------------------------------------------------ chunk images
@@ -66,7 +71,7 @@ struct PrepSmem {
   static constexpr int K = 0, QQ = PLANE, M = QQ, G = QQ + (MB > PLANE ? MB : PLANE), BYTES = G + (int)sizeof(Gates) + 128;
 };
 
-template <int KN>
+template <int KN, int NA>
 __global__ void __launch_bounds__(128, 6) delta_prep_kernel(const PrepArgs a) {
   using SM = PrepSmem<KN>;
   extern __shared__ uint8_t smem_raw[];
@@ -84,10 +89,10 @@ __global__ void __launch_bounds__(128, 6) delta_prep_kernel(const PrepArgs a) {
   if (t < 32) gates_warp(gt, a.dt + b * a.L * a.H + h, a.beta + b * a.L * a.H + h, a.H, a.A_log[h], t0, a.L, t);
   cp_async_wait_all();
   __syncthreads();
-  uint8_t* img = a.img + (bh * a.nseg + ci) * IMG;
-  float* go = reinterpret_cast<float*>(img + IMG_G);
+  uint8_t* img = a.img + (bh * a.nseg + ci) * img_bytes(NA);
+  float* go = reinterpret_cast<float*>(img + img_gates(NA));
   go[t] = t < Q ? gt.eg[t] : gt.wb[t - Q];
-  chunk_matrices<1, KN, 2, 3, true>(s + SM::K, s + SM::QQ, gt, a.scale, reinterpret_cast<float*>(smem + SM::M), img + IMG_AQ,
+  chunk_matrices<1, KN, NA, 3, true>(s + SM::K, s + SM::QQ, gt, a.scale, reinterpret_cast<float*>(smem + SM::M), img + IMG_AQ,
                               img + IMG_T, t, 1);
 }
 
@@ -548,6 +553,354 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
   }
 }
 
+
+// ------------------------------------------------------------------ the backward's chain
+// The same walk in reverse (formulas: delta_bwd.cu), transposed as above; dS^T is the state:
+//   R^T   = (dS^T K^T) diag(w beta) + dO^T (Aq diag(beta))
+//   dE^T  = R^T T
+//   dS^T <- exp(l_last) dS^T + (scale exp(l) dO)^T Q - (exp(l) dE)^T K
+// TMEM columns: [0, 192) dS planes, later the update's sum over planes 0, 1 and two planes of
+// scale exp(l) dO over plane 2 (the third: [480, 512)).  [192, 256) dS K.  [256, 352) dO^T in its
+// first 32, then R planes, then -exp(l) dE planes.  [352, 416) dE.  [416, 480) dO^T Aq.
+struct BackArgs {
+  const uint8_t* img;
+  const float* ds_in;
+  float *ds_out, *dstates, *derrs;
+  __nv_bfloat16* du;
+  int* status;
+  int64_t L, c0, nseg, nc;
+  int H, G, P, N, npb;
+  float scale;
+};
+
+template <int KN>
+struct BackSmem {
+  static constexpr int NB = KN / 64;
+  static constexpr int K = 0, QQ = K + NB * TILE, DO = QQ + NB * TILE, IM = DO + 2 * TILE,
+                       STAGE = (IM + IMG3 + 1023) / 1024 * 1024;
+  static constexpr int BAR = 2 * STAGE, BYTES = BAR + 256 + 1024;
+  static_assert(BYTES <= 232448, "shared-memory layout exceeds the per-block limit");
+};
+
+constexpr uint32_t C_AO = 416, C_D2 = 480;
+constexpr uint32_t B_A = 1, B_D = 11;   // named barriers: dO^T, planes of scale exp(l) dO (B_S, B_X, B_W as above)
+
+template <int KN>
+__global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_constant__ CUtensorMap tm_k,
+                                                                 const __grid_constant__ CUtensorMap tm_q,
+                                                                 const __grid_constant__ CUtensorMap tm_o,
+                                                                 const BackArgs a) {
+  using SM = BackSmem<KN>;
+  constexpr int NB = SM::NB, HN = KN / 2, NS = 3;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t bh = blockIdx.x / a.npb;
+  const int pb = (int)(blockIdx.x - bh * a.npb) * 128;
+  const int b = (int)(bh / a.H), h = (int)(bh - (int64_t)b * a.H), g = h / (a.H / a.G);
+  const int boxes = min(2, (a.P - pb) / 64);
+  const int n = (int)a.nseg;
+
+  uint64_t* bar = reinterpret_cast<uint64_t*>(smem + SM::BAR);
+  uint64_t *full = bar, *empty = bar + 2, *ksdone = bar + 4, *edone = bar + 5, *dsdone = bar + 6, *drain = bar + 7;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + SM::BAR + 192);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + SM::BAR + 196);
+  int* issued = reinterpret_cast<int*>(smem + SM::BAR + 200);
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1 + 8);   // the issuer's commit, chain warps
+    }
+    mbar_init(ksdone, 1);
+    mbar_init(edone, 1);
+    mbar_init(dsdone, 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    *issued = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // step k works on chunk n - 1 - k of the segment
+  auto stage = [&](int k) { return smem + (k & 1) * SM::STAGE; };
+  auto fail = [&](int code) {
+    *abort_flag = 1;
+    atomicExch(a.status, code);
+  };
+  auto waitw = [&](uint64_t* m, int phase, int code) {
+    const bool ok = mbar_wait_hot(m, phase & 1, abort_flag);
+    tc_fence_after();
+    if (__all_sync(0xffffffffu, ok)) return true;
+    if (lane == 0 && !*abort_flag) fail(code);
+    return false;
+  };
+  auto hand_over = [&](uint32_t x) {
+    tmem_wait_st();
+    tc_fence_before();
+    named_bar_arrive(x, B_ISSUE);
+  };
+  auto take = [&](uint32_t x) {
+    named_bar_sync(x, B_ISSUE);
+    tc_fence_after();
+  };
+  auto plane = [](int s, int hf) { return (uint32_t)(s < 2 ? HN * hf + (HN / 2) * s : KN + (HN / 2) * hf); };
+  auto dplane = [](int s) { return s < 2 ? 128u + 32u * s : C_D2; };   // of scale exp(l) dO
+
+  if (warp >= 4) {
+    // ================================================================ the chain
+    const int half = (warp >> 2) - 1, p = (warp & 3) * 32 + lane;
+    const uint32_t tl = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const bool live = p < boxes * 64;
+    const int64_t row = (bh * a.P + pb + p) * (int64_t)a.N + half * HN;
+    float S[HN];
+#pragma unroll
+    for (int j = 0; j < HN; j += 4) {
+      const float4 v = live && a.ds_in ? *reinterpret_cast<const float4*>(a.ds_in + row + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+      S[j] = v.x; S[j + 1] = v.y; S[j + 2] = v.z; S[j + 3] = v.w;
+    }
+    bool ok = true;
+    for (int k = 0; k < n; ++k) {
+      const int64_t cc = a.c0 + n - 1 - k;
+      const uint8_t* st = stage(k);
+      ok = ok && waitw(&full[k & 1], k >> 1, 2102);
+      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_G3) + 32 * half;
+      const float* wb = eg + Q;
+      const float el = (eg - 32 * half)[Q - 1];
+      const uint16_t* os = reinterpret_cast<const uint16_t*>(st + SM::DO + (p >> 6) * TILE) + (p & 63) + half * 32 * 64;
+      // dO^T, 32 tokens of this half
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        uint32_t u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          u[j] = __byte_perm(os[(16 * i + 2 * j) * 64], os[(16 * i + 2 * j + 1) * 64], 0x5410);
+        tmem_st8u(tl + C_XP + 16 * half + 8 * i, u);
+      }
+      hand_over(B_A);
+      // dS planes
+#pragma unroll
+      for (int i = 0; i < HN / 16; ++i) {
+        float r[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = S[16 * i + j];
+        uint32_t at[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) at[s] = tl + plane(s, half) + 8 * i;
+        store_planes<NS>(at, r);
+        hand_over(B_S + i);
+      }
+      if (live && ok) {
+        float4* dst = reinterpret_cast<float4*>(a.dstates) +
+                      ((bh * a.nc + cc) * (a.N / 4) + half * (HN / 4)) * (int64_t)a.P + pb + p;
+#pragma unroll
+        for (int j = 0; j < HN; j += 4) dst[(int64_t)(j / 4) * a.P] = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+      }
+      // R^T; the last tokens' products reach all columns and go first
+      ok = ok && waitw(ksdone, k, 2103);
+#pragma unroll 1
+      for (int i = 1; i >= 0; --i) {
+        float x[16], y[16];
+        tmem_get16(tl + C_KS + 32 * half + 16 * i, x);
+        tmem_get16(tl + C_AO + 32 * half + 16 * i, y);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 w4 = *reinterpret_cast<const float4*>(wb + 16 * i + j);
+          x[j] = w4.x * x[j] + y[j];
+          x[j + 1] = w4.y * x[j + 1] + y[j + 1];
+          x[j + 2] = w4.z * x[j + 2] + y[j + 2];
+          x[j + 3] = w4.w * x[j + 3] + y[j + 3];
+        }
+        store_planes<NS>(tl + C_XP + 48 * half + 8 * i, 16, x);
+        hand_over(B_X + i);
+      }
+      // scale exp(l) dO, while dE is made
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        float x[16];
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 e4 = *reinterpret_cast<const float4*>(eg + 16 * i + j);
+          const uint16_t* o = os + (16 * i + j) * 64;
+          x[j] = a.scale * e4.x * lo2(o[0]);
+          x[j + 1] = a.scale * e4.y * lo2(o[64]);
+          x[j + 2] = a.scale * e4.z * lo2(o[128]);
+          x[j + 3] = a.scale * e4.w * lo2(o[192]);
+        }
+        const uint32_t at[NS] = {tl + dplane(0) + 16 * half + 8 * i, tl + dplane(1) + 16 * half + 8 * i,
+                                 tl + dplane(2) + 16 * half + 8 * i};
+        store_planes<NS>(at, x);
+      }
+      hand_over(B_D);
+      // -exp(l) dE
+      ok = ok && waitw(edone, k, 2104);
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        float x[16];
+        tmem_get16(tl + C_E + 32 * half + 16 * i, x);
+#pragma unroll
+        for (int j = 0; j < 16; j += 4) {
+          const float4 e4 = *reinterpret_cast<const float4*>(eg + 16 * i + j);
+          x[j] *= -e4.x;
+          x[j + 1] *= -e4.y;
+          x[j + 2] *= -e4.z;
+          x[j + 3] *= -e4.w;
+        }
+        store_planes<NS>(tl + C_XP + 48 * half + 8 * i, 16, x);
+        hand_over(B_W + i);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[k & 1]);   // dO and the gates are read
+      // dE for the gradient kernel, du
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        float x[16];
+        tmem_get16(tl + C_E + 32 * half + 16 * i, x);
+        const int64_t tk = cc * Q + 32 * half + 16 * i;
+        const int left = live && ok ? (int)max((int64_t)0, min((int64_t)16, a.L - tk)) : 0;
+        const int64_t at = ((b * a.L + tk) * a.H + h) * (int64_t)a.P + pb + p;
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (j < left) {
+            a.derrs[at + (int64_t)j * a.H * a.P] = x[j];
+            a.du[at + (int64_t)j * a.H * a.P] = __float2bfloat16_rn(x[j]);
+          }
+      }
+      // dS^T
+      ok = ok && waitw(dsdone, k, 2105);
+#pragma unroll
+      for (int i = 0; i < HN / 16; ++i) {
+        float d[16];
+        tmem_get16(tl + HN * half + 16 * i, d);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) S[16 * i + j] = el * S[16 * i + j] + d[j];
+      }
+    }
+    if (ok && live) {
+#pragma unroll
+      for (int j = 0; j < HN; j += 4)
+        *reinterpret_cast<float4*>(a.ds_out + row + j) = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+    }
+  } else if (warp == 1) {
+    // ================================================================ copies
+    if (lane == 0) {
+      const uint32_t bytes = 2 * NB * TILE + boxes * TILE + IMG3;
+      for (int k = 0; k < n; ++k) {
+        if (k >= 2 && !mbar_wait(&empty[k & 1], ((k >> 1) - 1) & 1, abort_flag)) {
+          if (!*abort_flag) fail(2109);
+          break;
+        }
+        uint8_t* st = stage(k);
+        uint64_t* f = &full[k & 1];
+        const int c = n - 1 - k, t0 = (int)(a.c0 + c) * Q;
+        mbar_arrive_expect_tx(f, bytes);
+        for (int x = 0; x < NB; ++x) {
+          tma_load_3d(st + SM::K + x * TILE, &tm_k, g * a.N + 64 * x, t0, b, f);
+          tma_load_3d(st + SM::QQ + x * TILE, &tm_q, g * a.N + 64 * x, t0, b, f);
+        }
+        for (int x = 0; x < boxes; ++x) tma_load_3d(st + SM::DO + x * TILE, &tm_o, h * a.P + pb + 64 * x, t0, b, f);
+        asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                         smem_u32(st + SM::IM)),
+                     "l"(a.img + (bh * a.nseg + c) * IMG3), "r"(IMG3), "r"(smem_u32(f))
+                     : "memory");
+        *issued = k + 1;
+      }
+    }
+  } else if (warp == 0) {
+    // ================================================================ products
+    bool ok = true;
+    for (int k = 0; k < n; ++k) {
+      const uint32_t st = smem_u32(stage(k));
+      ok = ok && waitw(&full[k & 1], k >> 1, 2110);
+      // dO^T Aq: tokens 16 t .. reach the columns up to 16 t + 15
+      take(B_A);
+      if (ok && elect_one())
+#pragma unroll 1
+        for (int t = 3; t >= 0; --t)
+#pragma unroll
+          for (int z = 2; z >= 0; --z)
+            umma_bf16_ta(tmem + C_AO, tmem + C_XP + 8 * t,
+                         make_desc_sw128(st + SM::IM + IMG_AQ + z * SQ_BYTES, TILE) + 128 * t,
+                         make_idesc_bf16(128, 16 * (t + 1), false, true), t != 3 || z != 2);
+      // dS K
+#pragma unroll 1
+      for (int i = 0; i < HN / 16; ++i) {
+        take(B_S + i);
+        if (ok && elect_one())
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int s = NS - 1; s >= 0; --s) {
+              const int kk = hf * (HN / 16) + i;
+              umma_bf16_ta(tmem + C_KS, tmem + plane(s, hf) + 8 * i,
+                           make_desc_sw128(st + SM::K + (kk / 4) * TILE, 16) + 2 * (kk & 3),
+                           make_idesc_bf16(128, 64, false, false), i || hf || s != NS - 1);
+            }
+      }
+      umma_commit_warp(ksdone);   // both products
+      // dE
+#pragma unroll 1
+      for (int i = 1; i >= 0; --i) {
+        take(B_X + i);
+        if (ok && elect_one())
+#pragma unroll
+          for (int hf = 1; hf >= 0; --hf)
+#pragma unroll
+            for (int o = NS - 1; o >= 0; --o)
+#pragma unroll
+              for (int s = 0; s <= o; ++s) {
+                const int t = 2 * hf + i;
+                umma_bf16_ta(tmem + C_E, tmem + C_XP + 48 * hf + 16 * s + 8 * i,
+                             make_desc_sw128(st + SM::IM + IMG_T + (o - s) * SQ_BYTES, TILE) + 128 * t,
+                             make_idesc_bf16(128, 16 * (t + 1), false, true), t != 3 || o != NS - 1 || s);
+              }
+      }
+      umma_commit_warp(edone);
+      // the update, over the dS planes that dS K has read: Q's part, then K's
+      take(B_D);
+      if (ok && elect_one())
+#pragma unroll 1
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int s = NS - 1; s >= 0; --s)
+            umma_bf16_ta(tmem, tmem + dplane(s) + 8 * t, make_desc_sw128(st + SM::QQ, TILE) + 128 * t,
+                         make_idesc_bf16(128, KN, false, true), t || s != NS - 1);
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        take(B_W + i);
+        if (ok && elect_one())
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf)
+#pragma unroll
+            for (int s = NS - 1; s >= 0; --s)
+              umma_bf16_ta(tmem, tmem + C_XP + 48 * hf + 16 * s + 8 * i,
+                           make_desc_sw128(st + SM::K, TILE) + 128 * (2 * hf + i),
+                           make_idesc_bf16(128, KN, false, true), true);
+      }
+      umma_commit_warp(dsdone);
+      umma_commit_warp(&empty[k & 1]);
+    }
+    umma_commit_warp(drain);
+    mbar_wait(drain, 0, nullptr, 100000000ull);
+  }
+  // ================================================================ teardown
+  tc_fence_before();
+  __syncthreads();
+  if (tid == 0 && *abort_flag)   // copies that were started land before the block leaves
+    for (int k = max(0, *issued - 2); k < *issued; ++k) mbar_wait(&full[k & 1], (k >> 1) & 1, nullptr, 100000000ull);
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 bool map_bf16(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64_t d2, bool swizzle) {
   auto fn = tmap_encode_fn();
   if (!fn) return false;
@@ -560,13 +913,13 @@ bool map_bf16(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int64_t segment_chunks(int64_t streams, int64_t nc) {
-  return std::max<int64_t>(1, std::min(nc, IMAGE_BYTES / (streams * IMG)));
+int64_t segment_chunks(int64_t streams, int64_t nc, int img) {
+  return std::max<int64_t>(1, std::min(nc, IMAGE_BYTES / (streams * img)));
 }
 
 template <int KN, int NS>
 int run(const TcCall& a, cudaStream_t st) {
-  const int64_t streams = a.Bt * a.H, nc = cdiv(a.L, Q), seg = segment_chunks(streams, nc);
+  const int64_t streams = a.Bt * a.H, nc = cdiv(a.L, Q), seg = segment_chunks(streams, nc, IMG);
   CUtensorMap mk, mq, mu, my;
   if (!map_bf16(&mk, a.B, a.G * a.N, a.L, a.Bt, true) || !map_bf16(&mq, a.C, a.G * a.N, a.L, a.Bt, true) ||
       !map_bf16(&mu, a.u, a.H * a.P, a.L, a.Bt, false) || !map_bf16(&my, a.y, a.H * a.P, a.L, a.Bt, false)) {
@@ -578,7 +931,7 @@ int run(const TcCall& a, cudaStream_t st) {
     set_error("gated_delta_rule: device status word unavailable");
     return TSSM_ERR_CUDA;
   }
-  auto prep = delta_prep_kernel<KN>;
+  auto prep = delta_prep_kernel<KN, 2>;
   auto scan = delta_scan_kernel<KN, NS>;
   if (cudaFuncSetAttribute(prep, cudaFuncAttributeMaxDynamicSharedMemorySize, PrepSmem<KN>::BYTES) != cudaSuccess ||
       cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem<KN>::BYTES) != cudaSuccess)
@@ -598,6 +951,38 @@ int run(const TcCall& a, cudaStream_t st) {
   return check_launch("gated_delta_rule");
 }
 
+template <int KN>
+int run_back(const TcBackCall& a, cudaStream_t st) {
+  const int64_t streams = a.Bt * a.H, nc = cdiv(a.L, Q), seg = segment_chunks(streams, nc, IMG3);
+  CUtensorMap mk, mq, mo;
+  if (!map_bf16(&mk, a.B, a.G * a.N, a.L, a.Bt, true) || !map_bf16(&mq, a.C, a.G * a.N, a.L, a.Bt, true) ||
+      !map_bf16(&mo, a.dy, a.H * a.P, a.L, a.Bt, false)) {
+    set_error("gated_delta_rule_bwd: cuTensorMapEncodeTiled failed");
+    return TSSM_ERR_CUDA;
+  }
+  int* status = device_status_ptr();
+  if (!status) {
+    set_error("gated_delta_rule_bwd: device status word unavailable");
+    return TSSM_ERR_CUDA;
+  }
+  auto prep = delta_prep_kernel<KN, 3>;
+  auto scan = delta_back_scan_kernel<KN>;
+  if (cudaFuncSetAttribute(prep, cudaFuncAttributeMaxDynamicSharedMemorySize, PrepSmem<KN>::BYTES) != cudaSuccess ||
+      cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, BackSmem<KN>::BYTES) != cudaSuccess)
+    return check_launch("gated_delta_rule_bwd: set smem attribute");
+  uint8_t* img = (uint8_t*)a.ws;
+  for (int64_t end = nc; end > 0; end -= seg) {   // segments from the last; dh0 carries the state's gradient
+    const int64_t c0 = std::max<int64_t>(0, end - seg), m = end - c0;
+    const PrepArgs p{(const __nv_bfloat16*)a.B, (const __nv_bfloat16*)a.C, a.A_log, a.dt, a.beta, img, a.L, c0, m,
+                     (int)a.H, (int)a.G, (int)a.N, a.scale};
+    prep<<<(unsigned)(streams * m), 128, PrepSmem<KN>::BYTES, st>>>(p);
+    const BackArgs s{img, end == nc ? a.dh_last : a.dh0, a.dh0, a.dstates, a.derrs, (__nv_bfloat16*)a.du, status, a.L,
+                     c0, m, nc, (int)a.H, (int)a.G, (int)a.P, (int)a.N, (int)cdiv(a.P, 128), a.scale};
+    scan<<<(unsigned)(streams * s.npb), 384, BackSmem<KN>::BYTES, st>>>(mk, mq, mo, s);
+  }
+  return check_launch("gated_delta_rule_bwd: chain");
+}
+
 }  // namespace
 
 bool tc_takes(int64_t P, int64_t N, int dtype) {
@@ -605,12 +990,23 @@ bool tc_takes(int64_t P, int64_t N, int dtype) {
 }
 
 int64_t tc_workspace(int64_t Bt, int64_t L, int64_t H, int64_t P, int64_t N) {
-  const int64_t streams = Bt * H, nc = cdiv(L, Q), seg = segment_chunks(streams, nc);
+  const int64_t streams = Bt * H, nc = cdiv(L, Q), seg = segment_chunks(streams, nc, IMG);
   return streams * seg * IMG + (seg < nc ? streams * P * N * 4 : 0);
 }
 
+int64_t tc_back_workspace(int64_t Bt, int64_t L, int64_t H) {
+  return Bt * H * segment_chunks(Bt * H, cdiv(L, Q), IMG3) * IMG3;
+}
+
+int tc_back_run(const TcBackCall& a, cudaStream_t st) {
+  TSSM_REQUIRE(a.Bt * a.H * std::max(cdiv(a.P, 128), segment_chunks(a.Bt * a.H, cdiv(a.L, Q), IMG3)) < (int64_t(1) << 31) &&
+                   a.H * a.P < (int64_t(1) << 31) && a.G * a.N < (int64_t(1) << 31),
+               "gated_delta_rule_bwd: size out of range");
+  return a.N == 64 ? run_back<64>(a, st) : run_back<128>(a, st);
+}
+
 int tc_run(const TcCall& a, cudaStream_t st) {
-  TSSM_REQUIRE(a.Bt * a.H * std::max(cdiv(a.P, 128), segment_chunks(a.Bt * a.H, cdiv(a.L, Q))) < (int64_t(1) << 31) &&
+  TSSM_REQUIRE(a.Bt * a.H * std::max(cdiv(a.P, 128), segment_chunks(a.Bt * a.H, cdiv(a.L, Q), IMG)) < (int64_t(1) << 31) &&
                    a.H * a.P < (int64_t(1) << 31) && a.G * a.N < (int64_t(1) << 31),
                "gated_delta_rule: size out of range");
   const bool f32_out = a.h_last || a.states;

@@ -15,9 +15,20 @@ struct TcCall {
   int64_t Bt, L, H, G, P, N;
   float scale;
 };
+struct TcBackCall {   // the backward's chain: dE, du, dS1 of every chunk, dh0
+  const void *B, *C, *dy;
+  const float *A_log, *dt, *beta, *dh_last;
+  void* du;
+  float *dh0, *dstates, *derrs;
+  void* ws;
+  int64_t Bt, L, H, G, P, N;
+  float scale;
+};
 bool tc_takes(int64_t P, int64_t N, int dtype);   // shapes; the tensors must be 16-byte aligned as well
 int64_t tc_workspace(int64_t Bt, int64_t L, int64_t H, int64_t P, int64_t N);
 int tc_run(const TcCall& a, cudaStream_t st);
+int64_t tc_back_workspace(int64_t Bt, int64_t L, int64_t H);
+int tc_back_run(const TcBackCall& a, cudaStream_t st);
 
 }  // namespace delta
 }  // namespace tssm
