@@ -470,8 +470,9 @@ int tssm_gated_delta_step(const void* x, const void* dt, void* h, const void* A_
  * single token).  u, y [Bt,L,H,P] and B, C [Bt,L,G,N] io (f32 or bf16); dt,
  * beta [Bt,L,H] f32; A_log [H] f32; h0, h_last [Bt,H,P,N] f32 (either may be
  * null); N <= 128; all contiguous.  states [Bt,H,ceil(L/64),ceil(N/4),P,4]
- * f32 (the state before every 64-token chunk, four n beside each other) and errors [Bt,L,H,P] f32 (u - hd B) are
- * what the backward reads; both null when none follows.  workspace:
+ * f32 (the state before every 64-token chunk, four n beside each other) and
+ * errors [Bt,H,ceil(L/4),P,4] f32 (u - hd B, four tokens beside each other)
+ * are what the backward reads; 16-byte aligned, both null when none follows.  workspace:
  * tssm_gated_delta_rule_workspace_size bytes (0 for shapes that need none),
  * 16-byte aligned.
  */

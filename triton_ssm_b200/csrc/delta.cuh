@@ -121,10 +121,12 @@ __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool l
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void bar_sync(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 
-// The saved states of a chunk: [ceil(N / 4)][P][4] floats, so that lanes on neighbouring value
-// channels write (and read) neighbouring 16 bytes.  Two adjacent n (n even) of channel p:
-__device__ __forceinline__ float2* saved_pair(float* chunk, int P, int p, int n) {
-  return reinterpret_cast<float2*>(chunk + ((int64_t)(n >> 2) * P + p) * 4 + (n & 2));
+// What the forward saves, and the backward's chain leaves for its gradients, has a value
+// channel's rows four beside each other: the states of a chunk [ceil(N / 4)][P][4], the errors of
+// a (batch row, head) [ceil(L / 4)][P][4], so that lanes on neighbouring channels move neighbouring
+// 16 bytes.  Two adjacent n (or tokens; n even) of channel p:
+__device__ __forceinline__ float2* saved_pair(float* base, int P, int p, int64_t n) {
+  return reinterpret_cast<float2*>(base + ((n >> 2) * P + p) * 4 + (n & 2));
 }
 __host__ __device__ constexpr inline int64_t saved_floats(int64_t P, int64_t N) { return (N + 3) / 4 * 4 * P; }
 

@@ -37,7 +37,7 @@ struct BwdArgs {
   int H, G, P, N, npb;
   int64_t nc;
   float scale;
-  int vec_kq, vec_v, vec_p4;
+  int vec_kq, vec_v;
 };
 
 // ------------------------------------------------------------------ the chain
@@ -230,15 +230,18 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(cons
     }
     // dE in f32 for the gradient kernel, du in io
     const int64_t at = (b * a.L + t0) * su + (int64_t)h * a.P + pb + p0 + pr;
+    float* ep = a.derrs + bh * saved_floats(a.P, a.L);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int tk = 8 * i + q2 + (e & 1), p = (e >> 1) * 8;
-        if (tk < rows && p0 + pr + p < pvalid) {
-          a.derrs[at + (int64_t)tk * su + p] = er[i][e];
-          stf((T*)a.du + at + (int64_t)tk * su + p, er[i][e]);
-        }
+      for (int r = 0; r < 2; ++r) {
+        const int tk = 8 * i + q2, p = 8 * r;
+        if (p0 + pr + p >= pvalid) continue;
+        if ((tk & ~3) < rows)
+          *saved_pair(ep, a.P, pb + p0 + pr + p, t0 + tk) = make_float2(er[i][2 * r], er[i][2 * r + 1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (tk + e < rows) stf((T*)a.du + at + (int64_t)(tk + e) * su + p, er[i][2 * r + e]);
       }
   };
 
@@ -276,22 +279,6 @@ struct GradSmem {
 };
 constexpr int GT = 512;   // threads: warp = (16 tokens, a quarter of N)
 
-// Eight f32 of a tile's piece (row r, columns 8 c ..), zeros outside.
-__device__ __forceinline__ void fetch8(const float* src, int64_t stride, int rows, int valid, bool vec, int r, int c,
-                                       float (&f)[8]) {
-  if (vec) {
-#pragma unroll
-    for (int q = 0; q < 2; ++q) {
-      const float4 v = r < rows && 8 * c + 4 * q < valid
-                           ? *reinterpret_cast<const float4*>(src + (int64_t)r * stride + 8 * c + 4 * q)
-                           : make_float4(0.f, 0.f, 0.f, 0.f);
-      f[4 * q] = v.x; f[4 * q + 1] = v.y; f[4 * q + 2] = v.z; f[4 * q + 3] = v.w;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = r < rows && 8 * c + e < valid ? src[(int64_t)r * stride + 8 * c + e] : 0.f;
-  }
-}
 __device__ __forceinline__ void put8(uint8_t* dst, int plane, const float (&f)[8]) {
   uint32_t w[4][3];
 #pragma unroll
@@ -299,6 +286,19 @@ __device__ __forceinline__ void put8(uint8_t* dst, int plane, const float (&f)[8
 #pragma unroll
   for (int z = 0; z < 3; ++z)
     *reinterpret_cast<uint4*>(dst + z * plane) = make_uint4(w[0][z], w[1][z], w[2][z], w[3][z]);
+}
+
+// Four tokens (rows from r) of channels 2 lane, 2 lane + 1 into three planes of a 64 x 64 tile.
+__device__ __forceinline__ void put4x2(uint8_t* tile, int r, int lane, const float4 (&f)[2]) {
+  const float a[4] = {f[0].x, f[0].y, f[0].z, f[0].w}, b[4] = {f[1].x, f[1].y, f[1].z, f[1].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w[3];
+    split2<3>(a[i], b[i], w);
+#pragma unroll
+    for (int z = 0; z < 3; ++z)
+      *reinterpret_cast<uint32_t*>(tile + z * SQ_BYTES + tile_off<SQ_RB>(r + i, lane / 4) + 4 * (lane % 4)) = w[z];
+  }
 }
 
 template <int XS, int KN>
@@ -325,8 +325,8 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
   const float* S0 = a.states + (bh * a.nc + c) * saved_floats(a.P, a.N);
   const float* dS = a.dstates + (bh * a.nc + c) * saved_floats(a.P, a.N);
   const int64_t tok = (b * a.L + t0) * su + (int64_t)h * a.P;
-  // A thread's pieces: row er, piece ec of the 64 x 64 tiles; rows sr, piece sc of the state's.
-  const int er = tid / 8, ec = tid % 8, sr = tid % 64, sc = tid / 64;   // state: lanes on neighbouring rows
+  // A thread's state pieces: row sr, pieces sc, sc + 8.
+  const int sr = tid % 64, sc = tid / 64;   // lanes on neighbouring rows
   float fs[SP][8];                    // the next state pieces, in flight during the products
   auto fetch_state = [&](const float* src, int p0) {
 #pragma unroll
@@ -363,14 +363,19 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
     const int pv = min(64, a.P - p0);
     if (p0) __syncthreads();
     {
-      float fe[8], fd[8];
-      fetch8(a.errs + tok + p0, su, rows, pv, a.vec_p4, er, ec, fe);
-      fetch8(a.derrs + tok + p0, su, rows, pv, a.vec_p4, er, ec, fd);
+      float4 fe[2], fd[2];   // four tokens from 4 warp of channels 2 lane, 2 lane + 1
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const bool in = 4 * warp < rows && 2 * lane + q < pv;
+        const int64_t at = bh * saved_floats(a.P, a.L) + ((t0 / 4 + warp) * a.P + p0 + 2 * lane + q) * 4;
+        fe[q] = in ? *reinterpret_cast<const float4*>(a.errs + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+        fd[q] = in ? *reinterpret_cast<const float4*>(a.derrs + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
       load_planes<XS, 64, GT>(s + SM::DO, SQ_BYTES, (const T*)a.dy + tok + p0, su, rows, pv, a.vec_v, tid);
 #pragma unroll
       for (int i = 0; i < SP; ++i) put8(smem + SM::S + tile_off<RB>(sr, sc + 8 * i), SM::PLANE, fs[i]);
-      put8(smem + SM::E + tile_off<SQ_RB>(er, ec), SQ_BYTES, fe);
-      put8(smem + SM::DE + tile_off<SQ_RB>(er, ec), SQ_BYTES, fd);
+      put4x2(smem + SM::E, 4 * warp, lane, fe);
+      put4x2(smem + SM::DE, 4 * warp, lane, fd);
     }
     cp_async_wait_all();
     __syncthreads();
@@ -756,7 +761,7 @@ BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N
   const int64_t nc = cdiv(L, delta::Q);
   BwdSpace s;
   s.dstates = Bt * H * nc * saved_floats(P, N);
-  s.derrs = up(Bt * L * H * P);
+  s.derrs = Bt * H * saved_floats(P, L);
   s.part = H == G ? 0 : up(Bt * L * H * N);
   s.da = up(Bt * H * nc);
   s.img = tc_takes(P, N, dtype) ? tc_back_workspace(Bt, L, H) / 4 : 0;
@@ -802,7 +807,8 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
     if (cudaMemsetAsync(dA_log, 0, H * 4, st) != cudaSuccess) return check_launch("gated_delta_rule_bwd: clear");
     return TSSM_OK;
   }
-  TSSM_REQUIRE(Bt * L == 0 || aligned16(states), "gated_delta_rule_bwd: states must be 16-byte aligned");
+  TSSM_REQUIRE(Bt * L == 0 || (aligned16(states) && aligned16(errors)),
+               "gated_delta_rule_bwd: states and errors must be 16-byte aligned");
   const BwdSpace sp = space(Bt, L, H, G, P, N, dtype);
   BwdArgs a{};
   a.u = u; a.B = B; a.C = C; a.dy = dy;
@@ -824,7 +830,6 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
   const int per = dtype == TSSM_F32 ? 4 : 8;
   a.vec_kq = N % per == 0 && aligned16(B) && aligned16(C);
   a.vec_v = P % per == 0 && aligned16(dy);
-  a.vec_p4 = P % 4 == 0 && aligned16(errors);
   if (dtype == TSSM_F32) return N <= 64 ? launch_all<3, 64>(a, st) : launch_all<3, 128>(a, st);
   return N <= 64 ? launch_all<1, 64>(a, st) : launch_all<1, 128>(a, st);
 }

@@ -187,13 +187,14 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
       }
     }
     if (a.errs) {
-      float* ep = a.errs + ((b * a.L + t0) * a.H + h) * (int64_t)a.P + pb + p0 + pr;
+      float* ep = a.errs + bh * saved_floats(a.P, a.L);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int tk = 8 * i + q2 + (e & 1), p = (e >> 1) * 8;
-          if (tk < rows && p0 + pr + p < pvalid) ep[(int64_t)tk * su + p] = er[i][e];
+        for (int r = 0; r < 2; ++r) {   // groups of four tokens that reach the end; behind it e = 0
+          const int tk = 8 * i + q2, p = p0 + pr + 8 * r;
+          if ((tk & ~3) < rows && p < pvalid)
+            *saved_pair(ep, a.P, pb + p, t0 + tk) = make_float2(er[i][2 * r], er[i][2 * r + 1]);
         }
     }
     // O^T: the state's part (x is free now), then the chunk's own

@@ -348,11 +348,13 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
         tmem_get16(tl + C_E + 32 * half + 16, x[1]);
         if (a.errs && live && ok) {
           const int64_t tk = (a.c0 + c) * Q + 32 * half;
-          float* ep = a.errs + ((b * a.L + tk) * a.H + h) * (int64_t)a.P + pb + p;
+          float4* ep = reinterpret_cast<float4*>(a.errs + bh * saved_floats(a.P, a.L)) + tk / 4 * a.P + pb + p;
           const int left = (int)min((int64_t)32, a.L - tk);
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (j < left) ep[(int64_t)j * a.H * a.P] = x[j >> 4][j & 15];
+          for (int j = 0; j < 32; j += 4)   // tokens behind the end have e = 0
+            if (j < left)
+              ep[j / 4 * a.P] = make_float4(x[j >> 4][j & 15], x[j >> 4][(j + 1) & 15], x[j >> 4][(j + 2) & 15],
+                                            x[j >> 4][(j + 3) & 15]);
         }
         store_planes<2>(tl + C_E + 32 * half, 16, x[0]);
         store_planes<2>(tl + C_E + 32 * half + 8, 16, x[1]);
@@ -764,13 +766,15 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
         tmem_get16(tl + C_E + 32 * half + 16 * i, x);
         const int64_t tk = cc * Q + 32 * half + 16 * i;
         const int left = live && ok ? (int)max((int64_t)0, min((int64_t)16, a.L - tk)) : 0;
-        const int64_t at = ((b * a.L + tk) * a.H + h) * (int64_t)a.P + pb + p;
+        float4* ep = reinterpret_cast<float4*>(a.derrs + bh * saved_floats(a.P, a.L)) + tk / 4 * a.P + pb + p;
+        __nv_bfloat16* up = a.du + ((b * a.L + tk) * a.H + h) * (int64_t)a.P + pb + p;
+        const int su = a.H * a.P;
+#pragma unroll
+        for (int j = 0; j < 16; j += 4)
+          if (j < left) ep[j / 4 * a.P] = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
 #pragma unroll
         for (int j = 0; j < 16; ++j)
-          if (j < left) {
-            a.derrs[at + (int64_t)j * a.H * a.P] = x[j];
-            a.du[at + (int64_t)j * a.H * a.P] = __float2bfloat16_rn(x[j]);
-          }
+          if (j < left) up[j * su] = __float2bfloat16_rn(x[j]);
       }
       // dS^T
       ok = ok && waitw(dsdone, k, 2105);

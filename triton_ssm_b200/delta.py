@@ -69,7 +69,7 @@ def gated_delta_rule(u, A_log, B, C, dt, beta, scale=1.0, h0=None, return_state=
     f32 when ``return_state``, then, when ``save``, what
     ``gated_delta_rule_bwd`` reads: (the state before every chunk of 64 tokens
     [Bt,H,ceil(L/64),ceil(N/4),P,4], the prediction errors u_t - hd B_t
-    [Bt,L,H,P]), f32.
+    [Bt,H,ceil(L/4),P,4]), f32.
     """
     dev = same_device(u, A_log, B, C, dt, beta, h0, y)
     Bt, L, H, G, P, N = _rule_args("gated_delta_rule", u, A_log, B, C, dt, beta, h0)
@@ -83,7 +83,7 @@ def gated_delta_rule(u, A_log, B, C, dt, beta, scale=1.0, h0=None, return_state=
     f32 = dict(device=u.device, dtype=torch.float32)
     hl = torch.empty(Bt, H, P, N, **f32) if return_state else None
     states = torch.empty(Bt, H, -(-L // CHUNK), -(-N // 4), P, 4, **f32) if save else None
-    errors = torch.empty(Bt, L, H, P, **f32) if save else None
+    errors = torch.empty(Bt, H, -(-L // 4), P, 4, **f32) if save else None
     need = int(_lib.load_library().tssm_gated_delta_rule_workspace_size(Bt, L, H, G, P, N, dtype_code(u)))
     ws = torch.empty(need, dtype=torch.uint8, device=u.device) if need else None
     with on_device(dev):
@@ -111,7 +111,7 @@ def gated_delta_rule_bwd(u, A_log, B, C, dt, beta, dy, saved, scale=1.0, dh_last
     Bt, L, H, G, P, N = _rule_args("gated_delta_rule_bwd", u, A_log, B, C, dt, beta, dh_last)
     if dy.shape != u.shape or dy.dtype != u.dtype:
         raise ValueError("gated_delta_rule_bwd: dy must match u")
-    for t, shape in ((states, (Bt, H, -(-L // CHUNK), -(-N // 4), P, 4)), (errors, (Bt, L, H, P))):
+    for t, shape in ((states, (Bt, H, -(-L // CHUNK), -(-N // 4), P, 4)), (errors, (Bt, H, -(-L // 4), P, 4))):
         if tuple(t.shape) != shape or t.dtype != torch.float32 or not t.is_contiguous():
             raise ValueError("gated_delta_rule_bwd: saved must be what gated_delta_rule(..., save=True) returned")
     u, B, C, dy = _dense(u), _dense(B), _dense(C), _dense(dy)
