@@ -146,6 +146,13 @@ struct Gates {        // in shared memory
   float beta[Q];
 };
 
+static_assert(sizeof(Gates) % 16 == 0, "copied in 16-byte pieces");
+// 128 threads (t): the gates of a chunk to HBM.
+__device__ __forceinline__ void copy_gates(Gates* dst, const Gates& g, int t) {
+  for (int i = t; i < (int)(sizeof(Gates) / 16); i += 128)
+    reinterpret_cast<uint4*>(dst)[i] = reinterpret_cast<const uint4*>(&g)[i];
+}
+
 __device__ __forceinline__ float exp2_pair(float h, float l) {
   const float e = exp2f(h);
   return e + e * (l * 0.6931471805599453f);

@@ -32,6 +32,7 @@ struct BwdArgs {
   void *du, *dB, *dC;
   float *dA_log, *ddt, *dbeta, *dh0;
   float *dstates, *derrs, *dk_part, *dq_part, *da_part;   // workspace
+  Gates* gates;   // of every chunk, left by the chain
   void* img;   // the tcgen05 chain's workspace; null: the register chain
   int64_t Bt, L;
   int H, G, P, N, npb;
@@ -82,6 +83,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(cons
       gates_warp(gt, a.dt + b * a.L * a.H + h, a.beta + b * a.L * a.H + h, a.H, a.A_log[h], t0, a.L, t);
     cp_async_wait_all();
     bar_sync(1, 128);
+    if (pb == 0) copy_gates(a.gates + bh * a.nc + c, gt, t);
     chunk_matrices<XS, KN, 3, 3>(s + SM::K, s + SM::QQ, gt, a.scale, reinterpret_cast<float*>(smem + SM::M),
                                  buf + SM::AQ, buf + SM::T, t, 1);
   };
@@ -316,7 +318,7 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
   const int h = (int)(bh - b * a.H), g = h / (a.H / a.G);
   const int64_t t0 = c * Q, su = (int64_t)a.H * a.P, sk = (int64_t)a.G * a.N;
   const int rows = (int)min((int64_t)Q, a.L - t0);
-  Gates& gt = *reinterpret_cast<Gates*>(smem + SM::G);
+  const Gates& gt = *reinterpret_cast<const Gates*>(smem + SM::G);
   float* vec = reinterpret_cast<float*>(smem + SM::VEC);
   float *va = vec, *vb = vec + 4 * Q, *vw = vec + 8 * Q;   // [4][Q] row dots of a, b, and w e.(K dS1), by quarter
   float* seg = vec + 12 * Q;                               // [8][Q] column sums of Y by row eighth
@@ -327,8 +329,8 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
   const int64_t tok = (b * a.L + t0) * su + (int64_t)h * a.P;
   // A thread's state pieces: row sr, pieces sc, sc + 8.
   const int sr = tid % 64, sc = tid / 64;   // lanes on neighbouring rows
-  float fs[SP][8];                    // the next state pieces, in flight during the products
-  auto fetch_state = [&](const float* src, int p0) {
+  float fs[SP][8];   // the next pieces of S0 and dS1, in flight during the products
+  auto fetch_state = [&](const float* src, int p0, float (&fs)[SP][8]) {
 #pragma unroll
     for (int i = 0; i < SP; ++i)
 #pragma unroll
@@ -340,13 +342,15 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
         fs[i][4 * q] = v.x; fs[i][4 * q + 1] = v.y; fs[i][4 * q + 2] = v.z; fs[i][4 * q + 3] = v.w;
       }
   };
-  fetch_state(S0, 0);
+  float fd[SP][8];
+  fetch_state(S0, 0, fs);
+  fetch_state(dS, 0, fd);
+  if (tid < (int)(sizeof(Gates) / 16))
+    cp_async16(s + SM::G + 16 * tid, reinterpret_cast<const uint4*>(a.gates + bh * a.nc + c) + tid, true);
   load_planes<XS, KN, GT>(s + SM::K, SM::PLANE, (const T*)a.B + (b * a.L + t0) * sk + (int64_t)g * a.N, sk, rows, a.N,
                           a.vec_kq, tid);
   load_planes<XS, KN, GT>(s + SM::QQ, SM::PLANE, (const T*)a.C + (b * a.L + t0) * sk + (int64_t)g * a.N, sk, rows, a.N,
                           a.vec_kq, tid);
-  if (warp == 0)
-    gates_warp(gt, a.dt + b * a.L * a.H + h, a.beta + b * a.L * a.H + h, a.H, a.A_log[h], t0, a.L, lane);
 
   float dq0[NTQ][4], dk0[NTQ][4], dk1[NTQ][4], m1[2][4], m2[2][4];
   auto zero = [](auto& m) {
@@ -363,23 +367,26 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
     const int pv = min(64, a.P - p0);
     if (p0) __syncthreads();
     {
-      float4 fe[2], fd[2];   // four tokens from 4 warp of channels 2 lane, 2 lane + 1
+      float4 fe[2], fr[2];   // four tokens from 4 warp of channels 2 lane, 2 lane + 1
 #pragma unroll
       for (int q = 0; q < 2; ++q) {
         const bool in = 4 * warp < rows && 2 * lane + q < pv;
         const int64_t at = bh * saved_floats(a.P, a.L) + ((t0 / 4 + warp) * a.P + p0 + 2 * lane + q) * 4;
         fe[q] = in ? *reinterpret_cast<const float4*>(a.errs + at) : make_float4(0.f, 0.f, 0.f, 0.f);
-        fd[q] = in ? *reinterpret_cast<const float4*>(a.derrs + at) : make_float4(0.f, 0.f, 0.f, 0.f);
+        fr[q] = in ? *reinterpret_cast<const float4*>(a.derrs + at) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
       load_planes<XS, 64, GT>(s + SM::DO, SQ_BYTES, (const T*)a.dy + tok + p0, su, rows, pv, a.vec_v, tid);
 #pragma unroll
-      for (int i = 0; i < SP; ++i) put8(smem + SM::S + tile_off<RB>(sr, sc + 8 * i), SM::PLANE, fs[i]);
+      for (int i = 0; i < SP; ++i) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dot += fs[i][e] * fd[i][e];
+        put8(smem + SM::S + tile_off<RB>(sr, sc + 8 * i), SM::PLANE, fs[i]);
+      }
       put4x2(smem + SM::E, 4 * warp, lane, fe);
-      put4x2(smem + SM::DE, 4 * warp, lane, fd);
+      put4x2(smem + SM::DE, 4 * warp, lane, fr);
     }
     cp_async_wait_all();
     __syncthreads();
-    fetch_state(dS, p0);
 #pragma unroll 1
     for (int kk = 0; kk < 4; ++kk) {
       uint32_t fo[XS][4], fe[3][4], w[3][4];
@@ -402,25 +409,14 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
       }
     }
     __syncthreads();
-    // dS1 takes S0's place; <S0, dS1> on the way (the planes of S0 add up to its f32 values)
+    // dS1 takes S0's place
 #pragma unroll
-    for (int i = 0; i < SP; ++i) {
-      uint8_t* at = smem + SM::S + tile_off<RB>(sr, sc + 8 * i);
-      float o[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] = 0.f;
-#pragma unroll
-      for (int z = 2; z >= 0; --z) {
-        const uint4 v = *reinterpret_cast<const uint4*>(at + z * SM::PLANE);
-        o[0] += lo2(v.x); o[1] += hi2(v.x); o[2] += lo2(v.y); o[3] += hi2(v.y);
-        o[4] += lo2(v.z); o[5] += hi2(v.z); o[6] += lo2(v.w); o[7] += hi2(v.w);
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dot += o[e] * fs[i][e];
-      put8(at, SM::PLANE, fs[i]);
-    }
+    for (int i = 0; i < SP; ++i) put8(smem + SM::S + tile_off<RB>(sr, sc + 8 * i), SM::PLANE, fd[i]);
     __syncthreads();
-    if (p0 + 64 < a.P) fetch_state(S0, p0 + 64);
+    if (p0 + 64 < a.P) {
+      fetch_state(S0, p0 + 64, fs);
+      fetch_state(dS, p0 + 64, fd);
+    }
 #pragma unroll 1
     for (int kk = 0; kk < 4; ++kk) {
       uint32_t fe[3][4], w[3][4];
@@ -487,7 +483,7 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
     zero(gk);
     zero(gq);
     if (qt <= mt) {
-#pragma unroll 1
+#pragma unroll 4
       for (int kk = 0; kk < KN / 16; ++kk) {
         uint32_t fk[XS][4], fq[XS][4], w[XS][4];
 #pragma unroll
@@ -725,7 +721,7 @@ template <int XS, int KN>
 int launch_all(const BwdArgs& a, cudaStream_t st) {
   using T = typename std::conditional<XS == 1, __nv_bfloat16, float>::type;
   if (a.img) {
-    const TcBackCall t{a.B, a.C, a.dy, a.A_log, a.dt, a.beta, a.dh_last, a.du, a.dh0, a.dstates, a.derrs, a.img,
+    const TcBackCall t{a.B, a.C, a.dy, a.A_log, a.dt, a.beta, a.dh_last, a.du, a.dh0, a.dstates, a.derrs, a.gates, a.img,
                        a.Bt, a.L, a.H, a.G, a.P, a.N, a.scale};
     if (int e = tc_back_run(t, st)) return e;
   } else {
@@ -754,7 +750,7 @@ int launch_all(const BwdArgs& a, cudaStream_t st) {
 // Workspace in floats: dS1 of every chunk, dE, per-head dK and dQ (shared key heads), dA parts,
 // the tcgen05 chain's images.
 struct BwdSpace {
-  int64_t dstates, derrs, part, da, img, total;
+  int64_t dstates, derrs, part, da, gates, img, total;
 };
 BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N, int dtype) {
   auto up = [](int64_t n) { return (n + 3) / 4 * 4; };
@@ -765,7 +761,8 @@ BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N
   s.part = H == G ? 0 : up(Bt * L * H * N);
   s.da = up(Bt * H * nc);
   s.img = tc_takes(P, N, dtype) ? tc_back_workspace(Bt, L, H) / 4 : 0;
-  s.total = s.dstates + s.derrs + 2 * s.part + s.da + s.img;
+  s.gates = Bt * H * nc * (int64_t)(sizeof(Gates) / 4);
+  s.total = s.dstates + s.derrs + 2 * s.part + s.da + s.gates + s.img;
   return s;
 }
 
@@ -823,7 +820,8 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
   a.da_part = a.derrs + sp.derrs + 2 * sp.part;
   const uintptr_t bases = reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(dy) |
                           reinterpret_cast<uintptr_t>(dh_last) | reinterpret_cast<uintptr_t>(dh0);
-  a.img = sp.img && L > 0 && (bases & 15u) == 0 ? a.da_part + sp.da : nullptr;
+  a.gates = (Gates*)(a.da_part + sp.da);
+  a.img = sp.img && L > 0 && (bases & 15u) == 0 ? a.da_part + sp.da + sp.gates : nullptr;
   a.Bt = Bt; a.L = L; a.H = (int)H; a.G = (int)G; a.P = (int)P; a.N = (int)N;
   a.nc = cdiv(L, delta::Q);
   a.scale = (float)scale;

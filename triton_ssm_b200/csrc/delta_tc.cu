@@ -59,7 +59,8 @@ struct PrepArgs {
   const __nv_bfloat16 *B, *C;
   const float *A_log, *dt, *beta;
   uint8_t* img;
-  int64_t L, c0, nseg;   // first chunk and chunks of the segment
+  Gates* gates;          // [Bt, H, nc] or null: for the gradient kernel
+  int64_t L, c0, nseg, nc;   // first chunk and chunks of the segment
   int H, G, N;
   float scale;
 };
@@ -92,6 +93,7 @@ __global__ void __launch_bounds__(128, 6) delta_prep_kernel(const PrepArgs a) {
   uint8_t* img = a.img + (bh * a.nseg + ci) * img_bytes(NA);
   float* go = reinterpret_cast<float*>(img + img_gates(NA));
   go[t] = t < Q ? gt.eg[t] : gt.wb[t - Q];
+  if (a.gates) copy_gates(a.gates + bh * a.nc + a.c0 + ci, gt, t);
   chunk_matrices<1, KN, NA, 3, true>(s + SM::K, s + SM::QQ, gt, a.scale, reinterpret_cast<float*>(smem + SM::M), img + IMG_AQ,
                               img + IMG_T, t, 1);
 }
@@ -944,8 +946,8 @@ int run(const TcCall& a, cudaStream_t st) {
   float* carry = a.h_last ? a.h_last : (float*)(img + streams * seg * IMG);
   for (int64_t c0 = 0; c0 < nc; c0 += seg) {
     const int64_t m = std::min(seg, nc - c0);
-    const PrepArgs p{(const __nv_bfloat16*)a.B, (const __nv_bfloat16*)a.C, a.A_log, a.dt, a.beta, img, a.L, c0, m,
-                     (int)a.H, (int)a.G, (int)a.N, a.scale};
+    const PrepArgs p{(const __nv_bfloat16*)a.B, (const __nv_bfloat16*)a.C, a.A_log, a.dt, a.beta, img, nullptr, a.L, c0, m,
+                     nc, (int)a.H, (int)a.G, (int)a.N, a.scale};
     prep<<<(unsigned)(streams * m), 128, PrepSmem<KN>::BYTES, st>>>(p);
     const bool last = c0 + m == nc;
     const ScanArgs s{img, c0 ? carry : a.h0, last && !a.h_last ? nullptr : carry, a.states, a.errs, status, a.L, c0, m,
@@ -977,8 +979,8 @@ int run_back(const TcBackCall& a, cudaStream_t st) {
   uint8_t* img = (uint8_t*)a.ws;
   for (int64_t end = nc; end > 0; end -= seg) {   // segments from the last; dh0 carries the state's gradient
     const int64_t c0 = std::max<int64_t>(0, end - seg), m = end - c0;
-    const PrepArgs p{(const __nv_bfloat16*)a.B, (const __nv_bfloat16*)a.C, a.A_log, a.dt, a.beta, img, a.L, c0, m,
-                     (int)a.H, (int)a.G, (int)a.N, a.scale};
+    const PrepArgs p{(const __nv_bfloat16*)a.B, (const __nv_bfloat16*)a.C, a.A_log, a.dt, a.beta, img, (Gates*)a.gates, a.L, c0, m,
+                     nc, (int)a.H, (int)a.G, (int)a.N, a.scale};
     prep<<<(unsigned)(streams * m), 128, PrepSmem<KN>::BYTES, st>>>(p);
     const BackArgs s{img, end == nc ? a.dh_last : a.dh0, a.dh0, a.dstates, a.derrs, (__nv_bfloat16*)a.du, status, a.L,
                      c0, m, nc, (int)a.H, (int)a.G, (int)a.P, (int)a.N, (int)cdiv(a.P, 128), a.scale};

@@ -20,6 +20,7 @@ struct TcBackCall {   // the backward's chain: dE, du, dS1 of every chunk, dh0
   const float *A_log, *dt, *beta, *dh_last;
   void* du;
   float *dh0, *dstates, *derrs;
+  void* gates;   // one per (batch row, head, chunk)
   void* ws;
   int64_t Bt, L, H, G, P, N;
   float scale;
