@@ -491,7 +491,7 @@ int tssm_gated_delta_rule(const void* u, const void* A_log, const void* B, const
  * workspace: tssm_gated_delta_rule_bwd_workspace_size bytes, 16-byte aligned.
  */
 int64_t tssm_gated_delta_rule_bwd_workspace_size(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P,
-                                                 int64_t N, int dtype);
+                                                 int64_t N);
 int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const void* B, const void* C, const void* dt,
                               const void* beta, const void* dy, const void* states, const void* errors,
                               const void* dh_last, void* du, void* dA_log, void* dB, void* dC, void* ddt,

@@ -362,18 +362,29 @@ __device__ __forceinline__ void invert_unit_lower(float* M, int t, int bar) {
 // A 64 x 64 tile of planes: 128-byte rows.
 constexpr int SQ_RB = 128, SQ_BYTES = Q * SQ_RB;
 
+// A chunk's image, as it lies in shared memory: T planes, NA planes of Aq diag(beta), gates.
+constexpr int IMG_T = 0, IMG_AQ = 3 * SQ_BYTES;
+__host__ __device__ constexpr int img_gates(int na) { return IMG_AQ + na * SQ_BYTES; }
+__host__ __device__ constexpr int img_bytes(int na) { return img_gates(na) + (int)sizeof(Gates); }
+// NTH threads: an image to shared memory.
+template <int NA, int NTH>
+__device__ __forceinline__ void load_image(uint32_t dst, const uint8_t* src, int t) {
+#pragma unroll 4
+  for (int i = t; i < img_bytes(NA) / 16; i += NTH) cp_async16(dst + 16 * i, src + 16 * i, true);
+}
+
 // 128 threads (t = 0..127): from the loaded K, Q planes and the gates, the planes of
-// Aq diag(beta) (NA of them) and of T (NTP).  M is the f32 work matrix.  Entries of 16-blocks
+// Aq diag(beta) (NA of them) and of T (NTP).  M is the f32 work matrix; it may lie over the Q
+// planes (their product comes first).  Entries of 16-blocks
 // above the diagonal are not written: nobody reads them.
-// If ALIAS, M may lie over the Q planes (their product comes first).
-template <int XS, int KN, int NA, int NTP, bool ALIAS = false>
+template <int XS, int KN, int NA, int NTP>
 __device__ __forceinline__ void chunk_matrices(uint32_t k, uint32_t q, const Gates& g, float scale, float* M,
                                                uint8_t* aq, uint8_t* tp, int t, int bar) {
   constexpr int RB = KN * 2, PB = Q * RB, KK = KN / 16;
   const int w = t / 32, lane = t % 32, gr = lane / 4, q2 = 2 * (lane % 4);
 #pragma unroll
   for (int pass = 1; pass >= 0; --pass) {   // Q K^T, then K K^T with the rows dealt the other way round
-    if (ALIAS && pass == 0) bar_sync(bar, 128);
+    if (pass == 0) bar_sync(bar, 128);
     const int I = pass ? 3 - w : w, r0 = 16 * I + gr;
     uint32_t a[XS == 1 ? KK : 1][XS][4];   // this row block's operand (bf16: kept for all column blocks)
     if constexpr (XS == 1)

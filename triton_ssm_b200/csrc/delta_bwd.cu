@@ -32,11 +32,12 @@ struct BwdArgs {
   void *du, *dB, *dC;
   float *dA_log, *ddt, *dbeta, *dh0;
   float *dstates, *derrs, *dk_part, *dq_part, *da_part;   // workspace
-  Gates* gates;   // of every chunk, left by the chain
-  void* img;   // the tcgen05 chain's workspace; null: the register chain
-  int64_t Bt, L;
+  Gates* gates;   // of every chunk
+  uint8_t* img;   // of a segment
+  const float* ds_in;      // the chain's segment: its state gradient, first chunk, chunks
+  int64_t c0, nseg;
+  int64_t Bt, L, nc;
   int H, G, P, N, npb;
-  int64_t nc;
   float scale;
   int vec_kq, vec_v;
 };
@@ -47,8 +48,8 @@ struct ChainSmem {
   static constexpr int BUFS = XS == 1 ? 2 : 1;
   static constexpr int PB = 16 * NCW, PLANE = Q * KN * 2, DO_PLANE = Q * PB * 2;
   static constexpr int K = 0, QQ = K + XS * PLANE, DO = QQ + XS * PLANE, T = DO + XS * DO_PLANE, AQ = T + 3 * SQ_BYTES,
-                       G = AQ + 3 * SQ_BYTES, BUF = (G + (int)sizeof(Gates) + 127) / 128 * 128;
-  static constexpr int M = BUFS * BUF, BYTES = M + Q * AM * 4 + 128;
+                       G = AQ + 3 * SQ_BYTES, BUF = (G + (int)sizeof(Gates) + 127) / 128 * 128;   // T, AQ, G: an image
+  static constexpr int BYTES = BUFS * BUF + 128;
 };
 
 template <int XS, int KN, int NCW>
@@ -69,23 +70,19 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(cons
   const T* op = (const T*)a.dy + (b * a.L) * su + (int64_t)h * a.P + pb;
   const int pvalid = min(PB, a.P - pb);
 
-  auto prep = [&](int64_t c) {   // 128 threads
-    const int t = threadIdx.x - NCW * 32;
+  // Chunk c of the segment to shared memory: by the four loading warps, or (one buffer) by all.
+  constexpr int LT = SM::BUFS == 2 ? 128 : (NCW + 4) * 32;
+  auto load = [&](int64_t c) {
+    const int t = threadIdx.x - (SM::BUFS == 2 ? NCW * 32 : 0);
     uint8_t* buf = smem + (SM::BUFS == 2 ? (int)(c & 1) * SM::BUF : 0);
     const uint32_t s = smem_addr(buf);
-    const int64_t t0 = c * Q;
+    const int64_t t0 = (a.c0 + c) * Q;
     const int rows = (int)min((int64_t)Q, a.L - t0);
-    load_planes<XS, KN, 128>(s + SM::K, SM::PLANE, kp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
-    load_planes<XS, KN, 128>(s + SM::QQ, SM::PLANE, qp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
-    load_planes<XS, PB, 128>(s + SM::DO, SM::DO_PLANE, op + t0 * su, su, rows, pvalid, a.vec_v, t);
-    Gates& gt = *reinterpret_cast<Gates*>(buf + SM::G);
-    if (t < 32)
-      gates_warp(gt, a.dt + b * a.L * a.H + h, a.beta + b * a.L * a.H + h, a.H, a.A_log[h], t0, a.L, t);
+    load_image<3, LT>(s + SM::T, a.img + (bh * a.nseg + c) * img_bytes(3), t);
+    load_planes<XS, KN, LT>(s + SM::K, SM::PLANE, kp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
+    load_planes<XS, KN, LT>(s + SM::QQ, SM::PLANE, qp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
+    load_planes<XS, PB, LT>(s + SM::DO, SM::DO_PLANE, op + t0 * su, su, rows, pvalid, a.vec_v, t);
     cp_async_wait_all();
-    bar_sync(1, 128);
-    if (pb == 0) copy_gates(a.gates + bh * a.nc + c, gt, t);
-    chunk_matrices<XS, KN, 3, 3>(s + SM::K, s + SM::QQ, gt, a.scale, reinterpret_cast<float*>(smem + SM::M),
-                                 buf + SM::AQ, buf + SM::T, t, 1);
   };
 
   const int p0 = 16 * warp;
@@ -112,10 +109,10 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(cons
     uint8_t* buf = smem + (SM::BUFS == 2 ? (int)(c & 1) * SM::BUF : 0);
     const uint32_t s = smem_addr(buf);
     const Gates& gt = *reinterpret_cast<const Gates*>(buf + SM::G);
-    const int64_t t0 = c * Q;
+    const int64_t t0 = (a.c0 + c) * Q;
     const int rows = (int)min((int64_t)Q, a.L - t0);
     {
-      float* dst = a.dstates + (bh * a.nc + c) * saved_floats(a.P, a.N);
+      float* dst = a.dstates + (bh * a.nc + a.c0 + c) * saved_floats(a.P, a.N);
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -247,18 +244,18 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(cons
       }
   };
 
-  if (warp < NCW) state_io(nullptr, a.dh_last ? a.dh_last + srow : nullptr);
+  if (warp < NCW) state_io(nullptr, a.ds_in ? a.ds_in + srow : nullptr);
   if constexpr (SM::BUFS == 2) {
-    if (warp >= NCW && a.nc > 0) prep(a.nc - 1);
+    if (warp >= NCW) load(a.nseg - 1);
     __syncthreads();
-    for (int64_t c = a.nc - 1; c >= 0; --c) {
+    for (int64_t c = a.nseg - 1; c >= 0; --c) {
       if (warp < NCW) chain(c);
-      else if (c > 0) prep(c - 1);
+      else if (c > 0) load(c - 1);
       __syncthreads();
     }
   } else {
-    for (int64_t c = a.nc - 1; c >= 0; --c) {
-      if (warp >= NCW) prep(c);
+    for (int64_t c = a.nseg - 1; c >= 0; --c) {
+      load(c);
       __syncthreads();
       if (warp < NCW) chain(c);
       __syncthreads();
@@ -718,15 +715,29 @@ int launch_chain(BwdArgs a, cudaStream_t st) {
 }
 
 template <int XS, int KN>
-int launch_all(const BwdArgs& a, cudaStream_t st) {
+int launch_all(BwdArgs a, bool tc, cudaStream_t st) {
   using T = typename std::conditional<XS == 1, __nv_bfloat16, float>::type;
-  if (a.img) {
-    const TcBackCall t{a.B, a.C, a.dy, a.A_log, a.dt, a.beta, a.dh_last, a.du, a.dh0, a.dstates, a.derrs, a.gates, a.img,
-                       a.Bt, a.L, a.H, a.G, a.P, a.N, a.scale};
+  if (a.nc == 0) {   // no tokens: the state's gradient passes through
+    const size_t n = (size_t)(a.Bt * a.H * a.P) * a.N * 4;
+    if ((a.dh_last ? cudaMemcpyAsync(a.dh0, a.dh_last, n, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(a.dh0, 0, n, st)) !=
+        cudaSuccess)
+      return check_launch("gated_delta_rule_bwd: pass the state's gradient");
+  } else if (tc) {
+    const TcBackCall t{a.B, a.C, a.dy, a.A_log, a.dt, a.beta, a.dh_last, a.du, a.dh0, a.dstates, a.derrs, a.gates,
+                       a.img, a.Bt, a.L, a.H, a.G, a.P, a.N, a.scale};
     if (int e = tc_back_run(t, st)) return e;
   } else {
     const bool wide = a.P > 64 && a.Bt * a.H * cdiv(a.P, 128) >= num_sms();
-    if (int e = wide ? launch_chain<XS, KN, 8>(a, st) : launch_chain<XS, KN, 4>(a, st)) return e;
+    const int64_t seg = segment_chunks(a.Bt * a.H, a.nc, 3);
+    for (int64_t end = a.nc; end > 0; end -= seg) {   // segments from the last; dh0 carries the state's gradient
+      a.c0 = std::max<int64_t>(0, end - seg);
+      a.nseg = end - a.c0;
+      a.ds_in = end == a.nc ? a.dh_last : a.dh0;
+      const PrepCall p{a.B, a.C, a.A_log, a.dt, a.beta, a.img, a.gates, a.Bt, a.L, a.H, a.G, a.N, a.c0, a.nseg, a.nc,
+                       a.scale, a.vec_kq};
+      if (int e = prep_run(p, XS == 1 ? TSSM_BF16 : TSSM_F32, 3, st)) return e;
+      if (int e = wide ? launch_chain<XS, KN, 8>(a, st) : launch_chain<XS, KN, 4>(a, st)) return e;
+    }
   }
   if (a.nc > 0) {
     constexpr int bytes = GradSmem<XS, KN>::BYTES;
@@ -748,11 +759,11 @@ int launch_all(const BwdArgs& a, cudaStream_t st) {
 }
 
 // Workspace in floats: dS1 of every chunk, dE, per-head dK and dQ (shared key heads), dA parts,
-// the tcgen05 chain's images.
+// gates, a segment's images.
 struct BwdSpace {
   int64_t dstates, derrs, part, da, gates, img, total;
 };
-BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N, int dtype) {
+BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N) {
   auto up = [](int64_t n) { return (n + 3) / 4 * 4; };
   const int64_t nc = cdiv(L, delta::Q);
   BwdSpace s;
@@ -760,7 +771,7 @@ BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N
   s.derrs = Bt * H * saved_floats(P, L);
   s.part = H == G ? 0 : up(Bt * L * H * N);
   s.da = up(Bt * H * nc);
-  s.img = tc_takes(P, N, dtype) ? tc_back_workspace(Bt, L, H) / 4 : 0;
+  s.img = nc ? Bt * H * segment_chunks(Bt * H, nc, 3) * prep_image_bytes(3) / 4 : 0;
   s.gates = Bt * H * nc * (int64_t)(sizeof(Gates) / 4);
   s.total = s.dstates + s.derrs + 2 * s.part + s.da + s.gates + s.img;
   return s;
@@ -771,9 +782,9 @@ BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N
 }  // namespace tssm
 
 extern "C" int64_t tssm_gated_delta_rule_bwd_workspace_size(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P,
-                                                            int64_t N, int dtype) {
+                                                            int64_t N) {
   if (Bt <= 0 || L <= 0 || H <= 0 || G <= 0 || P <= 0 || N <= 0) return 0;
-  return tssm::delta::space(Bt, L, H, G, P, N, dtype).total * 4;
+  return tssm::delta::space(Bt, L, H, G, P, N).total * 4;
 }
 
 extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const void* B, const void* C, const void* dt,
@@ -795,7 +806,7 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
   TSSM_REQUIRE(A_log && dA_log && (Bt == 0 || dh0), "gated_delta_rule_bwd: null pointer");
   TSSM_REQUIRE(Bt * L == 0 || (u && B && C && dt && beta && dy && states && errors && du && dB && dC && ddt && dbeta),
                "gated_delta_rule_bwd: null pointer");
-  const int64_t need = tssm_gated_delta_rule_bwd_workspace_size(Bt, L, H, G, P, N, dtype);
+  const int64_t need = tssm_gated_delta_rule_bwd_workspace_size(Bt, L, H, G, P, N);
   TSSM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
                "gated_delta_rule_bwd: workspace of %lld bytes (16-byte aligned) needed, %lld given", (long long)need,
                (long long)workspace_bytes);
@@ -806,7 +817,7 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
   }
   TSSM_REQUIRE(Bt * L == 0 || (aligned16(states) && aligned16(errors)),
                "gated_delta_rule_bwd: states and errors must be 16-byte aligned");
-  const BwdSpace sp = space(Bt, L, H, G, P, N, dtype);
+  const BwdSpace sp = space(Bt, L, H, G, P, N);
   BwdArgs a{};
   a.u = u; a.B = B; a.C = C; a.dy = dy;
   a.A_log = (const float*)A_log; a.dt = (const float*)dt; a.beta = (const float*)beta;
@@ -821,13 +832,14 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
   const uintptr_t bases = reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(dy) |
                           reinterpret_cast<uintptr_t>(dh_last) | reinterpret_cast<uintptr_t>(dh0);
   a.gates = (Gates*)(a.da_part + sp.da);
-  a.img = sp.img && L > 0 && (bases & 15u) == 0 ? a.da_part + sp.da + sp.gates : nullptr;
+  a.img = (uint8_t*)(a.da_part + sp.da + sp.gates);
+  const bool tc = tc_takes(P, N, dtype) && (bases & 15u) == 0;
   a.Bt = Bt; a.L = L; a.H = (int)H; a.G = (int)G; a.P = (int)P; a.N = (int)N;
   a.nc = cdiv(L, delta::Q);
   a.scale = (float)scale;
   const int per = dtype == TSSM_F32 ? 4 : 8;
   a.vec_kq = N % per == 0 && aligned16(B) && aligned16(C);
   a.vec_v = P % per == 0 && aligned16(dy);
-  if (dtype == TSSM_F32) return N <= 64 ? launch_all<3, 64>(a, st) : launch_all<3, 128>(a, st);
-  return N <= 64 ? launch_all<1, 64>(a, st) : launch_all<1, 128>(a, st);
+  if (dtype == TSSM_F32) return N <= 64 ? launch_all<3, 64>(a, tc, st) : launch_all<3, 128>(a, tc, st);
+  return N <= 64 ? launch_all<1, 64>(a, tc, st) : launch_all<1, 128>(a, tc, st);
 }

@@ -8,8 +8,11 @@
 //     S^T  = exp(l_last) S^T + (E diag(w beta))^T K
 // Transposed, every product's result has the register layout of the next one's
 // left operand, so the chain needs no shared memory and no barrier; K, Q, T and
-// Aq are shared by the warps as right operands.  Four more warps load the next
-// chunk and build its A, T and Aq meanwhile (BUFS = 2), one barrier a chunk.
+// Aq are shared by the warps as right operands.  T and Aq come from delta_prep.cu;
+// four more warps load the next chunk meanwhile (bf16; f32 tiles fill the shared
+// memory, so there all warps load between chunks).  mma.sync gives a quarter of
+// tcgen05's rate here (1024 of 4096 multiply-adds a cycle and SM): this kernel is
+// for f32 and for shapes and addresses that delta_tc.cu does not take.
 #include "delta.cuh"
 #include "delta_tc.h"
 
@@ -26,18 +29,18 @@ struct FwdSmem {
   static constexpr int NAQ = XS == 1 ? 2 : 3;            // planes of Aq diag(beta)
   static constexpr int VROW = XS == 1 ? PB * 2 : (PB + 4) * 4;   // f32 values: padded rows
   static constexpr int K = 0, QQ = K + XS * PLANE, V = QQ + XS * PLANE, T = V + Q * VROW, AQ = T + 3 * SQ_BYTES,
-                       G = AQ + NAQ * SQ_BYTES, BUF = (G + (int)sizeof(Gates) + 127) / 128 * 128;
-  static constexpr int M = BUFS * BUF, BYTES = M + Q * AM * 4 + 128;
+                       G = AQ + NAQ * SQ_BYTES, BUF = (G + (int)sizeof(Gates) + 127) / 128 * 128;   // T, AQ, G: an image
+  static constexpr int BYTES = BUFS * BUF + 128;
 };
 
 struct FwdArgs {
   const void *u, *B, *C;
-  const float *A_log, *dt, *beta, *h0;
+  const uint8_t* img;
+  const float* h_in;
   void* y;
-  float *h_last, *states, *errs;
-  int64_t L;
+  float *h_out, *states, *errs;
+  int64_t L, c0, nseg, nc;   // first chunk and chunks of the segment; all chunks
   int H, G, P, N, npb;
-  int64_t nc;
   float scale;
   int vec_kq, vec_v;
 };
@@ -60,37 +63,35 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
   const T* vp = (const T*)a.u + (b * a.L) * su + (int64_t)h * a.P + pb;
   const int pvalid = min(PB, a.P - pb);
 
-  auto prep = [&](int64_t c) {   // 128 threads
-    const int t = threadIdx.x - NCW * 32;
+  // Chunk c of the segment to shared memory: by the four loading warps, or (one buffer) by all.
+  constexpr int LT = SM::BUFS == 2 ? 128 : (NCW + 4) * 32;
+  auto load = [&](int64_t c) {
+    const int t = threadIdx.x - (SM::BUFS == 2 ? NCW * 32 : 0);
     uint8_t* buf = smem + (SM::BUFS == 2 ? (int)(c & 1) * SM::BUF : 0);
     const uint32_t s = smem_addr(buf);
-    const int64_t t0 = c * Q;
+    const int64_t t0 = (a.c0 + c) * Q;
     const int rows = (int)min((int64_t)Q, a.L - t0);
-    load_planes<XS, KN, 128>(s + SM::K, SM::PLANE, kp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
-    load_planes<XS, KN, 128>(s + SM::QQ, SM::PLANE, qp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
+    load_image<SM::NAQ, LT>(s + SM::T, a.img + (bh * a.nseg + c) * img_bytes(SM::NAQ), t);
+    load_planes<XS, KN, LT>(s + SM::K, SM::PLANE, kp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
+    load_planes<XS, KN, LT>(s + SM::QQ, SM::PLANE, qp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
     if constexpr (XS == 1) {
-      load_planes<1, PB, 128>(s + SM::V, 0, vp + t0 * su, su, rows, pvalid, a.vec_v, t);
+      load_planes<1, PB, LT>(s + SM::V, 0, vp + t0 * su, su, rows, pvalid, a.vec_v, t);
     } else {
       float* vs = reinterpret_cast<float*>(buf + SM::V);
-      for (int i = t; i < Q * PB; i += 128) {
+#pragma unroll 4
+      for (int i = t; i < Q * PB; i += LT) {
         const int r = i / PB, p = i % PB;
         vs[r * (PB + 4) + p] = r < rows && p < pvalid ? ldf(vp + (t0 + r) * su + p) : 0.f;
       }
     }
-    Gates& gt = *reinterpret_cast<Gates*>(buf + SM::G);
-    if (t < 32)
-      gates_warp(gt, a.dt + b * a.L * a.H + h, a.beta + b * a.L * a.H + h, a.H, a.A_log[h], t0, a.L, t);
     cp_async_wait_all();
-    bar_sync(1, 128);
-    chunk_matrices<XS, KN, SM::NAQ, 3>(s + SM::K, s + SM::QQ, gt, a.scale, reinterpret_cast<float*>(smem + SM::M),
-                                       buf + SM::AQ, buf + SM::T, t, 1);
   };
 
   // ---- chain state
   const int p0 = 16 * warp;   // of the block's channels
   const int pr = lane / 4, q2 = 2 * (lane % 4);
   float S[NT][4];
-  const int64_t srow = (bh * a.P + pb + p0 + pr) * (int64_t)a.N;   // of h0, h_last
+  const int64_t srow = (bh * a.P + pb + p0 + pr) * (int64_t)a.N;   // of h_in, h_out
   auto state_io = [&](float* dst, const float* src) {
 #pragma unroll
     for (int j = 0; j < NT; ++j)
@@ -111,10 +112,10 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
     uint8_t* buf = smem + (SM::BUFS == 2 ? (int)(c & 1) * SM::BUF : 0);
     const uint32_t s = smem_addr(buf);
     const Gates& gt = *reinterpret_cast<const Gates*>(buf + SM::G);
-    const int64_t t0 = c * Q;
+    const int64_t t0 = (a.c0 + c) * Q;
     const int rows = (int)min((int64_t)Q, a.L - t0);
     if (a.states) {
-      float* dst = a.states + (bh * a.nc + c) * saved_floats(a.P, a.N);
+      float* dst = a.states + (bh * a.nc + a.c0 + c) * saved_floats(a.P, a.N);
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -298,24 +299,24 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
     }
   };
 
-  if (warp < NCW) state_io(nullptr, a.h0 ? a.h0 + srow : nullptr);
+  if (warp < NCW) state_io(nullptr, a.h_in ? a.h_in + srow : nullptr);
   if constexpr (SM::BUFS == 2) {
-    if (warp >= NCW && a.nc > 0) prep(0);
+    if (warp >= NCW) load(0);
     __syncthreads();
-    for (int64_t c = 0; c < a.nc; ++c) {
+    for (int64_t c = 0; c < a.nseg; ++c) {
       if (warp < NCW) chain(c);
-      else if (c + 1 < a.nc) prep(c + 1);
+      else if (c + 1 < a.nseg) load(c + 1);
       __syncthreads();
     }
   } else {
-    for (int64_t c = 0; c < a.nc; ++c) {
-      if (warp >= NCW) prep(c);
+    for (int64_t c = 0; c < a.nseg; ++c) {
+      load(c);
       __syncthreads();
       if (warp < NCW) chain(c);
       __syncthreads();
     }
   }
-  if (warp < NCW && a.h_last) state_io(a.h_last + srow, nullptr);
+  if (warp < NCW && a.h_out) state_io(a.h_out + srow, nullptr);
 }
 
 template <int XS, int KN, int NCW, int NS>
@@ -345,9 +346,12 @@ int by_block(const FwdArgs& a, int64_t Bt, cudaStream_t st) {
 
 extern "C" int64_t tssm_gated_delta_rule_workspace_size(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P,
                                                         int64_t N, int dtype) {
+  using namespace tssm;
   using namespace tssm::delta;
-  if (Bt <= 0 || L <= 0 || H <= 0 || G <= 0 || P <= 0 || !tc_takes(P, N, dtype)) return 0;
-  return tc_workspace(Bt, L, H, P, N);
+  if (Bt <= 0 || L <= 0 || H <= 0 || G <= 0 || P <= 0 || N <= 0) return 0;
+  const int na = dtype == TSSM_F32 ? 3 : 2;
+  const int64_t streams = Bt * H, nc = cdiv(L, delta::Q), seg = segment_chunks(streams, nc, na);
+  return streams * seg * prep_image_bytes(na) + (seg < nc ? streams * P * N * 4 : 0);
 }
 
 extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const void* B, const void* C, const void* dt,
@@ -376,23 +380,47 @@ extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const voi
   TSSM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
                "gated_delta_rule: workspace of %lld bytes (16-byte aligned) needed, %lld given", (long long)need,
                (long long)workspace_bytes);
-  if (need && (bases & 15u) == 0) {
+  const int na = dtype == TSSM_F32 ? 3 : 2;
+  const int64_t streams = Bt * H, nc = cdiv(L, delta::Q);
+  if (nc == 0) {   // no tokens: the state passes through
+    if (!h_last) return TSSM_OK;
+    const size_t bytes = (size_t)(streams * P * N) * 4;
+    if ((h0 ? cudaMemcpyAsync(h_last, h0, bytes, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(h_last, 0, bytes, st)) !=
+        cudaSuccess)
+      return check_launch("gated_delta_rule: pass the state");
+    return TSSM_OK;
+  }
+  const int64_t seg = segment_chunks(streams, nc, na);
+  uint8_t* img = (uint8_t*)workspace;
+  float* carry = h_last ? (float*)h_last : (float*)(img + streams * seg * prep_image_bytes(na));
+  if (tc_takes(P, N, dtype) && (bases & 15u) == 0) {
     const TcCall t{u, B, C, (const float*)A_log, (const float*)dt, (const float*)beta, (const float*)h0, y,
-                   (float*)h_last, (float*)states, (float*)errors, workspace, Bt, L, H, G, P, N, (float)scale};
+                   (float*)h_last, (float*)states, (float*)errors, img, carry, Bt, L, H, G, P, N, (float)scale};
     return tc_run(t, st);
   }
-  FwdArgs a{};
-  a.u = u; a.B = B; a.C = C;
-  a.A_log = (const float*)A_log; a.dt = (const float*)dt; a.beta = (const float*)beta; a.h0 = (const float*)h0;
-  a.y = y; a.h_last = (float*)h_last; a.states = (float*)states; a.errs = (float*)errors;
-  a.L = L; a.H = (int)H; a.G = (int)G; a.P = (int)P; a.N = (int)N;
-  a.nc = cdiv(L, delta::Q);
-  a.scale = (float)scale;
   const int per = dtype == TSSM_F32 ? 4 : 8;   // elements of 16 bytes
+  FwdArgs a{};
+  a.u = u; a.B = B; a.C = C; a.img = img;
+  a.y = y; a.states = (float*)states; a.errs = (float*)errors;
+  a.L = L; a.H = (int)H; a.G = (int)G; a.P = (int)P; a.N = (int)N;
+  a.nc = nc;
+  a.scale = (float)scale;
   a.vec_kq = N % per == 0 && aligned16(B) && aligned16(C);
   a.vec_v = P % per == 0 && aligned16(u) && aligned16(y);
-  if (dtype == TSSM_F32) return N <= 64 ? by_block<3, 64, 3>(a, Bt, st) : by_block<3, 128, 3>(a, Bt, st);
-  // f32 results (the state, what the backward reads) want three planes; y alone is bf16: two
-  if (h_last || states) return N <= 64 ? by_block<1, 64, 3>(a, Bt, st) : by_block<1, 128, 3>(a, Bt, st);
-  return N <= 64 ? by_block<1, 64, 2>(a, Bt, st) : by_block<1, 128, 2>(a, Bt, st);
+  for (int64_t c0 = 0; c0 < nc; c0 += seg) {
+    const int64_t m = std::min(seg, nc - c0);
+    const PrepCall p{B, C, (const float*)A_log, (const float*)dt, (const float*)beta, img, nullptr, Bt, L, H, G, N, c0,
+                     m, nc, (float)scale, a.vec_kq};
+    if (int e = prep_run(p, dtype, na, st)) return e;
+    a.c0 = c0; a.nseg = m;
+    a.h_in = c0 ? carry : (const float*)h0;
+    a.h_out = c0 + m == nc && !h_last ? nullptr : carry;
+    int e;
+    if (dtype == TSSM_F32) e = N <= 64 ? by_block<3, 64, 3>(a, Bt, st) : by_block<3, 128, 3>(a, Bt, st);
+    // f32 results (the state, what the backward reads) want three planes; y alone is bf16: two
+    else if (h_last || states) e = N <= 64 ? by_block<1, 64, 3>(a, Bt, st) : by_block<1, 128, 3>(a, Bt, st);
+    else e = N <= 64 ? by_block<1, 64, 2>(a, Bt, st) : by_block<1, 128, 2>(a, Bt, st);
+    if (e) return e;
+  }
+  return TSSM_OK;
 }

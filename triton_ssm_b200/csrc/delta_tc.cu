@@ -1,12 +1,7 @@
 // Chunked gated delta rule, forward, on tcgen05 (bf16, N = 64 or 128, P a
 // multiple of 64; formulas and precision: delta.cuh).
 //
-// Two kernels per segment of the sequence.  The chunk matrices T and
-// Aq diag(beta) depend on no state, so delta_prep_kernel builds them for every
-// (chunk, head) of the segment at once and leaves them in HBM as the shared-memory
-// images that the scan copies.  A segment's images take about IMAGE_BYTES and are
-// written and read while they are in L2.
-//
+// Per segment of the sequence delta_prep.cu makes the chunks' images, then
 // delta_scan_kernel: a block carries one (batch row, head) and 128 value channels,
 // transposed: TMEM lane = value channel p, so every step of the chain stays in its
 // thread.  Per chunk
@@ -35,6 +30,8 @@
 // goes on without waiting, storing nothing: the named barriers' counts stay whole.
 #include <cudaTypedefs.h>
 
+#include <cstddef>
+
 #include "delta.cuh"
 #include "delta_tc.h"
 #include "tcgen05.cuh"
@@ -46,57 +43,10 @@ namespace {
 using namespace sm100;
 
 constexpr int TILE = 8192;                       // [64 x 64] bf16
-// A chunk's image: T planes, NA planes of Aq diag(beta), exp(l) and w beta.
-constexpr int IMG_T = 0, IMG_AQ = 3 * SQ_BYTES;
-__host__ __device__ constexpr int img_gates(int na) { return IMG_AQ + na * SQ_BYTES; }
-__host__ __device__ constexpr int img_bytes(int na) { return img_gates(na) + 2 * Q * 4; }
-constexpr int IMG_G = img_gates(2), IMG = img_bytes(2);           // forward
-constexpr int IMG_G3 = img_gates(3), IMG3 = img_bytes(3);         // backward: f32 gradients want all of Aq
-constexpr int64_t IMAGE_BYTES = 256ll << 20;
-
-// ------------------------------------------------------------------ chunk images
-struct PrepArgs {
-  const __nv_bfloat16 *B, *C;
-  const float *A_log, *dt, *beta;
-  uint8_t* img;
-  Gates* gates;          // [Bt, H, nc] or null: for the gradient kernel
-  int64_t L, c0, nseg, nc;   // first chunk and chunks of the segment
-  int H, G, N;
-  float scale;
-};
-
-template <int KN>
-struct PrepSmem {
-  static constexpr int PLANE = Q * KN * 2;
-  static constexpr int MB = Q * AM * 4;   // the work matrix lies over the Q tile
-  static constexpr int K = 0, QQ = PLANE, M = QQ, G = QQ + (MB > PLANE ? MB : PLANE), BYTES = G + (int)sizeof(Gates) + 128;
-};
-
-template <int KN, int NA>
-__global__ void __launch_bounds__(128, 6) delta_prep_kernel(const PrepArgs a) {
-  using SM = PrepSmem<KN>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + ((128u - (smem_addr(smem_raw) & 127u)) & 127u);
-  const uint32_t s = smem_addr(smem);
-  const int t = threadIdx.x;
-  const int64_t bh = blockIdx.x / a.nseg, ci = blockIdx.x - bh * a.nseg, b = bh / a.H;
-  const int h = (int)(bh - b * a.H), g = h / (a.H / a.G);
-  const int64_t t0 = (a.c0 + ci) * Q, sk = (int64_t)a.G * a.N;
-  const int rows = (int)min((int64_t)Q, a.L - t0);
-  const int64_t at = (b * a.L + t0) * sk + (int64_t)g * a.N;
-  load_planes<1, KN, 128>(s + SM::K, 0, a.B + at, sk, rows, a.N, true, t);
-  load_planes<1, KN, 128>(s + SM::QQ, 0, a.C + at, sk, rows, a.N, true, t);
-  Gates& gt = *reinterpret_cast<Gates*>(smem + SM::G);
-  if (t < 32) gates_warp(gt, a.dt + b * a.L * a.H + h, a.beta + b * a.L * a.H + h, a.H, a.A_log[h], t0, a.L, t);
-  cp_async_wait_all();
-  __syncthreads();
-  uint8_t* img = a.img + (bh * a.nseg + ci) * img_bytes(NA);
-  float* go = reinterpret_cast<float*>(img + img_gates(NA));
-  go[t] = t < Q ? gt.eg[t] : gt.wb[t - Q];
-  if (a.gates) copy_gates(a.gates + bh * a.nc + a.c0 + ci, gt, t);
-  chunk_matrices<1, KN, NA, 3, true>(s + SM::K, s + SM::QQ, gt, a.scale, reinterpret_cast<float*>(smem + SM::M), img + IMG_AQ,
-                              img + IMG_T, t, 1);
-}
+constexpr int IMG = img_bytes(2), IMG_EG = img_gates(2) + (int)offsetof(Gates, eg);      // forward
+constexpr int IMG3 = img_bytes(3), IMG3_EG = img_gates(3) + (int)offsetof(Gates, eg);    // backward: all of Aq
+constexpr int EG_TO_WB = (int)(offsetof(Gates, wb) - offsetof(Gates, eg)) / 4;
+static_assert(IMG % 16 == 0 && IMG3 % 16 == 0 && IMG_EG % 16 == 0, "bulk copies, 16-byte reads");
 
 // ------------------------------------------------------------------ the scan
 struct ScanArgs {
@@ -301,8 +251,8 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       // X^T = V^T - exp(l) KS^T, 32 tokens of this half
       const uint8_t* st = stage(c);
       ok = ok && waitw(&full[c & 1], c >> 1, 2002);
-      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_G) + 32 * half;
-      const float* wb = eg + Q;
+      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_EG) + 32 * half;
+      const float* wb = eg + EG_TO_WB;
       const float el = (eg - 32 * half)[Q - 1];
       const uint16_t* vs = reinterpret_cast<const uint16_t*>(st + SM::V + (p >> 6) * TILE) + (p & 63) + half * 32 * 64;
       ok = ok && waitw(ksdone, c, 2003);
@@ -385,7 +335,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       const uint8_t* st = stage(c);
       // scale exp(l) QS^T goes back to its columns, where Aq diag(beta) E is added
       bool bad = !waitw(&full[c & 1], c >> 1, 2006) || !waitw(qdone, c, 2007);
-      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_G);
+      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_EG);
       if (!bad) {
 #pragma unroll 1
         for (int i = 0; i < Q; i += 16) {
@@ -674,8 +624,8 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
       const int64_t cc = a.c0 + n - 1 - k;
       const uint8_t* st = stage(k);
       ok = ok && waitw(&full[k & 1], k >> 1, 2102);
-      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_G3) + 32 * half;
-      const float* wb = eg + Q;
+      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG3_EG) + 32 * half;
+      const float* wb = eg + EG_TO_WB;
       const float el = (eg - 32 * half)[Q - 1];
       const uint16_t* os = reinterpret_cast<const uint16_t*>(st + SM::DO + (p >> 6) * TILE) + (p & 63) + half * 32 * 64;
       // dO^T, 32 tokens of this half
@@ -919,13 +869,9 @@ bool map_bf16(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int64_t segment_chunks(int64_t streams, int64_t nc, int img) {
-  return std::max<int64_t>(1, std::min(nc, IMAGE_BYTES / (streams * img)));
-}
-
 template <int KN, int NS>
 int run(const TcCall& a, cudaStream_t st) {
-  const int64_t streams = a.Bt * a.H, nc = cdiv(a.L, Q), seg = segment_chunks(streams, nc, IMG);
+  const int64_t streams = a.Bt * a.H, nc = cdiv(a.L, Q), seg = segment_chunks(streams, nc, 2);
   CUtensorMap mk, mq, mu, my;
   if (!map_bf16(&mk, a.B, a.G * a.N, a.L, a.Bt, true) || !map_bf16(&mq, a.C, a.G * a.N, a.L, a.Bt, true) ||
       !map_bf16(&mu, a.u, a.H * a.P, a.L, a.Bt, false) || !map_bf16(&my, a.y, a.H * a.P, a.L, a.Bt, false)) {
@@ -937,21 +883,16 @@ int run(const TcCall& a, cudaStream_t st) {
     set_error("gated_delta_rule: device status word unavailable");
     return TSSM_ERR_CUDA;
   }
-  auto prep = delta_prep_kernel<KN, 2>;
   auto scan = delta_scan_kernel<KN, NS>;
-  if (cudaFuncSetAttribute(prep, cudaFuncAttributeMaxDynamicSharedMemorySize, PrepSmem<KN>::BYTES) != cudaSuccess ||
-      cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem<KN>::BYTES) != cudaSuccess)
+  if (cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem<KN>::BYTES) != cudaSuccess)
     return check_launch("gated_delta_rule: set smem attribute");
-  uint8_t* img = (uint8_t*)a.ws;
-  float* carry = a.h_last ? a.h_last : (float*)(img + streams * seg * IMG);
   for (int64_t c0 = 0; c0 < nc; c0 += seg) {
     const int64_t m = std::min(seg, nc - c0);
-    const PrepArgs p{(const __nv_bfloat16*)a.B, (const __nv_bfloat16*)a.C, a.A_log, a.dt, a.beta, img, nullptr, a.L, c0, m,
-                     nc, (int)a.H, (int)a.G, (int)a.N, a.scale};
-    prep<<<(unsigned)(streams * m), 128, PrepSmem<KN>::BYTES, st>>>(p);
+    const PrepCall p{a.B, a.C, a.A_log, a.dt, a.beta, a.img, nullptr, a.Bt, a.L, a.H, a.G, a.N, c0, m, nc, a.scale, 1};
+    if (int e = prep_run(p, TSSM_BF16, 2, st)) return e;
     const bool last = c0 + m == nc;
-    const ScanArgs s{img, c0 ? carry : a.h0, last && !a.h_last ? nullptr : carry, a.states, a.errs, status, a.L, c0, m,
-                     nc, (int)a.H, (int)a.G, (int)a.P, (int)a.N, (int)cdiv(a.P, 128), a.scale};
+    const ScanArgs s{a.img, c0 ? a.carry : a.h0, last && !a.h_last ? nullptr : a.carry, a.states, a.errs, status, a.L,
+                     c0, m, nc, (int)a.H, (int)a.G, (int)a.P, (int)a.N, (int)cdiv(a.P, 128), a.scale};
     scan<<<(unsigned)(streams * s.npb), 512, ScanSmem<KN>::BYTES, st>>>(mk, mq, mu, my, s);
   }
   return check_launch("gated_delta_rule");
@@ -959,7 +900,7 @@ int run(const TcCall& a, cudaStream_t st) {
 
 template <int KN>
 int run_back(const TcBackCall& a, cudaStream_t st) {
-  const int64_t streams = a.Bt * a.H, nc = cdiv(a.L, Q), seg = segment_chunks(streams, nc, IMG3);
+  const int64_t streams = a.Bt * a.H, nc = cdiv(a.L, Q), seg = segment_chunks(streams, nc, 3);
   CUtensorMap mk, mq, mo;
   if (!map_bf16(&mk, a.B, a.G * a.N, a.L, a.Bt, true) || !map_bf16(&mq, a.C, a.G * a.N, a.L, a.Bt, true) ||
       !map_bf16(&mo, a.dy, a.H * a.P, a.L, a.Bt, false)) {
@@ -971,18 +912,14 @@ int run_back(const TcBackCall& a, cudaStream_t st) {
     set_error("gated_delta_rule_bwd: device status word unavailable");
     return TSSM_ERR_CUDA;
   }
-  auto prep = delta_prep_kernel<KN, 3>;
   auto scan = delta_back_scan_kernel<KN>;
-  if (cudaFuncSetAttribute(prep, cudaFuncAttributeMaxDynamicSharedMemorySize, PrepSmem<KN>::BYTES) != cudaSuccess ||
-      cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, BackSmem<KN>::BYTES) != cudaSuccess)
+  if (cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, BackSmem<KN>::BYTES) != cudaSuccess)
     return check_launch("gated_delta_rule_bwd: set smem attribute");
-  uint8_t* img = (uint8_t*)a.ws;
   for (int64_t end = nc; end > 0; end -= seg) {   // segments from the last; dh0 carries the state's gradient
     const int64_t c0 = std::max<int64_t>(0, end - seg), m = end - c0;
-    const PrepArgs p{(const __nv_bfloat16*)a.B, (const __nv_bfloat16*)a.C, a.A_log, a.dt, a.beta, img, (Gates*)a.gates, a.L, c0, m,
-                     nc, (int)a.H, (int)a.G, (int)a.N, a.scale};
-    prep<<<(unsigned)(streams * m), 128, PrepSmem<KN>::BYTES, st>>>(p);
-    const BackArgs s{img, end == nc ? a.dh_last : a.dh0, a.dh0, a.dstates, a.derrs, (__nv_bfloat16*)a.du, status, a.L,
+    const PrepCall p{a.B, a.C, a.A_log, a.dt, a.beta, a.img, a.gates, a.Bt, a.L, a.H, a.G, a.N, c0, m, nc, a.scale, 1};
+    if (int e = prep_run(p, TSSM_BF16, 3, st)) return e;
+    const BackArgs s{a.img, end == nc ? a.dh_last : a.dh0, a.dh0, a.dstates, a.derrs, (__nv_bfloat16*)a.du, status, a.L,
                      c0, m, nc, (int)a.H, (int)a.G, (int)a.P, (int)a.N, (int)cdiv(a.P, 128), a.scale};
     scan<<<(unsigned)(streams * s.npb), 384, BackSmem<KN>::BYTES, st>>>(mk, mq, mo, s);
   }
@@ -995,25 +932,14 @@ bool tc_takes(int64_t P, int64_t N, int dtype) {
   return dtype == TSSM_BF16 && (N == 64 || N == 128) && P % 64 == 0;
 }
 
-int64_t tc_workspace(int64_t Bt, int64_t L, int64_t H, int64_t P, int64_t N) {
-  const int64_t streams = Bt * H, nc = cdiv(L, Q), seg = segment_chunks(streams, nc, IMG);
-  return streams * seg * IMG + (seg < nc ? streams * P * N * 4 : 0);
-}
-
-int64_t tc_back_workspace(int64_t Bt, int64_t L, int64_t H) {
-  return Bt * H * segment_chunks(Bt * H, cdiv(L, Q), IMG3) * IMG3;
-}
-
 int tc_back_run(const TcBackCall& a, cudaStream_t st) {
-  TSSM_REQUIRE(a.Bt * a.H * std::max(cdiv(a.P, 128), segment_chunks(a.Bt * a.H, cdiv(a.L, Q), IMG3)) < (int64_t(1) << 31) &&
-                   a.H * a.P < (int64_t(1) << 31) && a.G * a.N < (int64_t(1) << 31),
+  TSSM_REQUIRE(a.Bt * a.H * cdiv(a.P, 128) < (int64_t(1) << 31) && a.H * a.P < (int64_t(1) << 31) && a.G * a.N < (int64_t(1) << 31),
                "gated_delta_rule_bwd: size out of range");
   return a.N == 64 ? run_back<64>(a, st) : run_back<128>(a, st);
 }
 
 int tc_run(const TcCall& a, cudaStream_t st) {
-  TSSM_REQUIRE(a.Bt * a.H * std::max(cdiv(a.P, 128), segment_chunks(a.Bt * a.H, cdiv(a.L, Q), IMG)) < (int64_t(1) << 31) &&
-                   a.H * a.P < (int64_t(1) << 31) && a.G * a.N < (int64_t(1) << 31),
+  TSSM_REQUIRE(a.Bt * a.H * cdiv(a.P, 128) < (int64_t(1) << 31) && a.H * a.P < (int64_t(1) << 31) && a.G * a.N < (int64_t(1) << 31),
                "gated_delta_rule: size out of range");
   const bool f32_out = a.h_last || a.states;
   if (a.N == 64) return f32_out ? run<64, 3>(a, st) : run<64, 2>(a, st);

@@ -1,4 +1,4 @@
-// The tcgen05 form of the chunked gated delta rule (delta_tc.cu), as the entry point calls it.
+// Host-side calls between the files of the chunked gated delta rule.
 #pragma once
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -6,29 +6,44 @@
 namespace tssm {
 namespace delta {
 
+// delta_prep.cu: the images of `chunks` chunks from c0 of every (batch row, head).
+struct PrepCall {
+  const void *B, *C;
+  const float *A_log, *dt, *beta;
+  uint8_t* img;
+  void* gates;   // [Bt, H, nc] gates as well, or null
+  int64_t Bt, L, H, G, N, c0, chunks, nc;
+  float scale;
+  int vec;       // N and the bases allow 16-byte pieces
+};
+int prep_run(const PrepCall& a, int dtype, int na, cudaStream_t st);   // na planes of Aq: 2 (bf16 y) or 3 (f32)
+int64_t prep_image_bytes(int na);
+int64_t prep_gates_bytes();
+int64_t segment_chunks(int64_t streams, int64_t nc, int na);   // chunks whose images are made at a time
+
+// delta_tc.cu: the scans on tcgen05 (bf16, N 64 or 128, P a multiple of 64, 16-byte aligned tensors).
 struct TcCall {
   const void *u, *B, *C;
   const float *A_log, *dt, *beta, *h0;
   void* y;
   float *h_last, *states, *errs;
-  void* ws;
+  uint8_t* img;
+  float* carry;   // the state between segments
   int64_t Bt, L, H, G, P, N;
   float scale;
 };
-struct TcBackCall {   // the backward's chain: dE, du, dS1 of every chunk, dh0
+struct TcBackCall {   // the backward's chain: dE, du, dS1 and gates of every chunk, dh0
   const void *B, *C, *dy;
   const float *A_log, *dt, *beta, *dh_last;
   void* du;
   float *dh0, *dstates, *derrs;
-  void* gates;   // one per (batch row, head, chunk)
-  void* ws;
+  void* gates;
+  uint8_t* img;
   int64_t Bt, L, H, G, P, N;
   float scale;
 };
-bool tc_takes(int64_t P, int64_t N, int dtype);   // shapes; the tensors must be 16-byte aligned as well
-int64_t tc_workspace(int64_t Bt, int64_t L, int64_t H, int64_t P, int64_t N);
+bool tc_takes(int64_t P, int64_t N, int dtype);
 int tc_run(const TcCall& a, cudaStream_t st);
-int64_t tc_back_workspace(int64_t Bt, int64_t L, int64_t H);
 int tc_back_run(const TcBackCall& a, cudaStream_t st);
 
 }  // namespace delta
