@@ -230,7 +230,7 @@ __device__ __forceinline__ void load_planes(uint32_t dst, int plane_bytes, const
       return;
     }
   }
-#pragma unroll 1
+#pragma unroll 2
   for (int i = t; i < Q * PIECES; i += NTH) {
     const int r = i / PIECES, c = i % PIECES;
     const uint32_t off = tile_off<RB>(r, c);

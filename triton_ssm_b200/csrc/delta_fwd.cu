@@ -78,10 +78,19 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
       load_planes<1, PB, LT>(s + SM::V, 0, vp + t0 * su, su, rows, pvalid, a.vec_v, t);
     } else {
       float* vs = reinterpret_cast<float*>(buf + SM::V);
+      if (a.vec_v) {
 #pragma unroll 4
-      for (int i = t; i < Q * PB; i += LT) {
-        const int r = i / PB, p = i % PB;
-        vs[r * (PB + 4) + p] = r < rows && p < pvalid ? ldf(vp + (t0 + r) * su + p) : 0.f;
+        for (int i = t; i < Q * PB / 4; i += LT) {
+          const int r = i / (PB / 4), p = i % (PB / 4) * 4;
+          const bool in = r < rows && p < pvalid;
+          cp_async16(s + SM::V + (r * (PB + 4) + p) * 4, in ? vp + (t0 + r) * su + p : vp, in);
+        }
+      } else {
+#pragma unroll 4
+        for (int i = t; i < Q * PB; i += LT) {
+          const int r = i / PB, p = i % PB;
+          vs[r * (PB + 4) + p] = r < rows && p < pvalid ? ldf(vp + (t0 + r) * su + p) : 0.f;
+        }
       }
     }
     cp_async_wait_all();
