@@ -54,6 +54,8 @@ struct ChainSmem {
 
 template <int XS, int KN, int NCW>
 __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(const BwdArgs a) {
+  let_next_start();
+  wait_for_previous();
   using T = typename std::conditional<XS == 1, __nv_bfloat16, float>::type;
   using SM = ChainSmem<XS, KN, NCW>;
   constexpr int PB = SM::PB, RB = KN * 2, NT = KN / 8, NS = 3, RV = PB * 2;
@@ -302,6 +304,8 @@ __device__ __forceinline__ void put4x2(uint8_t* tile, int r, int lane, const flo
 
 template <int XS, int KN>
 __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) {
+  let_next_start();
+  wait_for_previous();
   using T = typename std::conditional<XS == 1, __nv_bfloat16, float>::type;
   using SM = GradSmem<XS, KN>;
   constexpr int RB = KN * 2, NTQ = KN / 32;   // 8-wide tiles of a warp's quarter of N
@@ -668,6 +672,8 @@ template <typename T>
 __global__ void __launch_bounds__(256) delta_head_sum_kernel(const float* __restrict__ pk, const float* __restrict__ pq,
                                                              T* __restrict__ dB, T* __restrict__ dC, int64_t n, int G,
                                                              int rep, int N) {
+  let_next_start();
+  wait_for_previous();
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   const int64_t row = i / N;   // (token, key head)
@@ -685,6 +691,8 @@ __global__ void __launch_bounds__(256) delta_head_sum_kernel(const float* __rest
 // (the terms are of either sign).
 __global__ void __launch_bounds__(256) delta_da_kernel(const float* __restrict__ part, float* __restrict__ out,
                                                        int64_t Bt, int H, int64_t nc) {
+  let_next_start();
+  wait_for_previous();
   __shared__ double sm[256];
   double v = 0.0;
   for (int64_t i = threadIdx.x; i < Bt * nc; i += 256) {
@@ -710,7 +718,7 @@ int launch_chain(BwdArgs a, cudaStream_t st) {
     return check_launch("gated_delta_rule_bwd: set smem attribute");
   a.npb = (int)cdiv(a.P, 16 * NCW);
   TSSM_REQUIRE(a.Bt * a.H * a.npb < (int64_t(1) << 31), "gated_delta_rule_bwd: size out of range");
-  kern<<<(unsigned)(a.Bt * a.H * a.npb), (NCW + 4) * 32, bytes, st>>>(a);
+  launch_after(kern, dim3((unsigned)(a.Bt * a.H * a.npb)), (NCW + 4) * 32, bytes, st, a);
   return check_launch("gated_delta_rule_bwd: chain");
 }
 
@@ -734,7 +742,7 @@ int launch_all(BwdArgs a, bool tc, cudaStream_t st) {
       a.nseg = end - a.c0;
       a.ds_in = end == a.nc ? a.dh_last : a.dh0;
       const PrepCall p{a.B, a.C, a.A_log, a.dt, a.beta, a.img, a.gates, a.Bt, a.L, a.H, a.G, a.N, a.c0, a.nseg, a.nc,
-                       a.scale, a.vec_kq};
+                       a.scale, a.vec_kq, end < a.nc};
       if (int e = prep_run(p, XS == 1 ? TSSM_BF16 : TSSM_F32, 3, st)) return e;
       if (int e = wide ? launch_chain<XS, KN, 8>(a, st) : launch_chain<XS, KN, 4>(a, st)) return e;
     }
@@ -746,15 +754,15 @@ int launch_all(BwdArgs a, bool tc, cudaStream_t st) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
       return check_launch("gated_delta_rule_bwd: set smem attribute");
     TSSM_REQUIRE(a.Bt * a.H * a.nc < (int64_t(1) << 31), "gated_delta_rule_bwd: size out of range");
-    kern<<<(unsigned)(a.Bt * a.H * a.nc), GT, bytes, st>>>(a);
+    launch_after(kern, dim3((unsigned)(a.Bt * a.H * a.nc)), GT, bytes, st, a);
     if (a.dk_part) {
       const int64_t n = a.Bt * a.L * a.G * a.N;
       TSSM_REQUIRE(cdiv(n, 256) < (int64_t(1) << 31), "gated_delta_rule_bwd: size out of range");
-      delta_head_sum_kernel<T><<<(unsigned)cdiv(n, 256), 256, 0, st>>>(a.dk_part, a.dq_part, (T*)a.dB, (T*)a.dC, n,
-                                                                       a.G, a.H / a.G, a.N);
+      launch_after(delta_head_sum_kernel<T>, dim3((unsigned)cdiv(n, 256)), 256, 0, st, (const float*)a.dk_part,
+                   (const float*)a.dq_part, (T*)a.dB, (T*)a.dC, n, a.G, a.H / a.G, a.N);
     }
   }
-  delta_da_kernel<<<(unsigned)a.H, 256, 0, st>>>(a.da_part, a.dA_log, a.Bt, a.H, a.nc);
+  launch_after(delta_da_kernel, dim3((unsigned)a.H), 256, 0, st, (const float*)a.da_part, a.dA_log, a.Bt, a.H, a.nc);
   return check_launch("gated_delta_rule_bwd");
 }
 

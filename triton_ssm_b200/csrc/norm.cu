@@ -303,6 +303,8 @@ __global__ void __launch_bounds__(NT, NV == 1 ? 3 : NV == 2 ? 2 : 1) gn_token_bw
                                                           const float* __restrict__ rstd_i, T* __restrict__ dx,
                                                           float* __restrict__ part, int64_t rows, int groups, int Cg,
                                                           TokenGeom ge) {
+  let_next_start();
+  wait_for_previous();
   const int slot = threadIdx.x / ge.tl, lane = threadIdx.x % ge.tl;
   const int g = blockIdx.y * ge.gpb + slot % ge.gpb, rr = slot / ge.gpb;
   const bool live = rr < ge.rpb && g < groups;
@@ -392,6 +394,8 @@ __global__ void __launch_bounds__(NT, NV == 1 ? 3 : NV == 2 ? 2 : 1) gn_token_bw
 // out0[c] = sum_p part[0][p][c], out1[c] = sum_p part[1][p][c], in a fixed order.
 __global__ void __launch_bounds__(NT) gn_column_sum_kernel(const float* __restrict__ part, float* __restrict__ out0,
                                                            float* __restrict__ out1, int64_t parts, int64_t C) {
+  let_next_start();
+  wait_for_previous();
   __shared__ float sm[8][33];
   const int64_t c = (int64_t)blockIdx.x * 32 + threadIdx.x % 32;
   const int ty = threadIdx.x / 32;
@@ -436,6 +440,8 @@ __device__ __forceinline__ void chan(float& n, float& m, float& q, float n2, flo
 template <typename T, int V>
 __global__ void __launch_bounds__(NT, 4) gn_stats_kernel(const T* __restrict__ x, float2* __restrict__ st, int64_t L,
                                                       int64_t C, MapGeom ge) {
+  let_next_start();
+  wait_for_previous();
   __shared__ float sn[NT], sm[NT], sq[NT];
   const int tx = threadIdx.x % ge.cols, ty = threadIdx.x / ge.cols;
   const int64_t cv = (int64_t)blockIdx.y * ge.cols + tx, ncv = C / V;
@@ -501,6 +507,8 @@ __device__ __forceinline__ float block_sum(float v, float* sm) {   // every thre
 __global__ void __launch_bounds__(NT) gn_merge_kernel(const float2* __restrict__ st, float* __restrict__ mean_o,
                                                       float* __restrict__ rstd_o, int64_t L, int64_t ncv, int per,
                                                       int V, int groups, int64_t chunk, int64_t nchunks, float eps) {
+  let_next_start();
+  wait_for_previous();
   __shared__ float sm[NT / 32];
   const int64_t b = blockIdx.y;
   const int g = blockIdx.x;
@@ -533,6 +541,8 @@ __global__ void __launch_bounds__(NT, 4) gn_apply_kernel(const T* __restrict__ x
                                                       const float* __restrict__ b, const float* __restrict__ mean,
                                                       const float* __restrict__ rstd, T* __restrict__ y, int64_t L,
                                                       int64_t C, int groups, int Cg, MapGeom ge) {
+  let_next_start();
+  wait_for_previous();
   const int tx = threadIdx.x % ge.cols, ty = threadIdx.x / ge.cols;
   const int64_t cv = (int64_t)blockIdx.y * ge.cols + tx;
   if (ty >= ge.rows_y || cv >= C / V) return;
@@ -583,6 +593,8 @@ __global__ void __launch_bounds__(NT, 2) gn_bwd_sums_kernel(const T* __restrict_
                                                          const float* __restrict__ mean,
                                                          const float* __restrict__ rstd, float* __restrict__ part,
                                                          int64_t L, int64_t C, int groups, int Cg, MapGeom ge) {
+  let_next_start();
+  wait_for_previous();
   __shared__ float s0[NT][V], s1[NT][V];
   const int tx = threadIdx.x % ge.cols, ty = threadIdx.x / ge.cols;
   const int64_t cv = (int64_t)blockIdx.y * ge.cols + tx, c = cv * V, bz = blockIdx.z;
@@ -659,6 +671,8 @@ __global__ void __launch_bounds__(1024) gn_bwd_merge_kernel(const float* __restr
                                                             float* __restrict__ chan_sum, float2* __restrict__ gm,
                                                             int64_t L, int64_t C, int groups, int Cg, int64_t nchunks,
                                                             int64_t Bt, int64_t b0) {
+  let_next_start();
+  wait_for_previous();
   __shared__ float sa[32][33], sb[32][33];
   const int64_t b = blockIdx.y;
   const int g = blockIdx.x, tx = threadIdx.x % 32, ty = threadIdx.x / 32;
@@ -710,6 +724,8 @@ __global__ void __launch_bounds__(NT, 2) gn_bwd_apply_kernel(const T* __restrict
                                                           const float* __restrict__ rstd,
                                                           const float2* __restrict__ gm, T* __restrict__ dx,
                                                           int64_t L, int64_t C, int groups, int Cg, MapGeom ge) {
+  let_next_start();
+  wait_for_previous();
   const int tx = threadIdx.x % ge.cols, ty = threadIdx.x / ge.cols;
   const int64_t cv = (int64_t)blockIdx.y * ge.cols + tx;
   if (ty >= ge.rows_y || cv >= C / V) return;
@@ -846,8 +862,8 @@ void token_bwd(const Norm& a, const TokenGeom& ge, int nv) {
   if (nv == 1) go(gn_token_bwd_kernel<T, V, 1, SILU>);
   else if (nv == 2) go(gn_token_bwd_kernel<T, V, 2, SILU>);
   else go(gn_token_bwd_kernel<T, V, 4, SILU>);
-  gn_column_sum_kernel<<<dim3((unsigned)cdiv(a.C, 32), 2), NT, 0, a.st>>>((const float*)a.ws, (float*)a.dw,
-                                                                         (float*)a.db, (int64_t)grid.x * ge.rpb, a.C);
+  launch_after(gn_column_sum_kernel, dim3((unsigned)cdiv(a.C, 32), 2), NT, 0, a.st, (const float*)a.ws, (float*)a.dw,
+               (float*)a.db, (int64_t)grid.x * ge.rpb, a.C);
 }
 
 template <typename T, int V, bool SILU>
@@ -860,11 +876,12 @@ void map_fwd(const Norm& a) {
     dim3 grid((unsigned)ge.nchunks, (unsigned)ge.cblocks, (unsigned)nb);
     const T* x = (const T*)a.x + b0 * row;
     float *mean = (float*)a.mean + b0 * a.groups, *rstd = (float*)a.rstd + b0 * a.groups;
-    gn_stats_kernel<T, V><<<grid, NT, 0, a.st>>>(x, st, a.L, a.C, ge);
-    gn_merge_kernel<<<dim3((unsigned)a.groups, (unsigned)nb), NT, 0, a.st>>>(
-        st, mean, rstd, a.L, a.C / V, a.Cg / V, V, a.groups, ge.chunk, ge.nchunks, a.eps);
-    gn_apply_kernel<T, V, SILU><<<grid, NT, 0, a.st>>>(x, (const float*)a.w, (const float*)a.b, mean, rstd,
-                                                       (T*)a.y + b0 * row, a.L, a.C, a.groups, a.Cg, ge);
+    if (b0) launch_after(gn_stats_kernel<T, V>, grid, NT, 0, a.st, x, st, a.L, a.C, ge);
+    else gn_stats_kernel<T, V><<<grid, NT, 0, a.st>>>(x, st, a.L, a.C, ge);
+    launch_after(gn_merge_kernel, dim3((unsigned)a.groups, (unsigned)nb), NT, 0, a.st, (const float2*)st, mean, rstd,
+                 a.L, a.C / V, a.Cg / V, V, a.groups, ge.chunk, ge.nchunks, a.eps);
+    launch_after(gn_apply_kernel<T, V, SILU>, grid, NT, 0, a.st, x, (const float*)a.w, (const float*)a.b,
+                 (const float*)mean, (const float*)rstd, (T*)a.y + b0 * row, a.L, a.C, a.groups, a.Cg, ge);
   }
 }
 
@@ -880,15 +897,19 @@ void map_bwd(const Norm& a) {
     dim3 grid((unsigned)ge.nchunks, (unsigned)ge.cblocks, (unsigned)nb);
     const T *x = (const T*)a.x + b0 * row, *dy = (const T*)a.dy + b0 * row;
     const float *mean = (const float*)a.mean + b0 * a.groups, *rstd = (const float*)a.rstd + b0 * a.groups;
-    gn_bwd_sums_kernel<T, V, SILU><<<grid, NT, 0, a.st>>>(dy, x, (const float*)a.w, (const float*)a.b, mean, rstd,
-                                                          part, a.L, a.C, a.groups, a.Cg, ge);
-    gn_bwd_merge_kernel<<<dim3((unsigned)a.groups, (unsigned)nb), 1024, 0, a.st>>>(
-        part, (const float*)a.w, chan_sum, gm, a.L, a.C, a.groups, a.Cg, ge.nchunks, a.Bt, b0);
-    gn_bwd_apply_kernel<T, V, SILU><<<grid, NT, 0, a.st>>>(dy, x, (const float*)a.w, (const float*)a.b, mean, rstd,
-                                                           gm, (T*)a.y + b0 * row, a.L, a.C, a.groups, a.Cg, ge);
+    if (b0)
+      launch_after(gn_bwd_sums_kernel<T, V, SILU>, grid, NT, 0, a.st, dy, x, (const float*)a.w, (const float*)a.b, mean,
+                   rstd, part, a.L, a.C, a.groups, a.Cg, ge);
+    else
+      gn_bwd_sums_kernel<T, V, SILU><<<grid, NT, 0, a.st>>>(dy, x, (const float*)a.w, (const float*)a.b, mean, rstd,
+                                                            part, a.L, a.C, a.groups, a.Cg, ge);
+    launch_after(gn_bwd_merge_kernel, dim3((unsigned)a.groups, (unsigned)nb), 1024, 0, a.st, (const float*)part,
+                 (const float*)a.w, chan_sum, gm, a.L, a.C, a.groups, a.Cg, ge.nchunks, a.Bt, b0);
+    launch_after(gn_bwd_apply_kernel<T, V, SILU>, grid, NT, 0, a.st, dy, x, (const float*)a.w, (const float*)a.b, mean,
+                 rstd, (const float2*)gm, (T*)a.y + b0 * row, a.L, a.C, a.groups, a.Cg, ge);
   }
-  gn_column_sum_kernel<<<dim3((unsigned)cdiv(a.C, 32), 2), NT, 0, a.st>>>(chan_sum, (float*)a.dw, (float*)a.db, a.Bt,
-                                                                         a.C);
+  launch_after(gn_column_sum_kernel, dim3((unsigned)cdiv(a.C, 32), 2), NT, 0, a.st, (const float*)chan_sum,
+               (float*)a.dw, (float*)a.db, a.Bt, a.C);
 }
 
 template <typename T, int V, bool SILU>
