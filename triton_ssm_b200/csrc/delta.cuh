@@ -23,6 +23,14 @@ namespace delta {
 constexpr int Q = 64;   // tokens per chunk
 constexpr float LOG2E = 1.4426950408889634f;
 
+// A dependent kernel of a call: started early when it is small (its latency counts then);
+// larger grids gained nothing from it and lost 2 % behind the scans.
+template <typename... P, typename... A>
+inline void launch_next(void (*kern)(P...), unsigned blocks, int threads, size_t smem, cudaStream_t st, A&&... args) {
+  if ((int)blocks <= num_sms()) launch_after(kern, dim3(blocks), dim3(threads), smem, st, static_cast<A&&>(args)...);
+  else kern<<<blocks, threads, smem, st>>>(static_cast<P>(args)...);
+}
+
 // ------------------------------------------------------------------ tensor-core fragments
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

@@ -718,7 +718,7 @@ int launch_chain(BwdArgs a, cudaStream_t st) {
     return check_launch("gated_delta_rule_bwd: set smem attribute");
   a.npb = (int)cdiv(a.P, 16 * NCW);
   TSSM_REQUIRE(a.Bt * a.H * a.npb < (int64_t(1) << 31), "gated_delta_rule_bwd: size out of range");
-  launch_after(kern, dim3((unsigned)(a.Bt * a.H * a.npb)), (NCW + 4) * 32, bytes, st, a);
+  launch_next(kern, (unsigned)(a.Bt * a.H * a.npb), (NCW + 4) * 32, bytes, st, a);
   return check_launch("gated_delta_rule_bwd: chain");
 }
 
@@ -742,7 +742,7 @@ int launch_all(BwdArgs a, bool tc, cudaStream_t st) {
       a.nseg = end - a.c0;
       a.ds_in = end == a.nc ? a.dh_last : a.dh0;
       const PrepCall p{a.B, a.C, a.A_log, a.dt, a.beta, a.img, a.gates, a.Bt, a.L, a.H, a.G, a.N, a.c0, a.nseg, a.nc,
-                       a.scale, a.vec_kq, end < a.nc};
+                       a.scale, a.vec_kq};
       if (int e = prep_run(p, XS == 1 ? TSSM_BF16 : TSSM_F32, 3, st)) return e;
       if (int e = wide ? launch_chain<XS, KN, 8>(a, st) : launch_chain<XS, KN, 4>(a, st)) return e;
     }
@@ -754,15 +754,15 @@ int launch_all(BwdArgs a, bool tc, cudaStream_t st) {
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
       return check_launch("gated_delta_rule_bwd: set smem attribute");
     TSSM_REQUIRE(a.Bt * a.H * a.nc < (int64_t(1) << 31), "gated_delta_rule_bwd: size out of range");
-    launch_after(kern, dim3((unsigned)(a.Bt * a.H * a.nc)), GT, bytes, st, a);
+    launch_next(kern, (unsigned)(a.Bt * a.H * a.nc), GT, bytes, st, a);
     if (a.dk_part) {
       const int64_t n = a.Bt * a.L * a.G * a.N;
       TSSM_REQUIRE(cdiv(n, 256) < (int64_t(1) << 31), "gated_delta_rule_bwd: size out of range");
-      launch_after(delta_head_sum_kernel<T>, dim3((unsigned)cdiv(n, 256)), 256, 0, st, (const float*)a.dk_part,
+      launch_next(delta_head_sum_kernel<T>, (unsigned)cdiv(n, 256), 256, 0, st, (const float*)a.dk_part,
                    (const float*)a.dq_part, (T*)a.dB, (T*)a.dC, n, a.G, a.H / a.G, a.N);
     }
   }
-  launch_after(delta_da_kernel, dim3((unsigned)a.H), 256, 0, st, (const float*)a.da_part, a.dA_log, a.Bt, a.H, a.nc);
+  launch_next(delta_da_kernel, (unsigned)a.H, 256, 0, st, (const float*)a.da_part, a.dA_log, a.Bt, a.H, a.nc);
   return check_launch("gated_delta_rule_bwd");
 }
 

@@ -340,7 +340,7 @@ int launch(FwdArgs a, int64_t Bt, cudaStream_t st) {
   a.npb = (int)cdiv(a.P, 16 * NCW);
   const int64_t blocks = Bt * a.H * a.npb;
   TSSM_REQUIRE(blocks < (int64_t(1) << 31), "gated_delta_rule: size out of range");
-  launch_after(kern, dim3((unsigned)blocks), (NCW + 4) * 32, bytes, st, a);
+  launch_next(kern, (unsigned)blocks, (NCW + 4) * 32, bytes, st, a);
   return check_launch("gated_delta_rule");
 }
 
@@ -421,7 +421,7 @@ extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const voi
   for (int64_t c0 = 0; c0 < nc; c0 += seg) {
     const int64_t m = std::min(seg, nc - c0);
     const PrepCall p{B, C, (const float*)A_log, (const float*)dt, (const float*)beta, img, nullptr, Bt, L, H, G, N, c0,
-                     m, nc, (float)scale, a.vec_kq, c0 > 0};
+                     m, nc, (float)scale, a.vec_kq};
     if (int e = prep_run(p, dtype, na, st)) return e;
     a.c0 = c0; a.nseg = m;
     a.h_in = c0 ? carry : (const float*)h0;

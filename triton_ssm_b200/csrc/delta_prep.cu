@@ -23,7 +23,6 @@ struct PrepSmem {
 template <int XS, int KN, int NA>
 __global__ void __launch_bounds__(128, XS == 1 ? 6 : 2) delta_prep_kernel(const PrepCall a) {
   let_next_start();
-  wait_for_previous();
   using T = typename std::conditional<XS == 1, __nv_bfloat16, float>::type;
   using SM = PrepSmem<XS, KN>;
   extern __shared__ uint8_t smem_raw[];
@@ -54,9 +53,7 @@ int launch(const PrepCall& a, cudaStream_t st) {
   constexpr int bytes = PrepSmem<XS, KN>::BYTES;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
     return check_launch("gated_delta_rule: set smem attribute");
-  const dim3 grid((unsigned)(a.Bt * a.H * a.chunks));
-  if (a.after) launch_after(kern, grid, 128, bytes, st, a);
-  else kern<<<grid, 128, bytes, st>>>(a);
+  kern<<<(unsigned)(a.Bt * a.H * a.chunks), 128, bytes, st>>>(a);
   return check_launch("gated_delta_rule: chunk matrices");
 }
 

@@ -185,8 +185,6 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  let_next_start();
-  wait_for_previous();
 
   auto stage = [&](int c) { return smem + (c & 1) * SM::STAGE; };
   auto fail = [&](int code) {
@@ -583,8 +581,6 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  let_next_start();
-  wait_for_previous();
 
   // step k works on chunk n - 1 - k of the segment
   auto stage = [&](int k) { return smem + (k & 1) * SM::STAGE; };
@@ -892,12 +888,12 @@ int run(const TcCall& a, cudaStream_t st) {
     return check_launch("gated_delta_rule: set smem attribute");
   for (int64_t c0 = 0; c0 < nc; c0 += seg) {
     const int64_t m = std::min(seg, nc - c0);
-    const PrepCall p{a.B, a.C, a.A_log, a.dt, a.beta, a.img, nullptr, a.Bt, a.L, a.H, a.G, a.N, c0, m, nc, a.scale, 1, c0 > 0};
+    const PrepCall p{a.B, a.C, a.A_log, a.dt, a.beta, a.img, nullptr, a.Bt, a.L, a.H, a.G, a.N, c0, m, nc, a.scale, 1};
     if (int e = prep_run(p, TSSM_BF16, 2, st)) return e;
     const bool last = c0 + m == nc;
     const ScanArgs s{a.img, c0 ? a.carry : a.h0, last && !a.h_last ? nullptr : a.carry, a.states, a.errs, status, a.L,
                      c0, m, nc, (int)a.H, (int)a.G, (int)a.P, (int)a.N, (int)cdiv(a.P, 128), a.scale};
-    launch_after(scan, dim3((unsigned)(streams * s.npb)), 512, ScanSmem<KN>::BYTES, st, mk, mq, mu, my, s);
+    scan<<<(unsigned)(streams * s.npb), 512, ScanSmem<KN>::BYTES, st>>>(mk, mq, mu, my, s);
   }
   return check_launch("gated_delta_rule");
 }
@@ -921,11 +917,11 @@ int run_back(const TcBackCall& a, cudaStream_t st) {
     return check_launch("gated_delta_rule_bwd: set smem attribute");
   for (int64_t end = nc; end > 0; end -= seg) {   // segments from the last; dh0 carries the state's gradient
     const int64_t c0 = std::max<int64_t>(0, end - seg), m = end - c0;
-    const PrepCall p{a.B, a.C, a.A_log, a.dt, a.beta, a.img, a.gates, a.Bt, a.L, a.H, a.G, a.N, c0, m, nc, a.scale, 1, end < nc};
+    const PrepCall p{a.B, a.C, a.A_log, a.dt, a.beta, a.img, a.gates, a.Bt, a.L, a.H, a.G, a.N, c0, m, nc, a.scale, 1};
     if (int e = prep_run(p, TSSM_BF16, 3, st)) return e;
     const BackArgs s{a.img, end == nc ? a.dh_last : a.dh0, a.dh0, a.dstates, a.derrs, (__nv_bfloat16*)a.du, status, a.L,
                      c0, m, nc, (int)a.H, (int)a.G, (int)a.P, (int)a.N, (int)cdiv(a.P, 128), a.scale};
-    launch_after(scan, dim3((unsigned)(streams * s.npb)), 384, BackSmem<KN>::BYTES, st, mk, mq, mo, s);
+    scan<<<(unsigned)(streams * s.npb), 384, BackSmem<KN>::BYTES, st>>>(mk, mq, mo, s);
   }
   return check_launch("gated_delta_rule_bwd: chain");
 }

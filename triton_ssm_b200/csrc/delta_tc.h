@@ -15,7 +15,6 @@ struct PrepCall {
   int64_t Bt, L, H, G, N, c0, chunks, nc;
   float scale;
   int vec;       // N and the bases allow 16-byte pieces
-  int after;     // not the first kernel of its call
 };
 int prep_run(const PrepCall& a, int dtype, int na, cudaStream_t st);   // na planes of Aq: 2 (bf16 y) or 3 (f32)
 int64_t prep_image_bytes(int na);
