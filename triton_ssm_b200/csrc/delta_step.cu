@@ -7,8 +7,9 @@
 // other operands are shared by the P rows of a head).  Eight lanes own a row
 // and hold it in registers between the two dot products, so each row is read
 // and written once; lane l takes the 16-byte pieces l, l+8, ... so that eight
-// lanes cover 128 contiguous bytes per load.  A thread's ROWS rows belong to
-// one head (B, C in registers once) and their loads go out before any is used.
+// lanes cover 128 contiguous bytes per load.  One row a thread and many resident
+// blocks: at 192 streams x 32 heads of 128 x 128 the states (805 MB moved) take 120 us,
+// as long as a copy of them; two and four rows a thread took 125 to 170.
 #include "common.cuh"
 
 namespace tssm {
@@ -42,32 +43,28 @@ __device__ __forceinline__ float sum8(float v) {
 }
 
 // NV: 4-wide pieces of a row per lane (N <= 32 NV); VEC: 16-byte state and aligned B, C pieces.
-template <typename IO, int NV, int ROWS, bool VEC>
+template <typename IO, int NV, bool VEC>
 __global__ void __launch_bounds__(256) delta_step_kernel(
     const IO* __restrict__ x, const float* __restrict__ dt, float* __restrict__ h, const float* __restrict__ A_log,
     const IO* __restrict__ B, const IO* __restrict__ C, const float* __restrict__ beta, IO* __restrict__ y, int H,
     int G, int P, int N, int ptiles, float scale) {
   const int64_t sh = blockIdx.x / ptiles;   // (stream, head)
-  const int p0 = (int)(blockIdx.x - sh * ptiles) * (GROUPS * ROWS) + threadIdx.x / LANES;
+  const int p = (int)(blockIdx.x - sh * ptiles) * GROUPS + threadIdx.x / LANES;
+  const bool ok = p < P;
   const int l = threadIdx.x % LANES;
   const int64_t s = sh / H;
   const int hh = (int)(sh - s * H);
-  float* hp = h + (sh * P) * N;
-  float st[ROWS][NV][4];
+  float* hp = h + (sh * P + p) * N;
+  float st[NV][4];
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    const int p = p0 + r * GROUPS;
+  for (int j = 0; j < NV; ++j) {
+    const int n = 4 * (l + LANES * j);
+    if constexpr (VEC) {
+      const float4 v = ok && n < N ? __ldcs(reinterpret_cast<const float4*>(hp + n)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      st[j][0] = v.x; st[j][1] = v.y; st[j][2] = v.z; st[j][3] = v.w;
+    } else {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int n = 4 * (l + LANES * j);
-      if constexpr (VEC) {
-        const float4 v = p < P && n < N ? __ldcs(reinterpret_cast<const float4*>(hp + (int64_t)p * N + n))
-                                        : make_float4(0.f, 0.f, 0.f, 0.f);
-        st[r][j][0] = v.x; st[r][j][1] = v.y; st[r][j][2] = v.z; st[r][j][3] = v.w;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) st[r][j][i] = p < P && n + i < N ? hp[(int64_t)p * N + n + i] : 0.f;
-      }
+      for (int i = 0; i < 4; ++i) st[j][i] = ok && n + i < N ? hp[n + i] : 0.f;
     }
   }
   const int64_t kv = (s * G + hh / (H / G)) * N;
@@ -78,43 +75,35 @@ __global__ void __launch_bounds__(256) delta_step_kernel(
     load4<IO, VEC>(C + kv, 4 * (l + LANES * j), N, q[j]);
   }
   const float a = expf(-expf(__ldg(A_log + hh)) * __ldg(dt + sh));
-  const float bt = __ldg(beta + sh);
+  const float xv = ok ? ldf(x + sh * P + p) : 0.f;
+  float pred = 0.f;
 #pragma unroll
-  for (int r = 0; r < ROWS; ++r) {
-    const int p = p0 + r * GROUPS;
-    const bool ok = p < P;
-    const float xv = ok ? ldf(x + sh * P + p) : 0.f;
-    float pred = 0.f;
+  for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        st[r][j][i] *= a;
-        pred += st[r][j][i] * k[j][i];
-      }
-    const float e = bt * (xv - sum8(pred));
-    float out = 0.f;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int n = 4 * (l + LANES * j);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        st[r][j][i] += e * k[j][i];
-        out += st[r][j][i] * q[j][i];
-      }
-      if constexpr (VEC) {
-        if (ok && n < N)
-          __stcs(reinterpret_cast<float4*>(hp + (int64_t)p * N + n),
-                 make_float4(st[r][j][0], st[r][j][1], st[r][j][2], st[r][j][3]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (ok && n + i < N) hp[(int64_t)p * N + n + i] = st[r][j][i];
-      }
+    for (int i = 0; i < 4; ++i) {
+      st[j][i] *= a;
+      pred += st[j][i] * k[j][i];
     }
-    out = sum8(out);
-    if (ok && l == 0) stf(y + sh * P + p, scale * out);
+  const float e = __ldg(beta + sh) * (xv - sum8(pred));
+  float out = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    const int n = 4 * (l + LANES * j);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      st[j][i] += e * k[j][i];
+      out += st[j][i] * q[j][i];
+    }
+    if constexpr (VEC) {
+      if (ok && n < N) __stcs(reinterpret_cast<float4*>(hp + n), make_float4(st[j][0], st[j][1], st[j][2], st[j][3]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (ok && n + i < N) hp[n + i] = st[j][i];
+    }
   }
+  out = sum8(out);
+  if (ok && l == 0) stf(y + sh * P + p, scale * out);
 }
 
 struct StepArgs {
@@ -125,22 +114,17 @@ struct StepArgs {
   float scale;
 };
 
-template <typename IO, int NV, int ROWS, bool VEC>
+template <typename IO, int NV, bool VEC>
 void launch(const StepArgs& a, cudaStream_t st) {
-  const int ptiles = (int)cdiv(a.P, GROUPS * ROWS);
-  delta_step_kernel<IO, NV, ROWS, VEC><<<(unsigned)(a.S * a.H * ptiles), 256, 0, st>>>(
+  const int ptiles = (int)cdiv(a.P, GROUPS);
+  delta_step_kernel<IO, NV, VEC><<<(unsigned)(a.S * a.H * ptiles), 256, 0, st>>>(
       (const IO*)a.x, (const float*)a.dt, (float*)a.h, (const float*)a.A_log, (const IO*)a.B, (const IO*)a.C,
       (const float*)a.beta, (IO*)a.y, a.H, a.G, a.P, a.N, ptiles, a.scale);
 }
 
 template <typename IO, int NV>
 void pick(const StepArgs& a, bool vec, cudaStream_t st) {
-  // Four rows per thread keep enough loads in flight on a full GPU; with fewer blocks
-  // than SMs one row per thread spreads a small batch over more of them.
-  const bool many = a.P > GROUPS && a.S * a.H * cdiv(a.P, GROUPS * 4) >= 2 * num_sms();
-  constexpr int R = NV <= 4 ? 4 : 2;
-  if (vec) many ? launch<IO, NV, R, true>(a, st) : launch<IO, NV, 1, true>(a, st);
-  else many ? launch<IO, NV, R, false>(a, st) : launch<IO, NV, 1, false>(a, st);
+  vec ? launch<IO, NV, true>(a, st) : launch<IO, NV, false>(a, st);
 }
 
 template <typename IO>
