@@ -11,7 +11,9 @@
 //   S^T  = exp(l_last) S^T + (E diag(w beta))^T K   (S in f32 registers, the sum from TMEM)
 //   O^T  = scale exp(l) S^T Q^T + E^T (Aq diag(beta))^T   (two planes: y is bf16)
 // Warps: 0 issues the chain's products, 2 those of O, 1 copies, 4-11 are the chain (two
-// per 32 lanes, each half of the columns: S 64 f32 a thread), 12-15 the outputs.  The
+// per 32 lanes, each half of the columns: S 64 f32 a thread), 12-15 the outputs (four
+// chain warps per 32 lanes, a quarter each, took 3.8 instead of 3.2 us a chunk: they
+// slow the issuing warps down).  The
 // chain is serial, so its latency counts: pieces of its operands are handed over as
 // they are written, by named barriers (a hand-over through an mbarrier measured 136
 // cycles, through a barrier 25), and a product runs while the next piece is split.
