@@ -11,13 +11,15 @@
 //   S^T  = exp(l_last) S^T + (E diag(w beta))^T K   (S in f32 registers, the sum from TMEM)
 //   O^T  = scale exp(l) S^T Q^T + E^T (Aq diag(beta))^T   (two planes: y is bf16)
 // Warps: 0 issues the chain's products, 2 those of O, 1 copies, 4-11 are the chain (two
-// per 32 lanes, each half of the columns: S 64 f32 a thread), 12-15 the outputs (four
-// chain warps per 32 lanes, a quarter each, took 3.8 instead of 3.2 us a chunk: they
-// slow the issuing warps down).  The
+// per 32 lanes, each half of the columns: S 64 f32 a thread), 12-15 the outputs.  The
 // chain is serial, so its latency counts: pieces of its operands are handed over as
 // they are written, by named barriers (a hand-over through an mbarrier measured 136
 // cycles, through a barrier 25), and a product runs while the next piece is split.
 // tcgen05 takes 32 cycles per 128 x 64 x 16 and 190 from issue to a thread that waits.
+// Measured: 3.2 us a chunk (N = P = 128; 113 us for 2 x 2048 tokens x 16 heads, where the
+// tensor pipe is busy 45 % of the time on the SMs that have a block); four chain warps per
+// 32 lanes, a quarter of the columns each, took 3.8: they slow the issuing warps down.
+// Those sequences took 317 us in all on the register chain, 136 here.
 //
 // TMEM columns: [0, 192) S planes (planes 0, 1 of a half side by side, then both plane
 // 2s), later the state update's sum over planes 0, 1.  [192, 256) KS.  [256, 352) X
