@@ -199,3 +199,19 @@ def test_entry_point_refusals_without_gpu():
     bwd = lib.tssm_group_norm_act_bwd
     assert bwd(one, one, one, one, one, one, one, one, one, one, 1, 2, 3, 8, 2, 1, 0, 0) == 1
     assert bwd(one, one, one, one, 0, one, one, one, one, one, 1 << 20, 2, 3, 8, 2, 1, 0, 0) == 1
+
+
+def test_negative_eps_is_refused_without_gpu():
+    from triton_ssm_b200 import _lib
+    lib, one = _lib.load_library(), 4096   # a non-null address that nothing reads
+    for eps in (-1e-5, float("nan")):
+        assert lib.tssm_group_norm_act(one, one, one, one, one, one, one, 1 << 20, 2, 3, 8, 2, eps, 1, 0, 0) == 1
+
+
+@pytest.mark.gpu
+def test_eps_zero_negative_and_empty_maps(cuda_ops):
+    x, w, b, _ = (t.to(dev) for t in make(2, 0, 8, torch.float32))
+    _, mean, rstd = cuda_ops.group_norm_act(x, w, b, 2, eps=0, return_stats=True)
+    assert not mean.any() and bool(rstd.isinf().all())
+    with pytest.raises(ValueError, match="eps"):
+        cuda_ops.group_norm_act(x, w, b, 2, eps=-1.0)

@@ -985,6 +985,7 @@ extern "C" int tssm_group_norm_act(const void* x, const void* weight, const void
                                    int64_t C, int64_t groups, double eps, int act, int dtype, tssm_stream_t stream) {
   using namespace tssm;
   if (int e = check_sizes("group_norm_act", Bt, L, C, groups, act, dtype)) return e;
+  TSSM_REQUIRE(eps >= 0, "group_norm_act: eps must not be negative (got %g)", eps);
   if (Bt * L * C == 0) return TSSM_OK;
   TSSM_REQUIRE(x && weight && bias && y, "group_norm_act: null pointer");
   TSSM_REQUIRE((mean != nullptr) == (rstd != nullptr), "group_norm_act: mean and rstd go together");

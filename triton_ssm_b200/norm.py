@@ -49,7 +49,9 @@ def group_norm_act(x, weight, bias, groups, eps=1e-5, act="silu", return_stats=F
     [Bt,groups] f32 when ``return_stats`` (the backward takes them).
     """
     dev = same_device(x, weight, bias, y)
-    groups = int(groups)
+    groups, eps = int(groups), float(eps)
+    if not eps >= 0:
+        raise ValueError("group_norm_act: eps must not be negative (got %r)" % eps)
     Bt, L, C = _norm_args("group_norm_act", x, weight, bias, groups, act)
     x, weight, bias = x.contiguous(), weight.contiguous(), bias.contiguous()
     if y is None:
@@ -63,12 +65,12 @@ def group_norm_act(x, weight, bias, groups, eps=1e-5, act="silu", return_stats=F
         mean, rstd = torch.empty(2, Bt, groups, device=x.device, dtype=torch.float32)
         if L == 0:
             mean.zero_()
-            rstd.fill_(float(eps) ** -0.5)
+            rstd.fill_(eps ** -0.5 if eps else float("inf"))
     if not narrow:
         ws, need = _workspace(x, Bt, L, C, groups, False)
     with on_device(dev):
         call("tssm_group_norm_act", addr(x), addr(weight), addr(bias), addr(y), addr(mean), addr(rstd), addr(ws), need, Bt, L,
-             C, groups, float(eps), _ACT[act], dtype_code(x), raw_stream(dev))
+             C, groups, eps, _ACT[act], dtype_code(x), raw_stream(dev))
     return (y, mean, rstd) if return_stats else y
 
 
