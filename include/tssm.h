@@ -472,7 +472,8 @@ int tssm_gated_delta_step(const void* x, const void* dt, void* h, const void* A_
  * null); N <= 128; all contiguous.  states [Bt,H,ceil(L/64),ceil(N/4),P,4]
  * f32 (the state before every 64-token chunk, four n beside each other) and
  * errors [Bt,H,ceil(L/4),P,4] f32 (u - hd B, four tokens beside each other)
- * are what the backward reads; 16-byte aligned, both null when none follows.  workspace:
+ * are what the backward reads; 16-byte aligned, both null when none follows.
+ * h_last may be h0 (the state is then updated in place).  workspace:
  * tssm_gated_delta_rule_workspace_size bytes (0 for shapes that need none),
  * 16-byte aligned.
  */

@@ -815,7 +815,8 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
                "gated_delta_rule_bwd: H (%lld) must be a positive multiple of the key heads G (%lld)", (long long)H,
                (long long)G);
   TSSM_REQUIRE(dtype == TSSM_F32 || dtype == TSSM_BF16, "gated_delta_rule_bwd: dtype must be f32 or bf16 (got %d)", dtype);
-  TSSM_REQUIRE(L < (int64_t(1) << 31) && Bt < (int64_t(1) << 31) && H <= 1 << 20 && P <= 1 << 20,
+  TSSM_REQUIRE(L < (int64_t(1) << 31) && Bt < (int64_t(1) << 31) && H <= 1 << 20 && P <= 1 << 20 &&
+                   Bt * H * std::max(cdiv(L, delta::Q), cdiv(P, 16)) < (int64_t(1) << 31),
                "gated_delta_rule_bwd: size out of range");
   TSSM_REQUIRE(A_log && dA_log && (Bt == 0 || dh0), "gated_delta_rule_bwd: null pointer");
   TSSM_REQUIRE(Bt * L == 0 || (u && B && C && dt && beta && dy && states && errors && du && dB && dC && ddt && dbeta),

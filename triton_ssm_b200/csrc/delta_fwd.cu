@@ -380,7 +380,8 @@ extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const voi
   TSSM_REQUIRE(A_log && (L == 0 || (u && B && C && dt && beta && y)), "gated_delta_rule: null pointer");
   TSSM_REQUIRE((states != nullptr) == (errors != nullptr), "gated_delta_rule: states and errors go together");
   TSSM_REQUIRE(dtype == TSSM_F32 || dtype == TSSM_BF16, "gated_delta_rule: dtype must be f32 or bf16 (got %d)", dtype);
-  TSSM_REQUIRE(L < (int64_t(1) << 31) && Bt < (int64_t(1) << 31) && H <= 1 << 20 && P <= 1 << 20,
+  TSSM_REQUIRE(L < (int64_t(1) << 31) && Bt < (int64_t(1) << 31) && H <= 1 << 20 && P <= 1 << 20 &&
+                   Bt * H * std::max(cdiv(L, delta::Q), cdiv(P, 16)) < (int64_t(1) << 31),
                "gated_delta_rule: size out of range");
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   const uintptr_t bases = reinterpret_cast<uintptr_t>(u) | reinterpret_cast<uintptr_t>(B) |
@@ -394,7 +395,7 @@ extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const voi
   const int na = dtype == TSSM_F32 ? 3 : 2;
   const int64_t streams = Bt * H, nc = cdiv(L, delta::Q);
   if (nc == 0) {   // no tokens: the state passes through
-    if (!h_last) return TSSM_OK;
+    if (!h_last || h_last == h0) return TSSM_OK;
     const size_t bytes = (size_t)(streams * P * N) * 4;
     if ((h0 ? cudaMemcpyAsync(h_last, h0, bytes, cudaMemcpyDeviceToDevice, st) : cudaMemsetAsync(h_last, 0, bytes, st)) !=
         cudaSuccess)

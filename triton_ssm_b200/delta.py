@@ -58,7 +58,8 @@ def _rule_args(name, u, A_log, B, C, dt, beta, h0):
     return Bt, L, H, G, P, N
 
 
-def gated_delta_rule(u, A_log, B, C, dt, beta, scale=1.0, h0=None, return_state=False, save=False, y=None):
+def gated_delta_rule(u, A_log, B, C, dt, beta, scale=1.0, h0=None, return_state=False, save=False, y=None,
+                     h_last=None):
     """The gated delta rule over whole sequences.
 
     u [Bt,L,H*P] f32 or bf16; A_log [H] f32 (log(-A_h)); B, C [Bt,L,G,N] in
@@ -66,12 +67,13 @@ def gated_delta_rule(u, A_log, B, C, dt, beta, scale=1.0, h0=None, return_state=
     [Bt,H,P,N] f32 or None.  Values must be finite (a chunk of 64 tokens is one
     matrix problem); pad with zeros, dt = 0 and beta = 0.
     Returns y [Bt,L,H*P] in u's dtype, or a tuple: y, then h_last [Bt,H,P,N]
-    f32 when ``return_state``, then, when ``save``, what
+    f32 when ``return_state`` (written to the given ``h_last``, which may be
+    h0 itself: the state is then updated in place), then, when ``save``, what
     ``gated_delta_rule_bwd`` reads: (the state before every chunk of 64 tokens
     [Bt,H,ceil(L/64),ceil(N/4),P,4], the prediction errors u_t - hd B_t
     [Bt,H,ceil(L/4),P,4]), f32.
     """
-    dev = same_device(u, A_log, B, C, dt, beta, h0, y)
+    dev = same_device(u, A_log, B, C, dt, beta, h0, y, h_last)
     Bt, L, H, G, P, N = _rule_args("gated_delta_rule", u, A_log, B, C, dt, beta, h0)
     u, B, C = _dense(u), _dense(B), _dense(C)
     A_log, dt, beta = _f32(A_log), _f32(dt), _f32(beta)
@@ -81,7 +83,11 @@ def gated_delta_rule(u, A_log, B, C, dt, beta, scale=1.0, h0=None, return_state=
     elif y.shape != u.shape or y.dtype != u.dtype or not y.is_contiguous():
         raise ValueError("gated_delta_rule: y must be contiguous and match u")
     f32 = dict(device=u.device, dtype=torch.float32)
-    hl = torch.empty(Bt, H, P, N, **f32) if return_state else None
+    hl = h_last
+    if hl is None:
+        hl = torch.empty(Bt, H, P, N, **f32) if return_state else None
+    elif not return_state or hl.shape != (Bt, H, P, N) or hl.dtype != torch.float32 or not hl.is_contiguous():
+        raise ValueError("gated_delta_rule: h_last must be contiguous f32 [Bt,H,P,N], with return_state=True")
     states = torch.empty(Bt, H, -(-L // CHUNK), -(-N // 4), P, 4, **f32) if save else None
     errors = torch.empty(Bt, H, -(-L // 4), P, 4, **f32) if save else None
     need = int(_lib.load_library().tssm_gated_delta_rule_workspace_size(Bt, L, H, G, P, N, dtype_code(u)))
@@ -158,5 +164,5 @@ def gated_delta_step(x, dt, h, A_log, B, C, beta, scale=1.0, y=None):
         raise ValueError("gated_delta_step: y must be contiguous and match x")
     with on_device(dev):
         call("tssm_gated_delta_step", x.data_ptr(), dt.data_ptr(), h.data_ptr(), A_log.data_ptr(), B.data_ptr(),
-             C.data_ptr(), beta.data_ptr(), y.data_ptr(), S, H, G, P, N, scale, dtype_code(x), raw_stream(dev))
+             C.data_ptr(), beta.data_ptr(), y.data_ptr(), S, H, G, P, N, float(scale), dtype_code(x), raw_stream(dev))
     return y

@@ -95,7 +95,7 @@ class StreamingRing:
 
 class DeltaStream:
     """S independent streams of a gated-delta-rule layer: the state h [S,H,P,N]
-    f32 stays on the device, ``prefill`` advances every stream by a prompt,
+    f32 stays in place on the device, ``prefill`` advances every stream by a prompt,
     ``step`` by one token.  Outputs are normalised per token and head (group
     norm with H groups), then ``act``.
 
@@ -136,7 +136,8 @@ class DeltaStream:
         are shorter are padded at their end with zeros (dt = beta = 0).  Returns [S,L,H*P]."""
         if u.dim() != 3 or u.shape[0] != self.h.shape[0]:
             raise ValueError("DeltaStream.prefill: u must be [S,L,H*P] with S = %d streams" % self.h.shape[0])
-        y, self.h = gated_delta_rule(u, self.A_log, B, C, dt, beta, scale=self.scale, h0=self.h, return_state=True)
+        y, _ = gated_delta_rule(u, self.A_log, B, C, dt, beta, scale=self.scale, h0=self.h, return_state=True,
+                                h_last=self.h)
         self.tokens += u.shape[1]
         return self._norm(y)
 
