@@ -370,6 +370,29 @@ __device__ __forceinline__ void invert_unit_lower(float* M, int t, int bar) {
 // A 64 x 64 tile of planes: 128-byte rows.
 constexpr int SQ_RB = 128, SQ_BYTES = Q * SQ_RB;
 
+// Eight values, as three planes of 16-byte pieces.
+__device__ __forceinline__ void put8(uint8_t* dst, int plane, const float (&f)[8]) {
+  uint32_t w[4][3];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) split2<3>(f[2 * q], f[2 * q + 1], w[q]);
+#pragma unroll
+  for (int z = 0; z < 3; ++z)
+    *reinterpret_cast<uint4*>(dst + z * plane) = make_uint4(w[0][z], w[1][z], w[2][z], w[3][z]);
+}
+
+// Four tokens (rows from r) of channels 2 lane, 2 lane + 1 into three planes of a 64 x 64 tile.
+__device__ __forceinline__ void put4x2(uint8_t* tile, int r, int lane, const float4 (&f)[2]) {
+  const float a[4] = {f[0].x, f[0].y, f[0].z, f[0].w}, b[4] = {f[1].x, f[1].y, f[1].z, f[1].w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t w[3];
+    split2<3>(a[i], b[i], w);
+#pragma unroll
+    for (int z = 0; z < 3; ++z)
+      *reinterpret_cast<uint32_t*>(tile + z * SQ_BYTES + tile_off<SQ_RB>(r + i, lane / 4) + 4 * (lane % 4)) = w[z];
+  }
+}
+
 // A chunk's image, as it lies in shared memory: T planes, NA planes of Aq diag(beta), gates.
 constexpr int IMG_T = 0, IMG_AQ = 3 * SQ_BYTES;
 __host__ __device__ constexpr int img_gates(int na) { return IMG_AQ + na * SQ_BYTES; }

@@ -286,28 +286,6 @@ struct GradSmem {
 };
 constexpr int GT = 512;   // threads: warp = (16 tokens, a quarter of N)
 
-__device__ __forceinline__ void put8(uint8_t* dst, int plane, const float (&f)[8]) {
-  uint32_t w[4][3];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) split2<3>(f[2 * q], f[2 * q + 1], w[q]);
-#pragma unroll
-  for (int z = 0; z < 3; ++z)
-    *reinterpret_cast<uint4*>(dst + z * plane) = make_uint4(w[0][z], w[1][z], w[2][z], w[3][z]);
-}
-
-// Four tokens (rows from r) of channels 2 lane, 2 lane + 1 into three planes of a 64 x 64 tile.
-__device__ __forceinline__ void put4x2(uint8_t* tile, int r, int lane, const float4 (&f)[2]) {
-  const float a[4] = {f[0].x, f[0].y, f[0].z, f[0].w}, b[4] = {f[1].x, f[1].y, f[1].z, f[1].w};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t w[3];
-    split2<3>(a[i], b[i], w);
-#pragma unroll
-    for (int z = 0; z < 3; ++z)
-      *reinterpret_cast<uint32_t*>(tile + z * SQ_BYTES + tile_off<SQ_RB>(r + i, lane / 4) + 4 * (lane % 4)) = w[z];
-  }
-}
-
 template <int XS, int KN>
 __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) {
   let_next_start();
@@ -729,6 +707,18 @@ int launch_chain(BwdArgs a, cudaStream_t st) {
 }
 
 template <int XS, int KN>
+int launch_grad(const BwdArgs& a, cudaStream_t st) {
+  constexpr int bytes = GradSmem<XS, KN>::BYTES;
+  static_assert(bytes <= 232448, "shared-memory layout exceeds the per-block limit");
+  auto kern = delta_bwd_grad_kernel<XS, KN>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+    return check_launch("gated_delta_rule_bwd: set smem attribute");
+  TSSM_REQUIRE(a.Bt * a.H * a.nc < (int64_t(1) << 31), "gated_delta_rule_bwd: size out of range");
+  launch_next(kern, (unsigned)(a.Bt * a.H * a.nc), GT, bytes, st, a);
+  return check_launch("gated_delta_rule_bwd: gradients");
+}
+
+template <int XS, int KN>
 int launch_all(BwdArgs a, bool tc, cudaStream_t st) {
   using T = typename std::conditional<XS == 1, __nv_bfloat16, float>::type;
   if (a.nc == 0) {   // no tokens: the state's gradient passes through
@@ -754,18 +744,18 @@ int launch_all(BwdArgs a, bool tc, cudaStream_t st) {
     }
   }
   if (a.nc > 0) {
-    constexpr int bytes = GradSmem<XS, KN>::BYTES;
-    static_assert(bytes <= 232448, "shared-memory layout exceeds the per-block limit");
-    auto kern = delta_bwd_grad_kernel<XS, KN>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
-      return check_launch("gated_delta_rule_bwd: set smem attribute");
-    TSSM_REQUIRE(a.Bt * a.H * a.nc < (int64_t(1) << 31), "gated_delta_rule_bwd: size out of range");
-    launch_next(kern, (unsigned)(a.Bt * a.H * a.nc), GT, bytes, st, a);
-    if (a.dk_part) {
-      const int64_t n = a.Bt * a.L * a.G * a.N;
-      TSSM_REQUIRE(cdiv(n, 256) < (int64_t(1) << 31), "gated_delta_rule_bwd: size out of range");
-      launch_next(delta_head_sum_kernel<T>, (unsigned)cdiv(n, 256), 256, 0, st, (const float*)a.dk_part,
-                   (const float*)a.dq_part, (T*)a.dB, (T*)a.dC, n, a.G, a.H / a.G, a.N);
+    if (tc_grad_takes(a.H, a.G, a.N, tc)) {   // key heads summed as well
+      const TcGradCall t{a.B, a.C, a.dy, a.A_log, a.dt, a.states, a.errs, a.dstates, a.derrs, a.gates, a.dB, a.dC, a.ddt,
+                         a.dbeta, a.da_part, a.Bt, a.L, a.H, a.G, a.P, a.nc, a.scale, nullptr};
+      if (int e = tc_grad_run(t, st)) return e;
+    } else {
+      if (int e = launch_grad<XS, KN>(a, st)) return e;
+      if (a.dk_part) {
+        const int64_t n = a.Bt * a.L * a.G * a.N;
+        TSSM_REQUIRE(cdiv(n, 256) < (int64_t(1) << 31), "gated_delta_rule_bwd: size out of range");
+        launch_next(delta_head_sum_kernel<T>, (unsigned)cdiv(n, 256), 256, 0, st, (const float*)a.dk_part,
+                    (const float*)a.dq_part, (T*)a.dB, (T*)a.dC, n, a.G, a.H / a.G, a.N);
+      }
     }
   }
   launch_next(delta_da_kernel, (unsigned)a.H, 256, 0, st, (const float*)a.da_part, a.dA_log, a.Bt, a.H, a.nc);

@@ -75,12 +75,6 @@ constexpr uint32_t C_KS = 192, C_XP = 256, C_E = 352, C_O = 416;
 // named barriers (0: __syncthreads): outputs; pieces of S, X, E diag(w beta), E for their issuers
 constexpr uint32_t B_OUT = 1, B_S = 2, B_X = 6, B_W = 8, B_E = 10, B_ISSUE = 256 + 32;
 
-// One lane of a converged warp (always the same one).
-__device__ __forceinline__ bool elect_one() {
-  uint32_t e;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(e));
-  return e != 0;
-}
 // D (+)= A B with A in TMEM: row m in lane m, 16 bf16 of k in 8 columns.
 __device__ __forceinline__ void umma_bf16_ta(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
   asm volatile(
@@ -104,19 +98,6 @@ __device__ __forceinline__ void tmem_st8u(uint32_t taddr, const uint32_t (&u)[8]
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(u[0]),
                "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
                : "memory");
-}
-// 16 columns of TMEM into registers.  The wait is part of the statement, so that no use of
-// the values can be scheduled before it.
-__device__ __forceinline__ void tmem_get16(uint32_t taddr, float (&r)[16]) {
-  uint32_t* u = reinterpret_cast<uint32_t*>(r);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
-        "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
-      : "r"(taddr)
-      : "memory");
 }
 // 16 values as NS planes of 8 columns, plane s at taddr[s] (r is used up).
 template <int NS>

@@ -46,5 +46,20 @@ bool tc_takes(int64_t P, int64_t N, int dtype);
 int tc_run(const TcCall& a, cudaStream_t st);
 int tc_back_run(const TcBackCall& a, cudaStream_t st);
 
+// delta_grad_tc.cu: the gradients of every (chunk, head) on tcgen05 (what tc_takes, with N = 128 and
+// at most 8 value heads a key head).
+struct TcGradCall {
+  const void *B, *C, *dy;
+  const float *A_log, *dt, *states, *errs, *dstates, *derrs;
+  const void* gates;
+  void *dB, *dC;
+  float *ddt, *dbeta, *da_part;
+  int64_t Bt, L, H, G, P, nc;
+  float scale;
+  int* status;   // set by tc_grad_run
+};
+bool tc_grad_takes(int64_t H, int64_t G, int64_t N, bool tc);
+int tc_grad_run(TcGradCall a, cudaStream_t st);
+
 }  // namespace delta
 }  // namespace tssm
