@@ -2,7 +2,7 @@
 //
 // With dO, the gradient dS1 of the state behind a chunk, and E, S0 as the
 // forward saved them (w = exp(l_last - l), A strictly lower, both without beta):
-//     R   = diag(beta) (Aq^T dO + w K dS1)             dE = T^T R  (= dV)
+//     R   = diag(beta) (Aq^T dO + w K dS1)             dE = T^T R  (= du)
 //     dS0 = exp(l_last) dS1 + (scale exp(l) Q)^T dO - (exp(l) K)^T dE
 //     M1  = scale D (dO E^T) diag(beta)                M2 = D (dE E^T) diag(beta), strictly lower
 //     dQ  = scale exp(l) dO S0^T + M1 K
@@ -16,15 +16,18 @@
 //
 // The chain runs the chunks of a (batch row, head) backwards as the forward runs them
 // forwards, over the images of delta_prep.cu, and leaves dE and the dS1 of every chunk in
-// HBM.  bf16 shapes that delta_tc.cu takes run there; the kernel here (16 value channels
+// HBM (du, which is dE, is written by the gradient kernel: in the serial chain its narrow stores
+// took 20 us more than there).  bf16 shapes that delta_tc.cu takes run there; the kernel here (16 value channels
 // and a state gradient per warp, in registers) is for f32 and the others.  The gradient
-// kernel then takes all (chunk, head) pairs at once.  Shared key heads and dA_log are
+// kernel then takes all (chunk, head) pairs at once: delta_grad_tc.cu for the chain's bf16
+// shapes with N = 128, the one here (mma.sync) for the rest.  Shared key heads and dA_log are
 // summed last, in a fixed order, so results repeat bit for bit.
 //
 // Measured at 4 x 2048 tokens x 16 heads on 8 key heads, N = P = 128, bf16 (with the
-// forward 0.82 ms): images 37 us, chain 165, gradients 384, key heads 38, dA_log 3.  The
-// gradient kernel has 11 products of 64-wide tiles in 2 or 3 planes a pair: its mma.sync
-// pipe is busy 38 % of the time, the rest is the exposed loads of its one block an SM.
+// forward 0.62 ms): images 40 us, chain 151, gradients with du and the key heads' sums 262,
+// dA_log 3.  The gradient kernel here took 384 for them and 38 for the key heads: it has 11 products of
+// 64-wide tiles in 2 or 3 planes a pair, its mma.sync pipe is busy 38 % of the time, and the
+// loads of its one block an SM are exposed.
 #include "delta.cuh"
 #include "delta_tc.h"
 
@@ -235,8 +238,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(cons
         mma_planes<NS, XS, NS>(S[2 * nn], S[2 * nn + 1], fk, w);
       }
     }
-    // dE in f32 for the gradient kernel, du in io
-    const int64_t at = (b * a.L + t0) * su + (int64_t)h * a.P + pb + p0 + pr;
+    // dE for the gradient kernel
     float* ep = a.derrs + bh * saved_floats(a.P, a.L);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -246,9 +248,6 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(cons
         if (p0 + pr + p >= pvalid) continue;
         if ((tk & ~3) < rows)
           *saved_pair(ep, a.P, pb + p0 + pr + p, t0 + tk) = make_float2(er[i][2 * r], er[i][2 * r + 1]);
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-          if (tk + e < rows) stf((T*)a.du + at + (int64_t)(tk + e) * su + p, er[i][2 * r + e]);
       }
   };
 
@@ -369,6 +368,13 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
       }
       put4x2(smem + SM::E, 4 * warp, lane, fe);
       put4x2(smem + SM::DE, 4 * warp, lane, fr);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {   // du = dE
+        const float d[4] = {fr[q].x, fr[q].y, fr[q].z, fr[q].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (4 * warp + i < rows && 2 * lane + q < pv) stf((T*)a.du + tok + (4 * warp + i) * su + p0 + 2 * lane + q, d[i]);
+      }
     }
     cp_async_wait_all();
     __syncthreads();
@@ -727,7 +733,7 @@ int launch_all(BwdArgs a, bool tc, cudaStream_t st) {
         cudaSuccess)
       return check_launch("gated_delta_rule_bwd: pass the state's gradient");
   } else if (tc) {
-    const TcBackCall t{a.B, a.C, a.dy, a.A_log, a.dt, a.beta, a.dh_last, a.du, a.dh0, a.dstates, a.derrs, a.gates,
+    const TcBackCall t{a.B, a.C, a.dy, a.A_log, a.dt, a.beta, a.dh_last, a.dh0, a.dstates, a.derrs, a.gates,
                        a.img, a.Bt, a.L, a.H, a.G, a.P, a.N, a.scale};
     if (int e = tc_back_run(t, st)) return e;
   } else {
@@ -745,7 +751,7 @@ int launch_all(BwdArgs a, bool tc, cudaStream_t st) {
   }
   if (a.nc > 0) {
     if (tc_grad_takes(a.H, a.G, a.N, tc)) {   // key heads summed as well
-      const TcGradCall t{a.B, a.C, a.dy, a.A_log, a.dt, a.states, a.errs, a.dstates, a.derrs, a.gates, a.dB, a.dC, a.ddt,
+      const TcGradCall t{a.B, a.C, a.dy, a.A_log, a.dt, a.states, a.errs, a.dstates, a.derrs, a.gates, a.du, a.dB, a.dC, a.ddt,
                          a.dbeta, a.da_part, a.Bt, a.L, a.H, a.G, a.P, a.nc, a.scale, nullptr};
       if (int e = tc_grad_run(t, st)) return e;
     } else {
@@ -835,7 +841,8 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
   a.dq_part = sp.part ? a.dk_part + sp.part : nullptr;
   a.da_part = a.derrs + sp.derrs + 2 * sp.part;
   const uintptr_t bases = reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(dy) |
-                          reinterpret_cast<uintptr_t>(dh_last) | reinterpret_cast<uintptr_t>(dh0);
+                          reinterpret_cast<uintptr_t>(dh_last) | reinterpret_cast<uintptr_t>(dh0) |
+                          reinterpret_cast<uintptr_t>(du) | reinterpret_cast<uintptr_t>(dB) | reinterpret_cast<uintptr_t>(dC);
   a.gates = (Gates*)(a.da_part + sp.da);
   a.img = (uint8_t*)(a.da_part + sp.da + sp.gates);
   const bool tc = tc_takes(P, N, dtype) && (bases & 15u) == 0;

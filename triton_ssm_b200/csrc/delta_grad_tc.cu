@@ -11,8 +11,14 @@
 // dE E^T (triangles of 64 x 64, in registers), q.k and k.k stay on mma.sync, which runs meanwhile.
 //
 // 256 threads, 111 KB and half of TMEM: two blocks an SM, each waiting for its loads while the
-// other works.  The 64 x 128 accumulators of three such products leave no registers for a second
-// block; with them on mma.sync (one block of 512 threads) a chunk and head took 27 us on its SM.
+// other works (in registers, the three 64 x 128 accumulators leave room for one block only).
+// Blocks of one key head are a cluster: each leaves its dQ, dK in shared memory and sums a share
+// of the rows over all of them, in the heads' order (parts in HBM and a kernel for their sums took
+// 65 us more at 64 heads x 2048 tokens).
+// Measured there (2048 chunks and heads, P = 128, 16 value on 8 key heads): 262 us, 18 us for one on
+// its SM, against 27 on mma.sync.  Bound by shared memory: a 128 x 64 x 16 product reads 6 KB for
+// its 32 cycles, and planes, fragments and sums take about as many cycles again.  Fetching the next
+// blocks' states to L2 ahead made it slower (311): their own loads queued behind that.
 // K and Q come last, where dE and dO were.
 //
 // Every wait on an mbarrier is bounded; a block that gives up sets the status word and leaves its
@@ -175,6 +181,12 @@ __global__ void __launch_bounds__(NT, 2) delta_grad_tc_kernel(const TcGradCall a
     for (int r = 0; r < 2; ++r) {
       put4x2(smem + E, 4 * (warp + 8 * r), lane, fe[r]);
       put4x2(smem + DE, 4 * (warp + 8 * r), lane, fr[r]);
+      const float d0[4] = {fr[r][0].x, fr[r][0].y, fr[r][0].z, fr[r][0].w};
+      const float d1[4] = {fr[r][1].x, fr[r][1].y, fr[r][1].z, fr[r][1].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i)   // du = dE
+        if (4 * (warp + 8 * r) + i < rows)
+          *reinterpret_cast<uint32_t*>((T*)a.du + tok + (4 * (warp + 8 * r) + i) * su + p0 + 2 * lane) = pack2(d0[i], d1[i]);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) fetch(a.dstates, p0, i, fd[i]);   // arrives during the first products

@@ -19,7 +19,8 @@
 // Measured: 3.2 us a chunk (N = P = 128; 113 us for 2 x 2048 tokens x 16 heads, where the
 // tensor pipe is busy 45 % of the time on the SMs that have a block); four chain warps per
 // 32 lanes, a quarter of the columns each, took 3.8: they slow the issuing warps down.
-// Those sequences took 317 us in all on the register chain, 136 here.
+// States and errors for a backward, stored a quarter at a time between the steps: 4.4 us a chunk
+// (4.6 in one go).  Those sequences took 317 us in all on the register chain, 136 here.
 //
 // TMEM columns: [0, 192) S planes (planes 0, 1 of a half side by side, then both plane
 // 2s), later the state update's sum over planes 0, 1.  [192, 256) KS.  [256, 352) X
@@ -227,12 +228,15 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
         store_planes<NS>(at, r);
         hand_over(B_S + i);
       }
-      if (a.states && live && ok) {   // [N / 4][P][4]: 512 bytes a warp and store
+      auto save = [&](int q) {   // a quarter of the state, [N / 4][P][4]: 512 bytes a warp and store
+        if (!(a.states && live && ok)) return;
         float4* dst = reinterpret_cast<float4*>(a.states) +
                       ((bh * a.nc + a.c0 + c) * (a.N / 4) + half * (HN / 4)) * (int64_t)a.P + pb + p;
 #pragma unroll
-        for (int j = 0; j < HN; j += 4) dst[(int64_t)(j / 4) * a.P] = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
-      }
+        for (int j = q * HN / 4; j < (q + 1) * HN / 4; j += 4)
+          dst[(int64_t)(j / 4) * a.P] = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+      };
+      save(0);
       // X^T = V^T - exp(l) KS^T, 32 tokens of this half
       const uint8_t* st = stage(c);
       ok = ok && waitw(&full[c & 1], c >> 1, 2002);
@@ -259,6 +263,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
         store_planes<NS>(tl + C_XP + 48 * half + 8 * i, 16, x);
         hand_over(B_X + i);
       }
+      save(1);
       // E^T: planes of E diag(w beta) for the state
       ok = ok && waitw(edone, c, 2004);
 #pragma unroll 1
@@ -278,6 +283,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[c & 1]);   // V and the gates are read
+      save(2);
       // E's planes for O, over E (both pieces are read before either is written)
       {
         float x[2][16];
@@ -297,6 +303,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
         store_planes<2>(tl + C_E + 32 * half + 8, 16, x[1]);
       }
       hand_over(B_E);
+      save(3);
       // S^T
       ok = ok && waitw(dsdone, c, 2005);
 #pragma unroll
@@ -505,7 +512,6 @@ struct BackArgs {
   const uint8_t* img;
   const float* ds_in;
   float *ds_out, *dstates, *derrs;
-  __nv_bfloat16* du;
   int* status;
   int64_t L, c0, nseg, nc;
   int H, G, P, N, npb;
@@ -635,12 +641,15 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
         store_planes<NS>(at, r);
         hand_over(B_S + i);
       }
-      if (live && ok) {
+      auto save = [&](int q) {   // a quarter of the state's gradient
+        if (!(live && ok)) return;
         float4* dst = reinterpret_cast<float4*>(a.dstates) +
                       ((bh * a.nc + cc) * (a.N / 4) + half * (HN / 4)) * (int64_t)a.P + pb + p;
 #pragma unroll
-        for (int j = 0; j < HN; j += 4) dst[(int64_t)(j / 4) * a.P] = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
-      }
+        for (int j = q * HN / 4; j < (q + 1) * HN / 4; j += 4)
+          dst[(int64_t)(j / 4) * a.P] = make_float4(S[j], S[j + 1], S[j + 2], S[j + 3]);
+      };
+      save(0);
       // R^T; the last tokens' products reach all columns and go first
       ok = ok && waitw(ksdone, k, 2103);
 #pragma unroll 1
@@ -659,6 +668,7 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
         store_planes<NS>(tl + C_XP + 48 * half + 8 * i, 16, x);
         hand_over(B_X + i);
       }
+      save(1);
       // scale exp(l) dO, while dE is made
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
@@ -677,6 +687,7 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
         store_planes<NS>(at, x);
       }
       hand_over(B_D);
+      save(2);
       // -exp(l) dE
       ok = ok && waitw(edone, k, 2104);
 #pragma unroll 1
@@ -696,7 +707,8 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[k & 1]);   // dO and the gates are read
-      // dE for the gradient kernel, du
+      save(3);
+      // dE for the gradient kernel
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         float x[16];
@@ -704,14 +716,9 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
         const int64_t tk = cc * Q + 32 * half + 16 * i;
         const int left = live && ok ? (int)max((int64_t)0, min((int64_t)16, a.L - tk)) : 0;
         float4* ep = reinterpret_cast<float4*>(a.derrs + bh * saved_floats(a.P, a.L)) + tk / 4 * a.P + pb + p;
-        __nv_bfloat16* up = a.du + ((b * a.L + tk) * a.H + h) * (int64_t)a.P + pb + p;
-        const int su = a.H * a.P;
 #pragma unroll
         for (int j = 0; j < 16; j += 4)
           if (j < left) ep[j / 4 * a.P] = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (j < left) up[j * su] = __float2bfloat16_rn(x[j]);
       }
       // dS^T
       ok = ok && waitw(dsdone, k, 2105);
@@ -904,7 +911,7 @@ int run_back(const TcBackCall& a, cudaStream_t st) {
     const int64_t c0 = std::max<int64_t>(0, end - seg), m = end - c0;
     const PrepCall p{a.B, a.C, a.A_log, a.dt, a.beta, a.img, a.gates, a.Bt, a.L, a.H, a.G, a.N, c0, m, nc, a.scale, 1};
     if (int e = prep_run(p, TSSM_BF16, 3, st)) return e;
-    const BackArgs s{a.img, end == nc ? a.dh_last : a.dh0, a.dh0, a.dstates, a.derrs, (__nv_bfloat16*)a.du, status, a.L,
+    const BackArgs s{a.img, end == nc ? a.dh_last : a.dh0, a.dh0, a.dstates, a.derrs, status, a.L,
                      c0, m, nc, (int)a.H, (int)a.G, (int)a.P, (int)a.N, (int)cdiv(a.P, 128), a.scale};
     scan<<<(unsigned)(streams * s.npb), 384, BackSmem<KN>::BYTES, st>>>(mk, mq, mo, s);
   }

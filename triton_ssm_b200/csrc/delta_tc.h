@@ -32,10 +32,9 @@ struct TcCall {
   int64_t Bt, L, H, G, P, N;
   float scale;
 };
-struct TcBackCall {   // the backward's chain: dE, du, dS1 and gates of every chunk, dh0
+struct TcBackCall {   // the backward's chain: dE, dS1 and gates of every chunk, dh0
   const void *B, *C, *dy;
   const float *A_log, *dt, *beta, *dh_last;
-  void* du;
   float *dh0, *dstates, *derrs;
   void* gates;
   uint8_t* img;
@@ -52,7 +51,7 @@ struct TcGradCall {
   const void *B, *C, *dy;
   const float *A_log, *dt, *states, *errs, *dstates, *derrs;
   const void* gates;
-  void *dB, *dC;
+  void *du, *dB, *dC;
   float *ddt, *dbeta, *da_part;
   int64_t Bt, L, H, G, P, nc;
   float scale;
