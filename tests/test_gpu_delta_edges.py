@@ -3,7 +3,8 @@ and by captured steps, uninitialised buffers, many streams in f32, offsets behin
 import pytest
 import torch
 
-from test_gpu_delta import NAMES, make
+from oracle.delta import gated_delta_grads
+from test_gpu_delta import NAMES, check_grads, make, run_bwd
 from test_gpu_norm import make as make_norm
 
 dev = "cuda"
@@ -115,6 +116,21 @@ def test_many_narrow_streams_go_through_in_segments(cuda_ops, dtype, N, P):
 
     for x, y in zip(run(1), run(Bt // 2)):
         assert torch.equal(y[:2], x) and torch.equal(y[-2:], x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("Bt,L,H,G,P", [(2, 70, 6, 2, 64), (1, 129, 16, 2, 128), (3, 65, 32, 2, 64), (2, 64, 7, 1, 192)])
+def test_backward_of_shared_key_heads(cuda_ops, Bt, L, H, G, P, dtype):
+    """Key heads with 3, 7, 8 and 16 value heads each: their gradients are summed in different ways."""
+    N = 128
+    a, h0 = make(Bt, L, H, G, N, P, dtype, seed=L + H)
+    g = torch.Generator().manual_seed(H)
+    dy, dh = torch.randn(Bt, L, H, P, generator=g).to(dtype), 0.3 * torch.randn(Bt, H, P, N, generator=g)
+    grads = run_bwd(cuda_ops, a, h0, dy, dh, 0.3)
+    check_grads(grads, gated_delta_grads(*a.values(), dy, scale=0.3, h0=h0, dh_last=dh), a, dtype, L)
+    for x, y in zip(grads, run_bwd(cuda_ops, a, h0, dy, dh, 0.3)):
+        assert torch.equal(x, y)
 
 
 def rand(*shape, dtype=torch.float32):
