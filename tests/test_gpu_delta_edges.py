@@ -133,6 +133,44 @@ def test_backward_of_shared_key_heads(cuda_ops, Bt, L, H, G, P, dtype):
         assert torch.equal(x, y)
 
 
+@pytest.mark.gpu
+def test_two_backwards_at_once_and_captured(cuda_ops):
+    """Two calls on two streams, and both replayed from one graph, give what each gives alone."""
+    work = []
+    for seed, (Bt, L, H, G, P) in ((47, (4, 260, 8, 2, 128)), (48, (3, 200, 6, 6, 64))):
+        a, h0 = make(Bt, L, H, G, 128, P, torch.bfloat16, seed=seed)
+        args, h = on(a), h0.to(dev)
+        dy = torch.randn(Bt, L, H * P, device=dev).bfloat16()
+        _, saved = cuda_ops.gated_delta_rule(*args, h0=h, save=True)
+        work.append((args, dy, saved))
+    alone = [cuda_ops.gated_delta_rule_bwd(*w[0], w[1], w[2]) for w in work]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in work]
+
+    def both():
+        out = []
+        for s, (args, dy, saved) in zip(streams, work):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                out.append(cuda_ops.gated_delta_rule_bwd(*args, dy, saved))
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+        return out
+
+    got = both()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = both()
+    for _ in range(2):
+        for t in (t for o in again for t in o):
+            t.zero_()
+        graph.replay()
+    torch.cuda.synchronize()
+    for one, x, y in zip(alone, got, again):
+        assert all(torch.equal(p, q) and torch.equal(p, r) for p, q, r in zip(one, x, y))
+
+
 def rand(*shape, dtype=torch.float32):
     return torch.randn(*shape, device=dev, dtype=dtype)
 
