@@ -45,13 +45,13 @@ struct FwdArgs {
   int vec_kq, vec_v;
 };
 
-template <int XS, int KN, int NCW, int NS>
+template <int XS, int KN, int NCW>
 __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdArgs a) {
   let_next_start();
   wait_for_previous();
   using T = typename std::conditional<XS == 1, __nv_bfloat16, float>::type;
   using SM = FwdSmem<XS, KN, NCW>;
-  constexpr int PB = SM::PB, RB = KN * 2, NT = KN / 8, NQ = XS == 1 ? 2 : 3;
+  constexpr int PB = SM::PB, RB = KN * 2, NT = KN / 8, NS = 3, NQ = XS == 1 ? 2 : 3;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((128u - (smem_addr(smem_raw) & 127u)) & 127u);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -330,11 +330,11 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
   if (warp < NCW && a.h_out) state_io(a.h_out + srow, nullptr);
 }
 
-template <int XS, int KN, int NCW, int NS>
+template <int XS, int KN, int NCW>
 int launch(FwdArgs a, int64_t Bt, cudaStream_t st) {
   constexpr int bytes = FwdSmem<XS, KN, NCW>::BYTES;
   static_assert(bytes <= 232448, "shared-memory layout exceeds the per-block limit");
-  auto kern = delta_fwd_kernel<XS, KN, NCW, NS>;
+  auto kern = delta_fwd_kernel<XS, KN, NCW>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
     return check_launch("gated_delta_rule: set smem attribute");
   a.npb = (int)cdiv(a.P, 16 * NCW);
@@ -344,11 +344,11 @@ int launch(FwdArgs a, int64_t Bt, cudaStream_t st) {
   return check_launch("gated_delta_rule");
 }
 
-template <int XS, int KN, int NS>
+template <int XS, int KN>
 int by_block(const FwdArgs& a, int64_t Bt, cudaStream_t st) {
   // 128 channels a block when that still fills the SMs, else 64
-  if (a.P > 64 && Bt * a.H * cdiv(a.P, 128) >= num_sms()) return launch<XS, KN, 8, NS>(a, Bt, st);
-  return launch<XS, KN, 4, NS>(a, Bt, st);
+  if (a.P > 64 && Bt * a.H * cdiv(a.P, 128) >= num_sms()) return launch<XS, KN, 8>(a, Bt, st);
+  return launch<XS, KN, 4>(a, Bt, st);
 }
 
 }  // namespace
@@ -428,10 +428,8 @@ extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const voi
     a.h_in = c0 ? carry : (const float*)h0;
     a.h_out = c0 + m == nc && !h_last ? nullptr : carry;
     int e;
-    if (dtype == TSSM_F32) e = N <= 64 ? by_block<3, 64, 3>(a, Bt, st) : by_block<3, 128, 3>(a, Bt, st);
-    // f32 results (the state, what the backward reads) want three planes; y alone is bf16: two
-    else if (h_last || states) e = N <= 64 ? by_block<1, 64, 3>(a, Bt, st) : by_block<1, 128, 3>(a, Bt, st);
-    else e = N <= 64 ? by_block<1, 64, 2>(a, Bt, st) : by_block<1, 128, 2>(a, Bt, st);
+    if (dtype == TSSM_F32) e = N <= 64 ? by_block<3, 64>(a, Bt, st) : by_block<3, 128>(a, Bt, st);
+    else e = N <= 64 ? by_block<1, 64>(a, Bt, st) : by_block<1, 128>(a, Bt, st);
     if (e) return e;
   }
   return TSSM_OK;

@@ -122,14 +122,13 @@ __device__ __forceinline__ void store_planes(uint32_t taddr, uint32_t step, floa
   store_planes<NS>(at, r);
 }
 
-// NS: planes of the state and of X, E (3 when an f32 result is asked for, else 2).
-template <int KN, int NS>
+template <int KN>
 __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constant__ CUtensorMap tm_k,
                                                             const __grid_constant__ CUtensorMap tm_q,
                                                             const __grid_constant__ CUtensorMap tm_u,
                                                             const __grid_constant__ CUtensorMap tm_y, const ScanArgs a) {
   using SM = ScanSmem<KN>;
-  constexpr int NB = SM::NB, HN = KN / 2;   // HN: state columns of a thread
+  constexpr int NB = SM::NB, HN = KN / 2, NS = 3;   // HN: state columns of a thread; NS: planes of the state, X and E
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -861,7 +860,7 @@ bool map_bf16(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int KN, int NS>
+template <int KN>
 int run(const TcCall& a, cudaStream_t st) {
   const int64_t streams = a.Bt * a.H, nc = cdiv(a.L, Q), seg = segment_chunks(streams, nc, 2);
   CUtensorMap mk, mq, mu, my;
@@ -875,7 +874,7 @@ int run(const TcCall& a, cudaStream_t st) {
     set_error("gated_delta_rule: device status word unavailable");
     return TSSM_ERR_CUDA;
   }
-  auto scan = delta_scan_kernel<KN, NS>;
+  auto scan = delta_scan_kernel<KN>;
   if (cudaFuncSetAttribute(scan, cudaFuncAttributeMaxDynamicSharedMemorySize, ScanSmem<KN>::BYTES) != cudaSuccess)
     return check_launch("gated_delta_rule: set smem attribute");
   for (int64_t c0 = 0; c0 < nc; c0 += seg) {
@@ -933,9 +932,7 @@ int tc_back_run(const TcBackCall& a, cudaStream_t st) {
 int tc_run(const TcCall& a, cudaStream_t st) {
   TSSM_REQUIRE(a.Bt * a.H * cdiv(a.P, 128) < (int64_t(1) << 31) && a.H * a.P < (int64_t(1) << 31) && a.G * a.N < (int64_t(1) << 31),
                "gated_delta_rule: size out of range");
-  const bool f32_out = a.h_last || a.states;
-  if (a.N == 64) return f32_out ? run<64, 3>(a, st) : run<64, 2>(a, st);
-  return f32_out ? run<128, 3>(a, st) : run<128, 2>(a, st);
+  return a.N == 64 ? run<64>(a, st) : run<128>(a, st);
 }
 
 }  // namespace delta
