@@ -393,22 +393,20 @@ __device__ __forceinline__ void put4x2(uint8_t* tile, int r, int lane, const flo
   }
 }
 
-// A chunk's image, as it lies in shared memory: T planes, NA planes of Aq diag(beta), gates.
-constexpr int IMG_T = 0, IMG_AQ = 3 * SQ_BYTES;
-__host__ __device__ constexpr int img_gates(int na) { return IMG_AQ + na * SQ_BYTES; }
-__host__ __device__ constexpr int img_bytes(int na) { return img_gates(na) + (int)sizeof(Gates); }
+// A chunk's image, as it lies in shared memory: planes of T and of Aq diag(beta), gates.
+constexpr int IMG_T = 0, IMG_AQ = 3 * SQ_BYTES, IMG_GATES = 6 * SQ_BYTES, IMG_BYTES = IMG_GATES + (int)sizeof(Gates);
 // NTH threads: an image to shared memory.
-template <int NA, int NTH>
+template <int NTH>
 __device__ __forceinline__ void load_image(uint32_t dst, const uint8_t* src, int t) {
 #pragma unroll 4
-  for (int i = t; i < img_bytes(NA) / 16; i += NTH) cp_async16(dst + 16 * i, src + 16 * i, true);
+  for (int i = t; i < IMG_BYTES / 16; i += NTH) cp_async16(dst + 16 * i, src + 16 * i, true);
 }
 
-// 128 threads (t = 0..127): from the loaded K, Q planes and the gates, the planes of
-// Aq diag(beta) (NA of them) and of T (NTP).  M is the f32 work matrix; it may lie over the Q
+// 128 threads (t = 0..127): from the loaded K, Q planes and the gates, the three planes of
+// Aq diag(beta) and of T.  M is the f32 work matrix; it may lie over the Q
 // planes (their product comes first).  Entries of 16-blocks
 // above the diagonal are not written: nobody reads them.
-template <int XS, int KN, int NA, int NTP>
+template <int XS, int KN>
 __device__ __forceinline__ void chunk_matrices(uint32_t k, uint32_t q, const Gates& g, float scale, float* M,
                                                uint8_t* aq, uint8_t* tp, int t, int bar) {
   constexpr int RB = KN * 2, PB = Q * RB, KK = KN / 16;
@@ -463,10 +461,10 @@ __device__ __forceinline__ void chunk_matrices(uint32_t k, uint32_t q, const Gat
           if (pass == 0) {
             *reinterpret_cast<float2*>(M + i * AM + j) = make_float2(v[2 * r], v[2 * r + 1]);
           } else {
-            uint32_t p[NA];
-            split2<NA>(v[2 * r], v[2 * r + 1], p);
+            uint32_t p[3];
+            split2<3>(v[2 * r], v[2 * r + 1], p);
 #pragma unroll
-            for (int s = 0; s < NA; ++s)
+            for (int s = 0; s < 3; ++s)
               *reinterpret_cast<uint32_t*>(aq + s * SQ_BYTES + tile_off<SQ_RB>(i, 2 * J + n) + 2 * q2) = p[s];
           }
         }
@@ -481,13 +479,13 @@ __device__ __forceinline__ void chunk_matrices(uint32_t k, uint32_t q, const Gat
     const int i = 16 * bi + (idx % 32) / 2, c = 2 * bj + idx % 2;
     const float4 x = *reinterpret_cast<const float4*>(M + i * AM + 8 * c);
     const float4 y = *reinterpret_cast<const float4*>(M + i * AM + 8 * c + 4);
-    uint32_t r[4][NTP];
-    split2<NTP>(x.x, x.y, r[0]);
-    split2<NTP>(x.z, x.w, r[1]);
-    split2<NTP>(y.x, y.y, r[2]);
-    split2<NTP>(y.z, y.w, r[3]);
+    uint32_t r[4][3];
+    split2<3>(x.x, x.y, r[0]);
+    split2<3>(x.z, x.w, r[1]);
+    split2<3>(y.x, y.y, r[2]);
+    split2<3>(y.z, y.w, r[3]);
 #pragma unroll
-    for (int s = 0; s < NTP; ++s)
+    for (int s = 0; s < 3; ++s)
       *reinterpret_cast<uint4*>(tp + s * SQ_BYTES + tile_off<SQ_RB>(i, c)) =
           make_uint4(r[0][s], r[1][s], r[2][s], r[3][s]);
   }

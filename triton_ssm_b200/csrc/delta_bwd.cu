@@ -89,7 +89,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(cons
     const uint32_t s = smem_addr(buf);
     const int64_t t0 = (a.c0 + c) * Q;
     const int rows = (int)min((int64_t)Q, a.L - t0);
-    load_image<3, LT>(s + SM::T, a.img + (bh * a.nseg + c) * img_bytes(3), t);
+    load_image<LT>(s + SM::T, a.img + (bh * a.nseg + c) * IMG_BYTES, t);
     load_planes<XS, KN, LT>(s + SM::K, SM::PLANE, kp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
     load_planes<XS, KN, LT>(s + SM::QQ, SM::PLANE, qp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
     load_planes<XS, PB, LT>(s + SM::DO, SM::DO_PLANE, op + t0 * su, su, rows, pvalid, a.vec_v, t);
@@ -738,14 +738,14 @@ int launch_all(BwdArgs a, bool tc, cudaStream_t st) {
     if (int e = tc_back_run(t, st)) return e;
   } else {
     const bool wide = a.P > 64 && a.Bt * a.H * cdiv(a.P, 128) >= num_sms();
-    const int64_t seg = segment_chunks(a.Bt * a.H, a.nc, 3);
+    const int64_t seg = segment_chunks(a.Bt * a.H, a.nc);
     for (int64_t end = a.nc; end > 0; end -= seg) {   // segments from the last; dh0 carries the state's gradient
       a.c0 = std::max<int64_t>(0, end - seg);
       a.nseg = end - a.c0;
       a.ds_in = end == a.nc ? a.dh_last : a.dh0;
       const PrepCall p{a.B, a.C, a.A_log, a.dt, a.beta, a.img, a.gates, a.Bt, a.L, a.H, a.G, a.N, a.c0, a.nseg, a.nc,
                        a.scale, a.vec_kq};
-      if (int e = prep_run(p, XS == 1 ? TSSM_BF16 : TSSM_F32, 3, st)) return e;
+      if (int e = prep_run(p, XS == 1 ? TSSM_BF16 : TSSM_F32, st)) return e;
       if (int e = wide ? launch_chain<XS, KN, 8>(a, st) : launch_chain<XS, KN, 4>(a, st)) return e;
     }
   }
@@ -781,7 +781,7 @@ BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N
   s.derrs = Bt * H * saved_floats(P, L);
   s.part = H == G ? 0 : up(Bt * L * H * N);
   s.da = up(Bt * H * nc);
-  s.img = nc ? Bt * H * segment_chunks(Bt * H, nc, 3) * prep_image_bytes(3) / 4 : 0;
+  s.img = nc ? Bt * H * segment_chunks(Bt * H, nc) * prep_image_bytes() / 4 : 0;
   s.gates = Bt * H * nc * (int64_t)(sizeof(Gates) / 4);
   s.total = s.dstates + s.derrs + 2 * s.part + s.da + s.gates + s.img;
   return s;

@@ -26,10 +26,9 @@ struct FwdSmem {
   static constexpr int BUFS = XS == 1 ? 2 : 1;
   static constexpr int PB = 16 * NCW;                    // value channels of the block
   static constexpr int PLANE = Q * KN * 2;
-  static constexpr int NAQ = XS == 1 ? 2 : 3;            // planes of Aq diag(beta)
   static constexpr int VROW = XS == 1 ? PB * 2 : (PB + 4) * 4;   // f32 values: padded rows
   static constexpr int K = 0, QQ = K + XS * PLANE, V = QQ + XS * PLANE, T = V + Q * VROW, AQ = T + 3 * SQ_BYTES,
-                       G = AQ + NAQ * SQ_BYTES, BUF = (G + (int)sizeof(Gates) + 127) / 128 * 128;   // T, AQ, G: an image
+                       G = AQ + 3 * SQ_BYTES, BUF = (G + (int)sizeof(Gates) + 127) / 128 * 128;   // T, AQ, G: an image
   static constexpr int BYTES = BUFS * BUF + 128;
 };
 
@@ -51,7 +50,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
   wait_for_previous();
   using T = typename std::conditional<XS == 1, __nv_bfloat16, float>::type;
   using SM = FwdSmem<XS, KN, NCW>;
-  constexpr int PB = SM::PB, RB = KN * 2, NT = KN / 8, NS = 3, NQ = XS == 1 ? 2 : 3;
+  constexpr int PB = SM::PB, RB = KN * 2, NT = KN / 8, NS = 3;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + ((128u - (smem_addr(smem_raw) & 127u)) & 127u);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -73,7 +72,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
     const uint32_t s = smem_addr(buf);
     const int64_t t0 = (a.c0 + c) * Q;
     const int rows = (int)min((int64_t)Q, a.L - t0);
-    load_image<SM::NAQ, LT>(s + SM::T, a.img + (bh * a.nseg + c) * img_bytes(SM::NAQ), t);
+    load_image<LT>(s + SM::T, a.img + (bh * a.nseg + c) * IMG_BYTES, t);
     load_planes<XS, KN, LT>(s + SM::K, SM::PLANE, kp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
     load_planes<XS, KN, LT>(s + SM::QQ, SM::PLANE, qp + t0 * sk, sk, rows, a.N, a.vec_kq, t);
     if constexpr (XS == 1) {
@@ -216,14 +215,14 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
       for (int e = 0; e < 4; ++e) x[i][e] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < KN / 16; ++kk) {
-      uint32_t f[NQ][4];
-      split_a<NQ>(S[2 * kk], S[2 * kk + 1], f);
+      uint32_t f[NS][4];
+      split_a<NS>(S[2 * kk], S[2 * kk + 1], f);
 #pragma unroll
       for (int np = 0; np < 4; ++np) {
         uint32_t w[XS][4];
 #pragma unroll
         for (int z = 0; z < XS; ++z) ldsm4(w[z], at_b<RB>(s + SM::QQ + z * SM::PLANE, 16 * np, 2 * kk, lane));
-        mma_planes<NQ, XS, NQ>(x[2 * np], x[2 * np + 1], f, w);
+        mma_planes<NS, XS, NS>(x[2 * np], x[2 * np + 1], f, w);
       }
     }
 #pragma unroll
@@ -236,14 +235,14 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
     }
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      uint32_t f[NQ][4];
-      split_a<NQ>(er[2 * t], er[2 * t + 1], f);
+      uint32_t f[NS][4];
+      split_a<NS>(er[2 * t], er[2 * t + 1], f);
 #pragma unroll
       for (int np = t; np < 4; ++np) {
-        uint32_t w[NQ][4];
+        uint32_t w[NS][4];
 #pragma unroll
-        for (int z = 0; z < NQ; ++z) ldsm4(w[z], at_b<SQ_RB>(s + SM::AQ + z * SQ_BYTES, 16 * np, 2 * t, lane));
-        mma_planes<NQ, NQ, NQ>(x[2 * np], x[2 * np + 1], f, w);
+        for (int z = 0; z < NS; ++z) ldsm4(w[z], at_b<SQ_RB>(s + SM::AQ + z * SQ_BYTES, 16 * np, 2 * t, lane));
+        mma_planes<NS, NS, NS>(x[2 * np], x[2 * np + 1], f, w);
       }
     }
     // y: through this warp's own columns of the value tile (bf16), one 16-byte piece a lane
@@ -360,9 +359,8 @@ extern "C" int64_t tssm_gated_delta_rule_workspace_size(int64_t Bt, int64_t L, i
   using namespace tssm;
   using namespace tssm::delta;
   if (Bt <= 0 || L <= 0 || H <= 0 || G <= 0 || P <= 0 || N <= 0) return 0;
-  const int na = dtype == TSSM_F32 ? 3 : 2;
-  const int64_t streams = Bt * H, nc = cdiv(L, delta::Q), seg = segment_chunks(streams, nc, na);
-  return streams * seg * prep_image_bytes(na) + (seg < nc ? streams * P * N * 4 : 0);
+  const int64_t streams = Bt * H, nc = cdiv(L, delta::Q), seg = segment_chunks(streams, nc);
+  return streams * seg * prep_image_bytes() + (seg < nc ? streams * P * N * 4 : 0);
 }
 
 extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const void* B, const void* C, const void* dt,
@@ -392,7 +390,6 @@ extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const voi
   TSSM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
                "gated_delta_rule: workspace of %lld bytes (16-byte aligned) needed, %lld given", (long long)need,
                (long long)workspace_bytes);
-  const int na = dtype == TSSM_F32 ? 3 : 2;
   const int64_t streams = Bt * H, nc = cdiv(L, delta::Q);
   if (nc == 0) {   // no tokens: the state passes through
     if (!h_last || h_last == h0) return TSSM_OK;
@@ -402,9 +399,9 @@ extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const voi
       return check_launch("gated_delta_rule: pass the state");
     return TSSM_OK;
   }
-  const int64_t seg = segment_chunks(streams, nc, na);
+  const int64_t seg = segment_chunks(streams, nc);
   uint8_t* img = (uint8_t*)workspace;
-  float* carry = h_last ? (float*)h_last : (float*)(img + streams * seg * prep_image_bytes(na));
+  float* carry = h_last ? (float*)h_last : (float*)(img + streams * seg * prep_image_bytes());
   if (tc_takes(P, N, dtype) && (bases & 15u) == 0) {
     const TcCall t{u, B, C, (const float*)A_log, (const float*)dt, (const float*)beta, (const float*)h0, y,
                    (float*)h_last, (float*)states, (float*)errors, img, carry, Bt, L, H, G, P, N, (float)scale};
@@ -423,7 +420,7 @@ extern "C" int tssm_gated_delta_rule(const void* u, const void* A_log, const voi
     const int64_t m = std::min(seg, nc - c0);
     const PrepCall p{B, C, (const float*)A_log, (const float*)dt, (const float*)beta, img, nullptr, Bt, L, H, G, N, c0,
                      m, nc, (float)scale, a.vec_kq};
-    if (int e = prep_run(p, dtype, na, st)) return e;
+    if (int e = prep_run(p, dtype, st)) return e;
     a.c0 = c0; a.nseg = m;
     a.h_in = c0 ? carry : (const float*)h0;
     a.h_out = c0 + m == nc && !h_last ? nullptr : carry;

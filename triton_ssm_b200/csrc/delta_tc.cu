@@ -9,23 +9,25 @@
 //   X^T  = V^T - exp(l) KS^T    threads: TMEM -> registers -> X planes (TMEM)
 //   E^T  = X^T T^T              A: X planes, B: T planes, 16-column steps of the triangle
 //   S^T  = exp(l_last) S^T + (E diag(w beta))^T K   (S in f32 registers, the sum from TMEM)
-//   O^T  = scale exp(l) S^T Q^T + E^T (Aq diag(beta))^T   (two planes: y is bf16)
+//   O^T  = scale exp(l) S^T Q^T + E^T (Aq diag(beta))^T
 // Warps: 0 issues the chain's products, 2 those of O, 1 copies, 4-11 are the chain (two
 // per 32 lanes, each half of the columns: S 64 f32 a thread), 12-15 the outputs.  The
 // chain is serial, so its latency counts: pieces of its operands are handed over as
 // they are written, by named barriers (a hand-over through an mbarrier measured 136
 // cycles, through a barrier 25), and a product runs while the next piece is split.
 // tcgen05 takes 32 cycles per 128 x 64 x 16 and 190 from issue to a thread that waits.
-// Measured: 3.2 us a chunk (N = P = 128; 113 us for 2 x 2048 tokens x 16 heads, where the
-// tensor pipe is busy 45 % of the time on the SMs that have a block); four chain warps per
-// 32 lanes, a quarter of the columns each, took 3.8: they slow the issuing warps down.
+// Measured: 3.7 us a chunk (N = P = 128; 118 us for 2 x 2048 tokens x 16 heads).  With two
+// planes for O it is 3.5, but one y in 450 then misses the nearest bf16 value (one in 5000
+// with three).  Holding the third plane's QS back until X is made gained nothing.  Four chain
+// warps per 32 lanes, a quarter of the columns each, were a fifth slower than two: they slow
+// the issuing warps down.
 // States and errors for a backward, stored a quarter at a time between the steps: 4.4 us a chunk
 // (4.6 in one go).  Those sequences took 317 us in all on the register chain, 136 here.
 //
 // TMEM columns: [0, 192) S planes (planes 0, 1 of a half side by side, then both plane
 // 2s), later the state update's sum over planes 0, 1.  [192, 256) KS.  [256, 352) X
-// planes, then E diag(w beta) planes, 48 per half.  [352, 416) E, then its two planes
-// for O.  [416, 480) QS, then O.  A thread overwrites columns of
+// planes, then E diag(w beta) planes, 48 per half.  [352, 416) E, then its planes 0, 1
+// for O; [480, 512) plane 2.  [416, 480) QS, then O.  A thread overwrites columns of
 // its own lane and half only, so only products are waited for.
 //
 // Loops are left rolled where registers allow: unrolled (130 KB of code) the warps
@@ -48,10 +50,9 @@ namespace {
 using namespace sm100;
 
 constexpr int TILE = 8192;                       // [64 x 64] bf16
-constexpr int IMG = img_bytes(2), IMG_EG = img_gates(2) + (int)offsetof(Gates, eg);      // forward
-constexpr int IMG3 = img_bytes(3), IMG3_EG = img_gates(3) + (int)offsetof(Gates, eg);    // backward: all of Aq
+constexpr int IMG = IMG_BYTES, IMG_EG = IMG_GATES + (int)offsetof(Gates, eg);
 constexpr int EG_TO_WB = (int)(offsetof(Gates, wb) - offsetof(Gates, eg)) / 4;
-static_assert(IMG % 16 == 0 && IMG3 % 16 == 0 && IMG_EG % 16 == 0, "bulk copies, 16-byte reads");
+static_assert(IMG % 16 == 0 && IMG_EG % 16 == 0, "bulk copies, 16-byte reads");
 
 // ------------------------------------------------------------------ the scan
 struct ScanArgs {
@@ -72,7 +73,7 @@ struct ScanSmem {
   static_assert(BYTES <= 232448, "shared-memory layout exceeds the per-block limit");
 };
 
-constexpr uint32_t C_KS = 192, C_XP = 256, C_E = 352, C_O = 416;
+constexpr uint32_t C_KS = 192, C_XP = 256, C_E = 352, C_O = 416, C_E2 = 480;
 // named barriers (0: __syncthreads): outputs; pieces of S, X, E diag(w beta), E for their issuers
 constexpr uint32_t B_OUT = 1, B_S = 2, B_X = 6, B_W = 8, B_E = 10, B_ISSUE = 256 + 32;
 
@@ -298,8 +299,12 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
               ep[j / 4 * a.P] = make_float4(x[j >> 4][j & 15], x[j >> 4][(j + 1) & 15], x[j >> 4][(j + 2) & 15],
                                             x[j >> 4][(j + 3) & 15]);
         }
-        store_planes<2>(tl + C_E + 32 * half, 16, x[0]);
-        store_planes<2>(tl + C_E + 32 * half + 8, 16, x[1]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t at[NS] = {tl + C_E + 32 * half + 8 * i, tl + C_E + 32 * half + 16 + 8 * i,
+                                   tl + C_E2 + 16 * half + 8 * i};
+          store_planes<NS>(at, x[i]);
+        }
       }
       hand_over(B_E);
       save(3);
@@ -463,10 +468,10 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
 #pragma unroll 1
         for (int kk = 0; kk < KN / 16; ++kk)
 #pragma unroll
-          for (int s = 1; s >= 0; --s)
+          for (int s = NS - 1; s >= 0; --s)
             umma_bf16_ta(tmem + C_O, tmem + plane(s, kk / (HN / 16)) + 8 * (kk % (HN / 16)),
                          make_desc_sw128(st + SM::QQ + (kk / 4) * TILE, 16) + 2 * (kk & 3),
-                         make_idesc_bf16(128, 64, false, false), s != 1 || kk);
+                         make_idesc_bf16(128, 64, false, false), s != NS - 1 || kk);
       umma_commit_warp(qdone);
       take(B_E);
       ok = ok && waitw(qread, c, 2015);
@@ -474,10 +479,10 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
 #pragma unroll 1
         for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int o = 1; o >= 0; --o)
+          for (int o = NS - 1; o >= 0; --o)
 #pragma unroll
             for (int s = 0; s <= o; ++s)
-              umma_bf16_ta(tmem + C_O + 16 * t, tmem + C_E + 32 * (t >> 1) + 16 * s + 8 * (t & 1),
+              umma_bf16_ta(tmem + C_O + 16 * t, tmem + (s < 2 ? C_E + 32 * (t >> 1) + 16 * s : C_E2 + 16 * (t >> 1)) + 8 * (t & 1),
                            make_desc_sw128(st + SM::IM + IMG_AQ + (o - s) * SQ_BYTES, 16) + 130 * t,
                            make_idesc_bf16(128, 64 - 16 * t, false, false), true);   // onto scale exp(l) QS
       umma_commit_warp(odone);
@@ -521,7 +526,7 @@ template <int KN>
 struct BackSmem {
   static constexpr int NB = KN / 64;
   static constexpr int K = 0, QQ = K + NB * TILE, DO = QQ + NB * TILE, IM = DO + 2 * TILE,
-                       STAGE = (IM + IMG3 + 1023) / 1024 * 1024;
+                       STAGE = (IM + IMG + 1023) / 1024 * 1024;
   static constexpr int BAR = 2 * STAGE, BYTES = BAR + 256 + 1024;
   static_assert(BYTES <= 232448, "shared-memory layout exceeds the per-block limit");
 };
@@ -614,7 +619,7 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
       const int64_t cc = a.c0 + n - 1 - k;
       const uint8_t* st = stage(k);
       ok = ok && waitw(&full[k & 1], k >> 1, 2102);
-      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG3_EG) + 32 * half;
+      const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_EG) + 32 * half;
       const float* wb = eg + EG_TO_WB;
       const float el = (eg - 32 * half)[Q - 1];
       const uint16_t* os = reinterpret_cast<const uint16_t*>(st + SM::DO + (p >> 6) * TILE) + (p & 63) + half * 32 * 64;
@@ -737,7 +742,7 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
   } else if (warp == 1) {
     // ================================================================ copies
     if (lane == 0) {
-      const uint32_t bytes = 2 * NB * TILE + boxes * TILE + IMG3;
+      const uint32_t bytes = 2 * NB * TILE + boxes * TILE + IMG;
       for (int k = 0; k < n; ++k) {
         if (k >= 2 && !mbar_wait(&empty[k & 1], ((k >> 1) - 1) & 1, abort_flag)) {
           if (!*abort_flag) fail(2109);
@@ -754,7 +759,7 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
         for (int x = 0; x < boxes; ++x) tma_load_3d(st + SM::DO + x * TILE, &tm_o, h * a.P + pb + 64 * x, t0, b, f);
         asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
                          smem_u32(st + SM::IM)),
-                     "l"(a.img + (bh * a.nseg + c) * IMG3), "r"(IMG3), "r"(smem_u32(f))
+                     "l"(a.img + (bh * a.nseg + c) * IMG), "r"(IMG), "r"(smem_u32(f))
                      : "memory");
         *issued = k + 1;
       }
@@ -862,7 +867,7 @@ bool map_bf16(CUtensorMap* m, const void* base, uint64_t d0, uint64_t d1, uint64
 
 template <int KN>
 int run(const TcCall& a, cudaStream_t st) {
-  const int64_t streams = a.Bt * a.H, nc = cdiv(a.L, Q), seg = segment_chunks(streams, nc, 2);
+  const int64_t streams = a.Bt * a.H, nc = cdiv(a.L, Q), seg = segment_chunks(streams, nc);
   CUtensorMap mk, mq, mu, my;
   if (!map_bf16(&mk, a.B, a.G * a.N, a.L, a.Bt, true) || !map_bf16(&mq, a.C, a.G * a.N, a.L, a.Bt, true) ||
       !map_bf16(&mu, a.u, a.H * a.P, a.L, a.Bt, false) || !map_bf16(&my, a.y, a.H * a.P, a.L, a.Bt, false)) {
@@ -880,7 +885,7 @@ int run(const TcCall& a, cudaStream_t st) {
   for (int64_t c0 = 0; c0 < nc; c0 += seg) {
     const int64_t m = std::min(seg, nc - c0);
     const PrepCall p{a.B, a.C, a.A_log, a.dt, a.beta, a.img, nullptr, a.Bt, a.L, a.H, a.G, a.N, c0, m, nc, a.scale, 1};
-    if (int e = prep_run(p, TSSM_BF16, 2, st)) return e;
+    if (int e = prep_run(p, TSSM_BF16, st)) return e;
     const bool last = c0 + m == nc;
     const ScanArgs s{a.img, c0 ? a.carry : a.h0, last && !a.h_last ? nullptr : a.carry, a.states, a.errs, status, a.L,
                      c0, m, nc, (int)a.H, (int)a.G, (int)a.P, (int)a.N, (int)cdiv(a.P, 128), a.scale};
@@ -891,7 +896,7 @@ int run(const TcCall& a, cudaStream_t st) {
 
 template <int KN>
 int run_back(const TcBackCall& a, cudaStream_t st) {
-  const int64_t streams = a.Bt * a.H, nc = cdiv(a.L, Q), seg = segment_chunks(streams, nc, 3);
+  const int64_t streams = a.Bt * a.H, nc = cdiv(a.L, Q), seg = segment_chunks(streams, nc);
   CUtensorMap mk, mq, mo;
   if (!map_bf16(&mk, a.B, a.G * a.N, a.L, a.Bt, true) || !map_bf16(&mq, a.C, a.G * a.N, a.L, a.Bt, true) ||
       !map_bf16(&mo, a.dy, a.H * a.P, a.L, a.Bt, false)) {
@@ -909,7 +914,7 @@ int run_back(const TcBackCall& a, cudaStream_t st) {
   for (int64_t end = nc; end > 0; end -= seg) {   // segments from the last; dh0 carries the state's gradient
     const int64_t c0 = std::max<int64_t>(0, end - seg), m = end - c0;
     const PrepCall p{a.B, a.C, a.A_log, a.dt, a.beta, a.img, a.gates, a.Bt, a.L, a.H, a.G, a.N, c0, m, nc, a.scale, 1};
-    if (int e = prep_run(p, TSSM_BF16, 3, st)) return e;
+    if (int e = prep_run(p, TSSM_BF16, st)) return e;
     const BackArgs s{a.img, end == nc ? a.dh_last : a.dh0, a.dh0, a.dstates, a.derrs, status, a.L,
                      c0, m, nc, (int)a.H, (int)a.G, (int)a.P, (int)a.N, (int)cdiv(a.P, 128), a.scale};
     scan<<<(unsigned)(streams * s.npb), 384, BackSmem<KN>::BYTES, st>>>(mk, mq, mo, s);

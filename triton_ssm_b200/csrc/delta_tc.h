@@ -16,10 +16,9 @@ struct PrepCall {
   float scale;
   int vec;       // N and the bases allow 16-byte pieces
 };
-int prep_run(const PrepCall& a, int dtype, int na, cudaStream_t st);   // na planes of Aq: 2 (bf16 y) or 3 (f32)
-int64_t prep_image_bytes(int na);
-int64_t prep_gates_bytes();
-int64_t segment_chunks(int64_t streams, int64_t nc, int na);   // chunks whose images are made at a time
+int prep_run(const PrepCall& a, int dtype, cudaStream_t st);
+int64_t prep_image_bytes();
+int64_t segment_chunks(int64_t streams, int64_t nc);   // chunks whose images are made at a time
 
 // delta_tc.cu: the scans on tcgen05 (bf16, N 64 or 128, P a multiple of 64, 16-byte aligned tensors).
 struct TcCall {
