@@ -59,3 +59,37 @@ def test_y_is_rounded_once(cuda_ops, part, N, P):
     mag = scale * q * (s.abs() + b * (v.abs() + s.abs() * k) * k)
     d = (y.double().cpu().view_as(ref) - ref).abs() - half_step(ref)
     assert bool((d <= 2.0 ** -19 * mag).all()), "%d of %d values beyond" % (int((d > 2.0 ** -19 * mag).sum()), d.numel())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,P", [(128, 128), (64, 64), (24, 40)])
+def test_key_and_query_gradients_are_rounded_once(cuda_ops, N, P):
+    """Two tokens, k_0 on the first half of the coordinates, k_1 and q_1 on one of the second half, dy only for
+    token 1 and channel p, no decay: on the first half dC_1 = scale beta_0 dy u_0p k_0 and
+    dB_1 = -beta_0 beta_1 scale (q_1 k_1) dy u_0p k_0.  Every product on the way has one term, so that the values
+    before their rounding are off by about 30 f32 roundings of 2^-24: 2^-19.  Factors held to 16 bits would be off
+    by up to 2^-18."""
+    Bt, H, n, p, scale = 512, 8, N - 3, P - 7, 0.75
+    g = torch.Generator().manual_seed(N)
+
+    def rand(*shape):
+        return torch.rand(*shape, generator=g).add(0.5).bfloat16()
+
+    u, dy = torch.randn(Bt, 2, H, P, generator=g).bfloat16(), torch.zeros(Bt, 2, H, P).bfloat16()
+    dy[:, 1, :, p] = rand(Bt, H)
+    B, C = torch.zeros(Bt, 2, H, N).bfloat16(), torch.zeros(Bt, 2, H, N).bfloat16()
+    B[:, 0, :, :N // 2] = rand(Bt, H, N // 2)
+    B[:, 1, :, n], C[:, 1, :, n] = rand(Bt, H), rand(Bt, H)
+    beta = torch.rand(Bt, 2, H, generator=g)
+    args = (u.flatten(2).to(dev), torch.zeros(H, device=dev), B.to(dev), C.to(dev), torch.zeros(Bt, 2, H, device=dev),
+            beta.to(dev))
+    _, saved = cuda_ops.gated_delta_rule(*args, scale=scale, save=True)
+    grads = cuda_ops.gated_delta_rule_bwd(*args, dy.flatten(2).to(dev), saved, scale=scale)
+    b = beta.double()
+    m1 = scale * b[:, 0] * dy[:, 1, :, p].double() * u[:, 0, :, p].double()
+    m2 = m1 * b[:, 1] * B[:, 1, :, n].double() * C[:, 1, :, n].double()
+    k0 = B[:, 0, :, :N // 2].double()
+    for name, x, ref in (("dC", grads[3], m1[..., None] * k0), ("dB", grads[2], -m2[..., None] * k0)):
+        d = (x[:, 1, :, :N // 2].double().cpu() - ref).abs() - half_step(ref)
+        bad = d > 2.0 ** -19 * ref.abs()
+        assert not bool(bad.any()), "%s: %d of %d values beyond" % (name, int(bad.sum()), d.numel())

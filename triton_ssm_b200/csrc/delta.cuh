@@ -11,9 +11,9 @@
 // beta multiplies columns only, so that nothing is ever divided by it.
 //
 // Precision: a matrix product on the tensor cores takes bf16 operands.  An f32
-// operand is split into 2 or 3 bf16 planes (8 bits each, 3 planes are exact to
-// f32) and the products of planes i + j < planes are summed in f32: the state,
-// the errors and every f32 result keep f32 accuracy; bf16 inputs are one plane.
+// operand is split into three bf16 planes (8 bits each: exact to f32) and the
+// products of planes i + j < 3 are summed in f32: every result has f32 accuracy,
+// a bf16 one is then rounded once; bf16 inputs are one plane.
 #pragma once
 #include "common.cuh"
 

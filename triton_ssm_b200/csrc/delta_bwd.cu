@@ -24,10 +24,10 @@
 // summed last, in a fixed order, so results repeat bit for bit.
 //
 // Measured at 4 x 2048 tokens x 16 heads on 8 key heads, N = P = 128, bf16 (with the
-// forward 0.62 ms): images 40 us, chain 151, gradients with du and the key heads' sums 262,
-// dA_log 3.  The gradient kernel here took 384 for them and 38 for the key heads: it has 11 products of
-// 64-wide tiles in 2 or 3 planes a pair, its mma.sync pipe is busy 38 % of the time, and the
-// loads of its one block an SM are exposed.
+// forward 0.64 ms): images 40 us, chain 153, gradients with du and the key heads' sums 270,
+// dA_log 3.  The gradient kernel here took 384 for them and 38 for the key heads (M1, M2 in two
+// planes then): it has 11 products of 64-wide tiles in up to three planes, its mma.sync pipe is
+// busy 38 % of the time, and the loads of its one block an SM are exposed.
 #include "delta.cuh"
 #include "delta_tc.h"
 
@@ -275,7 +275,6 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(cons
 template <int XS, int KN>
 struct GradSmem {
   static constexpr int PLANE = Q * KN * 2;        // of K, Q, and of 64 state rows
-  static constexpr int NMP = XS == 1 ? 2 : 3;     // planes of M1, M2: they end in dQ, dK only
   static constexpr int K = 0, QQ = K + XS * PLANE, DO = QQ + XS * PLANE, E = DO + XS * SQ_BYTES, DE = E + 3 * SQ_BYTES,
                        S = DE + 3 * SQ_BYTES, G = S + 3 * PLANE, VEC = G + (int)sizeof(Gates);
   static constexpr int M1 = E, M2 = DE;           // after the channel loop
@@ -506,12 +505,12 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
           u2[e] = f2 * gt.beta[jj];
           Y[i * 65 + jj] = yy[e];
         }
-        uint32_t p1[SM::NMP], p2[SM::NMP];
-        split2<SM::NMP>(u1[0], u1[1], p1);
-        split2<SM::NMP>(u2[0], u2[1], p2);
+        uint32_t p1[3], p2[3];
+        split2<3>(u1[0], u1[1], p1);
+        split2<3>(u2[0], u2[1], p2);
         const uint32_t off = tile_off<SQ_RB>(i, 2 * qt + nt) + 2 * q2;
 #pragma unroll
-        for (int z = 0; z < SM::NMP; ++z) {
+        for (int z = 0; z < 3; ++z) {
           *reinterpret_cast<uint32_t*>(smem + SM::M1 + z * SQ_BYTES + off) = p1[z];
           *reinterpret_cast<uint32_t*>(smem + SM::M2 + z * SQ_BYTES + off) = p2[z];
         }
@@ -521,11 +520,9 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
   __syncthreads();
   // dQ += M1 K;  dK += M1^T Q - M2 K - M2^T K   (lower triangles: 16-blocks i >= j)
   zero(dk1);
-  constexpr int NMP = SM::NMP;
-  constexpr int NM = XS == 1 ? NMP : 3;
 #pragma unroll 1
   for (int t = 0; t < 4; ++t) {
-    uint32_t f[NMP][4], w[XS][4], w2[XS][4];
+    uint32_t f[3][4], w[XS][4], w2[XS][4];
 #pragma unroll
     for (int nn = 0; nn < NTQ / 2; ++nn) {
 #pragma unroll
@@ -535,20 +532,20 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
       }
       if (t <= mt) {   // rows i = 16 mt, k = j = 16 t
 #pragma unroll
-        for (int z = 0; z < NMP; ++z) ldsm4(f[z], at_a<SQ_RB>(s + SM::M1 + z * SQ_BYTES, 16 * mt, 2 * t, lane));
-        mma_planes<NMP, XS, NM>(dq0[2 * nn], dq0[2 * nn + 1], f, w);
+        for (int z = 0; z < 3; ++z) ldsm4(f[z], at_a<SQ_RB>(s + SM::M1 + z * SQ_BYTES, 16 * mt, 2 * t, lane));
+        mma_planes<3, XS, 3>(dq0[2 * nn], dq0[2 * nn + 1], f, w);
 #pragma unroll
-        for (int z = 0; z < NMP; ++z) ldsm4(f[z], at_a<SQ_RB>(s + SM::M2 + z * SQ_BYTES, 16 * mt, 2 * t, lane));
-        mma_planes<NMP, XS, NM>(dk1[2 * nn], dk1[2 * nn + 1], f, w);
+        for (int z = 0; z < 3; ++z) ldsm4(f[z], at_a<SQ_RB>(s + SM::M2 + z * SQ_BYTES, 16 * mt, 2 * t, lane));
+        mma_planes<3, XS, 3>(dk1[2 * nn], dk1[2 * nn + 1], f, w);
       }
       if (t >= mt) {   // rows j = 16 mt, k = i = 16 t: the transposes
         const uint32_t off = tile_off<SQ_RB>(16 * t + ((lane >> 4) << 3) + (lane & 7), 2 * mt + ((lane >> 3) & 1));
 #pragma unroll
-        for (int z = 0; z < NMP; ++z) ldsm4t(f[z], s + SM::M1 + z * SQ_BYTES + off);
-        mma_planes<NMP, XS, NM>(dk0[2 * nn], dk0[2 * nn + 1], f, w2);
+        for (int z = 0; z < 3; ++z) ldsm4t(f[z], s + SM::M1 + z * SQ_BYTES + off);
+        mma_planes<3, XS, 3>(dk0[2 * nn], dk0[2 * nn + 1], f, w2);
 #pragma unroll
-        for (int z = 0; z < NMP; ++z) ldsm4t(f[z], s + SM::M2 + z * SQ_BYTES + off);
-        mma_planes<NMP, XS, NM>(dk1[2 * nn], dk1[2 * nn + 1], f, w);
+        for (int z = 0; z < 3; ++z) ldsm4t(f[z], s + SM::M2 + z * SQ_BYTES + off);
+        mma_planes<3, XS, 3>(dk1[2 * nn], dk1[2 * nn + 1], f, w);
       }
     }
   }

@@ -6,7 +6,7 @@
 //   dQ0^T = S0^T dO^T        dK0^T = S0^T dE^T       dK1^T = dS1^T E^T       (64 value channels a step)
 //   dQ^T  = scale exp(l) dQ0^T + K^T M1^T
 //   dK^T  = w beta dK1^T - exp(l) dK0^T + Q^T M1 - K^T M2^T - K^T M2
-// with S0, dS1, E, dE in three bf16 planes (products of planes i + j < 3) and M1, M2 in two.  The
+// with S0, dS1, E, dE, M1 and M2 in three bf16 planes (products of planes i + j < 3).  The
 // state parts are scaled in place, so that the last line's products add onto them.  dO E^T and
 // dE E^T (triangles of 64 x 64, in registers), q.k and k.k stay on mma.sync, which runs meanwhile.
 //
@@ -15,7 +15,7 @@
 // Blocks of one key head are a cluster: each leaves its dQ, dK in shared memory and sums a share
 // of the rows over all of them, in the heads' order (parts in HBM and a kernel for their sums took
 // 65 us more at 64 heads x 2048 tokens).
-// Measured there (2048 chunks and heads, P = 128, 16 value on 8 key heads): 262 us, 18 us for one on
+// Measured there (2048 chunks and heads, P = 128, 16 value on 8 key heads): 270 us, 18 us for one on
 // its SM, against 27 on mma.sync.  Bound by shared memory: a 128 x 64 x 16 product reads 6 KB for
 // its 32 cycles, and planes, fragments and sums take about as many cycles again.  Fetching the next
 // blocks' states to L2 ahead made it slower (311): their own loads queued behind that.
@@ -36,7 +36,7 @@ constexpr int NT = 256, N = 128, TILE = SQ_BYTES, PLANE = 2 * TILE;   // a plane
 constexpr int S = 0, E = S + 3 * PLANE, DE = E + 3 * TILE, DO = DE + 3 * TILE, G = DO + TILE,
               VEC = G + (int)sizeof(Gates), BAR = VEC + (3 * 4 * Q + 4 * Q + 8) * 4, BYTES = BAR + 64 + 1024;
 constexpr int K = DE, QQ = K + PLANE;                            // when the last channels' dE, dO have been read
-constexpr int M1 = S, M2 = S + 2 * TILE, Y = S + 4 * TILE;       // after the products over p; Y: 64 x 65 floats
+constexpr int M1 = S, M2 = S + 3 * TILE, Y = S + 6 * TILE;       // after the products over p; Y: 64 x 65 floats
 constexpr int OUT = S;                                           // last: dQ, dK [64][128] f32
 static_assert(QQ + PLANE == G && Y + Q * 65 * 4 <= K && OUT + 2 * Q * N * 4 <= G && BAR % 8 == 0, "regions");
 static_assert(2 * (BYTES + 1024) <= 233472, "two blocks an SM");
@@ -293,12 +293,12 @@ __global__ void __launch_bounds__(NT, 2) delta_grad_tc_kernel(const TcGradCall a
           u1[e] = f1 * gt.beta[jj];
           u2[e] = -f2 * gt.beta[jj];
         }
-        uint32_t p1[2], p2[2];
-        split2<2>(u1[0], u1[1], p1);
-        split2<2>(u2[0], u2[1], p2);
+        uint32_t p1[3], p2[3];
+        split2<3>(u1[0], u1[1], p1);
+        split2<3>(u2[0], u2[1], p2);
         const uint32_t off = tile_off<SQ_RB>(i, 4 * qh + 2 * x + nt) + 2 * q2;
 #pragma unroll
-        for (int z = 0; z < 2; ++z) {
+        for (int z = 0; z < 3; ++z) {
           *reinterpret_cast<uint32_t*>(smem + M1 + z * TILE + off) = p1[z];
           *reinterpret_cast<uint32_t*>(smem + M2 + z * TILE + off) = p2[z];
         }
@@ -356,7 +356,7 @@ __global__ void __launch_bounds__(NT, 2) delta_grad_tc_kernel(const TcGradCall a
       for (int kk = 0; kk < 4; ++kk) {
         const uint64_t k = make_desc_sw128(s + K, TILE) + 128 * kk, q = make_desc_sw128(s + QQ, TILE) + 128 * kk;
 #pragma unroll
-        for (int z = 1; z >= 0; --z) {
+        for (int z = 2; z >= 0; --z) {
           const uint64_t p1 = make_desc_sw128(s + M1 + z * TILE, 16), p2 = make_desc_sw128(s + M2 + z * TILE, 16);
           umma_bf16(tmem + C_Q, k, p1 + 2 * kk, ID, true);
           umma_bf16(tmem + C_K, q, p1 + 128 * kk, IDT, true);
