@@ -33,7 +33,8 @@ def _nvcc():
 
 
 def _headers():
-    return glob.glob(os.path.join(CSRC, "*.cuh")) + glob.glob(os.path.join(ROOT, "include", "*.h"))
+    return [h for p in (os.path.join(CSRC, "*.cuh"), os.path.join(CSRC, "*.h"), os.path.join(ROOT, "include", "*.h"))
+            for h in glob.glob(p)]
 
 
 def _stale(src, obj, hdr_mtime):
