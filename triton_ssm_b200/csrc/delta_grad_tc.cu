@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(NT, 2) delta_grad_tc_kernel(const TcGradCall a
       }
 #pragma unroll
     for (int i = 0; i < 4; ++i) fetch(a.states, p0, i, fs[i]);
-    if (it) wait(bdone, it - 1, 2101);
+    if (it) wait(bdone, it - 1, 3201);
     load_planes<1, 64, NT>(s + DO, 0, (const T*)a.dy + tok + p0, su, rows, 64, true, tid);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(NT, 2) delta_grad_tc_kernel(const TcGradCall a
         mma_planes<3, 3, 3>(m2[2 * x], m2[2 * x + 1], fe, w);
       }
     }
-    wait(adone, it, 2102);
+    wait(adone, it, 3202);
 #pragma unroll
     for (int i = 0; i < 4; ++i) put(i, fd[i]);   // dS1 takes S0's place
     fence_proxy_async_smem();
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(NT, 2) delta_grad_tc_kernel(const TcGradCall a
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
   if (lane == 0) red[warp] = dot;
-  wait(bdone, steps - 1, 2103);
+  wait(bdone, steps - 1, 3203);
   cp_async_wait_all();
   __syncthreads();
   // q.k and k.k of this warp's 16 x 32 block, then M1, -M2 (planes) and Y
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(NT, 2) delta_grad_tc_kernel(const TcGradCall a
     __syncthreads();
     if (lane == 0) red[warp] = da;
   }
-  wait(mdone, 0, 2104);
+  wait(mdone, 0, 3204);
   __syncthreads();   // Y has been read, M1 and M2 by the products
   // dQ, dK in f32, then the sums over the key head's value heads, in their order: this block's share of the rows
   float* out = reinterpret_cast<float*>(smem + OUT);

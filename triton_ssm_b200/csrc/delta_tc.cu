@@ -239,12 +239,12 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       save(0);
       // X^T = V^T - exp(l) KS^T, 32 tokens of this half
       const uint8_t* st = stage(c);
-      ok = ok && waitw(&full[c & 1], c >> 1, 2002);
+      ok = ok && waitw(&full[c & 1], c >> 1, 3002);
       const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_EG) + 32 * half;
       const float* wb = eg + EG_TO_WB;
       const float el = (eg - 32 * half)[Q - 1];
       const uint16_t* vs = reinterpret_cast<const uint16_t*>(st + SM::V + (p >> 6) * TILE) + (p & 63) + half * 32 * 64;
-      ok = ok && waitw(ksdone, c, 2003);
+      ok = ok && waitw(ksdone, c, 3003);
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         float x[16];
@@ -265,7 +265,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       }
       save(1);
       // E^T: planes of E diag(w beta) for the state
-      ok = ok && waitw(edone, c, 2004);
+      ok = ok && waitw(edone, c, 3004);
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         float x[16];
@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       hand_over(B_E);
       save(3);
       // S^T
-      ok = ok && waitw(dsdone, c, 2005);
+      ok = ok && waitw(dsdone, c, 3005);
 #pragma unroll
       for (int i = 0; i < HN / 16; ++i) {
         float d[16];
@@ -330,7 +330,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
     for (int c = 0; c < n; ++c) {
       const uint8_t* st = stage(c);
       // scale exp(l) QS^T goes back to its columns, where Aq diag(beta) E is added
-      bool bad = !waitw(&full[c & 1], c >> 1, 2006) || !waitw(qdone, c, 2007);
+      bool bad = !waitw(&full[c & 1], c >> 1, 3006) || !waitw(qdone, c, 3007);
       const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_EG);
       if (!bad) {
 #pragma unroll 1
@@ -349,7 +349,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
         }
         tmem_wait_st();
         arrive_warp(qread);
-        bad = !waitw(odone, c, 2008);
+        bad = !waitw(odone, c, 3008);
       }
       if (tid == 384 && c > 0) bulk_wait_read<0>();   // the last chunk's store has left the tile
       if (named_bar_or(B_OUT, 128, bad)) break;
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       const uint32_t bytes = 2 * NB * TILE + boxes * TILE + IMG;
       for (int c = 0; c < n; ++c) {
         if (c >= 2 && !mbar_wait(&empty[c & 1], ((c >> 1) - 1) & 1, abort_flag)) {
-          if (!*abort_flag) fail(2009);
+          if (!*abort_flag) fail(3009);
           break;
         }
         uint8_t* st = stage(c);
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
     bool ok = true;
     for (int c = 0; c < n; ++c) {
       const uint32_t st = smem_u32(stage(c));
-      ok = ok && waitw(&full[c & 1], c >> 1, 2010);
+      ok = ok && waitw(&full[c & 1], c >> 1, 3010);
       // KS
 #pragma unroll 1
       for (int i = 0; i < HN / 16; ++i) {
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       }
       umma_commit_warp(ksdone);
       // E, where O's product of the chunk before has read its planes
-      ok = ok && (c == 0 || waitw(odone, c - 1, 2018));
+      ok = ok && (c == 0 || waitw(odone, c - 1, 3018));
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         take(B_X + i);
@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
       }
       umma_commit_warp(edone);
       // state update, over S planes 0 and 1, which QS has read by now
-      ok = ok && waitw(qdone, c, 2011);
+      ok = ok && waitw(qdone, c, 3011);
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         take(B_W + i);
@@ -463,7 +463,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
     for (int c = 0; c < n; ++c) {
       const uint32_t st = smem_u32(stage(c));
       // QS behind KS (it runs while X is made), once the columns of the last output are read
-      ok = ok && waitw(&full[c & 1], c >> 1, 2012) && waitw(ksdone, c, 2013) && (c == 0 || waitw(oread, c - 1, 2014));
+      ok = ok && waitw(&full[c & 1], c >> 1, 3012) && waitw(ksdone, c, 3013) && (c == 0 || waitw(oread, c - 1, 3014));
       if (ok && elect_one())
 #pragma unroll 1
         for (int kk = 0; kk < KN / 16; ++kk)
@@ -474,7 +474,7 @@ __global__ void __launch_bounds__(512, 1) delta_scan_kernel(const __grid_constan
                          make_idesc_bf16(128, 64, false, false), s != NS - 1 || kk);
       umma_commit_warp(qdone);
       take(B_E);
-      ok = ok && waitw(qread, c, 2015);
+      ok = ok && waitw(qread, c, 3015);
       if (ok && elect_one())
 #pragma unroll 1
         for (int t = 0; t < 4; ++t)
@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
     for (int k = 0; k < n; ++k) {
       const int64_t cc = a.c0 + n - 1 - k;
       const uint8_t* st = stage(k);
-      ok = ok && waitw(&full[k & 1], k >> 1, 2102);
+      ok = ok && waitw(&full[k & 1], k >> 1, 3102);
       const float* eg = reinterpret_cast<const float*>(st + SM::IM + IMG_EG) + 32 * half;
       const float* wb = eg + EG_TO_WB;
       const float el = (eg - 32 * half)[Q - 1];
@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
       };
       save(0);
       // R^T; the last tokens' products reach all columns and go first
-      ok = ok && waitw(ksdone, k, 2103);
+      ok = ok && waitw(ksdone, k, 3103);
 #pragma unroll 1
       for (int i = 1; i >= 0; --i) {
         float x[16], y[16];
@@ -693,7 +693,7 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
       hand_over(B_D);
       save(2);
       // -exp(l) dE
-      ok = ok && waitw(edone, k, 2104);
+      ok = ok && waitw(edone, k, 3104);
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
         float x[16];
@@ -725,7 +725,7 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
           if (j < left) ep[j / 4 * a.P] = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
       }
       // dS^T
-      ok = ok && waitw(dsdone, k, 2105);
+      ok = ok && waitw(dsdone, k, 3105);
 #pragma unroll
       for (int i = 0; i < HN / 16; ++i) {
         float d[16];
@@ -745,7 +745,7 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
       const uint32_t bytes = 2 * NB * TILE + boxes * TILE + IMG;
       for (int k = 0; k < n; ++k) {
         if (k >= 2 && !mbar_wait(&empty[k & 1], ((k >> 1) - 1) & 1, abort_flag)) {
-          if (!*abort_flag) fail(2109);
+          if (!*abort_flag) fail(3109);
           break;
         }
         uint8_t* st = stage(k);
@@ -769,7 +769,7 @@ __global__ void __launch_bounds__(384, 1) delta_back_scan_kernel(const __grid_co
     bool ok = true;
     for (int k = 0; k < n; ++k) {
       const uint32_t st = smem_u32(stage(k));
-      ok = ok && waitw(&full[k & 1], k >> 1, 2110);
+      ok = ok && waitw(&full[k & 1], k >> 1, 3110);
       // dO^T Aq: tokens 16 t .. reach the columns up to 16 t + 15
       take(B_A);
       if (ok && elect_one())
