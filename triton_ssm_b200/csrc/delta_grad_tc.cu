@@ -21,8 +21,9 @@
 // blocks' states to L2 ahead made it slower (311): their own loads queued behind that.
 // K and Q come last, where dE and dO were.
 //
-// Every wait on an mbarrier is bounded; a block that gives up sets the status word and leaves its
-// results unwritten.
+// Every wait on an mbarrier is bounded.  A block that gives up sets the status word and goes on
+// without waiting; it writes no ddt, dbeta and dA_log behind that, and no block of its cluster writes
+// dB and dC, which would hold its part.
 #include "delta.cuh"
 #include "delta_tc.h"
 #include "tcgen05.cuh"
@@ -51,6 +52,13 @@ __device__ __forceinline__ float4 ld_peer(uint32_t addr, uint32_t rank) {   // f
       "{\n\t.reg .b32 p;\n\tmapa.shared::cluster.u32 p, %4, %5;\n\t"
       "ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [p];\n\t}"
       : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr), "r"(rank) : "memory");
+  return v;
+}
+__device__ __forceinline__ int ld_peer_int(uint32_t addr, uint32_t rank) {
+  int v;
+  asm volatile(
+      "{\n\t.reg .b32 p;\n\tmapa.shared::cluster.u32 p, %1, %2;\n\tld.shared::cluster.s32 %0, [p];\n\t}"
+      : "=r"(v) : "r"(addr), "r"(rank) : "memory");
   return v;
 }
 
@@ -459,7 +467,9 @@ __global__ void __launch_bounds__(NT, 2) delta_grad_tc_kernel(const TcGradCall a
   tc_fence_before();
   if (rep > 1) cluster_sync();
   else __syncthreads();
-  const bool ok = !*abort_flag;
+  bool ok = !*abort_flag;
+  if (rep > 1)
+    for (int x = 0; x < rep; ++x) ok &= !ld_peer_int(s + BAR + 5 * 8, x);
   for (int i = (int)rank + rep * warp; i < rows && ok; i += rep * (NT / 32)) {
     const int64_t at = (b * a.L + t0 + i) * sk + (int64_t)g * N + 4 * lane;
 #pragma unroll
