@@ -489,10 +489,15 @@ int tssm_gated_delta_rule(const void* u, const void* A_log, const void* B, const
  * Backward of tssm_gated_delta_rule: from the same inputs, dy (as y), the
  * forward's states and errors, and dh_last (f32 or null), the gradients du,
  * dB, dC (io), dA_log [H], ddt, dbeta [Bt,L,H] and dh0 (f32).  Deterministic.
- * workspace: tssm_gated_delta_rule_bwd_workspace_size bytes, 16-byte aligned.
+ * workspace, 16-byte aligned: tssm_gated_delta_rule_bwd_workspace_size bytes
+ * suffice for either dtype.  The _dtype form gives what this dtype needs when
+ * every tensor is 16-byte aligned: bf16 shapes whose shared key heads are
+ * summed on chip need 8 Bt L H N bytes less.
  */
 int64_t tssm_gated_delta_rule_bwd_workspace_size(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P,
                                                  int64_t N);
+int64_t tssm_gated_delta_rule_bwd_workspace_size_dtype(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P,
+                                                       int64_t N, int dtype);
 int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const void* B, const void* C, const void* dt,
                               const void* beta, const void* dy, const void* states, const void* errors,
                               const void* dh_last, void* du, void* dA_log, void* dB, void* dC, void* ddt,

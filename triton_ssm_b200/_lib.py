@@ -58,6 +58,7 @@ SIGNATURES = {
     "tssm_gated_delta_rule_workspace_size": ([I64] * 6 + [I32], I64),
     "tssm_gated_delta_rule": ([P] * 12 + [I64] * 7 + [F64, I32, P], I32),
     "tssm_gated_delta_rule_bwd_workspace_size": ([I64] * 6, I64),
+    "tssm_gated_delta_rule_bwd_workspace_size_dtype": ([I64] * 6 + [I32], I64),
     "tssm_gated_delta_rule_bwd": ([P] * 18 + [I64] * 7 + [F64, I32, P], I32),
     "tssm_group_norm_workspace_size": ([I64] * 4 + [I32, I32], I64),
     "tssm_group_norm_act": ([P] * 7 + [I64] * 5 + [F64, I32, I32, P], I32),

@@ -765,20 +765,20 @@ int launch_all(BwdArgs a, bool tc, cudaStream_t st) {
   return check_launch("gated_delta_rule_bwd");
 }
 
-// Workspace in floats: dS1 of every chunk, dE, per-head dK and dQ (shared key heads), dA parts,
-// gates, a segment's images.
+// Workspace in floats: dS1 of every chunk, dE, per-head dK and dQ (shared key heads that the gradient
+// kernel does not sum itself), dA parts, gates, a segment's images.
 struct BwdSpace {
   int64_t dstates, derrs, part, da, gates, img, total;
 };
-BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N) {
+BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N, bool tc) {   // tc: the chain is delta_tc.cu's
   auto up = [](int64_t n) { return (n + 3) / 4 * 4; };
   const int64_t nc = cdiv(L, delta::Q);
   BwdSpace s;
   s.dstates = Bt * H * nc * saved_floats(P, N);
   s.derrs = Bt * H * saved_floats(P, L);
-  s.part = H == G ? 0 : up(Bt * L * H * N);
+  s.part = H == G || tc_grad_takes(H, G, N, tc) ? 0 : up(Bt * L * H * N);
   s.da = up(Bt * H * nc);
-  s.img = nc ? Bt * H * segment_chunks(Bt * H, nc) * prep_image_bytes() / 4 : 0;
+  s.img = Bt * nc ? Bt * H * segment_chunks(Bt * H, nc) * prep_image_bytes() / 4 : 0;
   s.gates = Bt * H * nc * (int64_t)(sizeof(Gates) / 4);
   s.total = s.dstates + s.derrs + 2 * s.part + s.da + s.gates + s.img;
   return s;
@@ -791,7 +791,13 @@ BwdSpace space(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P, int64_t N
 extern "C" int64_t tssm_gated_delta_rule_bwd_workspace_size(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P,
                                                             int64_t N) {
   if (Bt <= 0 || L <= 0 || H <= 0 || G <= 0 || P <= 0 || N <= 0) return 0;
-  return tssm::delta::space(Bt, L, H, G, P, N).total * 4;
+  return tssm::delta::space(Bt, L, H, G, P, N, false).total * 4;
+}
+
+extern "C" int64_t tssm_gated_delta_rule_bwd_workspace_size_dtype(int64_t Bt, int64_t L, int64_t H, int64_t G, int64_t P,
+                                                                  int64_t N, int dtype) {
+  if (Bt <= 0 || L <= 0 || H <= 0 || G <= 0 || P <= 0 || N <= 0) return 0;
+  return tssm::delta::space(Bt, L, H, G, P, N, tssm::delta::tc_takes(P, N, dtype)).total * 4;
 }
 
 extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const void* B, const void* C, const void* dt,
@@ -814,7 +820,12 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
   TSSM_REQUIRE(A_log && dA_log && (Bt == 0 || dh0), "gated_delta_rule_bwd: null pointer");
   TSSM_REQUIRE(Bt * L == 0 || (u && B && C && dt && beta && dy && states && errors && du && dB && dC && ddt && dbeta),
                "gated_delta_rule_bwd: null pointer");
-  const int64_t need = tssm_gated_delta_rule_bwd_workspace_size(Bt, L, H, G, P, N);
+  const uintptr_t bases = reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(dy) |
+                          reinterpret_cast<uintptr_t>(dh_last) | reinterpret_cast<uintptr_t>(dh0) |
+                          reinterpret_cast<uintptr_t>(du) | reinterpret_cast<uintptr_t>(dB) | reinterpret_cast<uintptr_t>(dC);
+  const bool tc = tc_takes(P, N, dtype) && (bases & 15u) == 0;
+  const BwdSpace sp = space(Bt, L, H, G, P, N, tc);
+  const int64_t need = sp.total * 4;
   TSSM_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)),
                "gated_delta_rule_bwd: workspace of %lld bytes (16-byte aligned) needed, %lld given", (long long)need,
                (long long)workspace_bytes);
@@ -825,7 +836,6 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
   }
   TSSM_REQUIRE(Bt * L == 0 || (aligned16(states) && aligned16(errors)),
                "gated_delta_rule_bwd: states and errors must be 16-byte aligned");
-  const BwdSpace sp = space(Bt, L, H, G, P, N);
   BwdArgs a{};
   a.u = u; a.B = B; a.C = C; a.dy = dy;
   a.A_log = (const float*)A_log; a.dt = (const float*)dt; a.beta = (const float*)beta;
@@ -837,12 +847,8 @@ extern "C" int tssm_gated_delta_rule_bwd(const void* u, const void* A_log, const
   a.dk_part = sp.part ? a.derrs + sp.derrs : nullptr;
   a.dq_part = sp.part ? a.dk_part + sp.part : nullptr;
   a.da_part = a.derrs + sp.derrs + 2 * sp.part;
-  const uintptr_t bases = reinterpret_cast<uintptr_t>(B) | reinterpret_cast<uintptr_t>(C) | reinterpret_cast<uintptr_t>(dy) |
-                          reinterpret_cast<uintptr_t>(dh_last) | reinterpret_cast<uintptr_t>(dh0) |
-                          reinterpret_cast<uintptr_t>(du) | reinterpret_cast<uintptr_t>(dB) | reinterpret_cast<uintptr_t>(dC);
   a.gates = (Gates*)(a.da_part + sp.da);
   a.img = (uint8_t*)(a.da_part + sp.da + sp.gates);
-  const bool tc = tc_takes(P, N, dtype) && (bases & 15u) == 0;
   a.Bt = Bt; a.L = L; a.H = (int)H; a.G = (int)G; a.P = (int)P; a.N = (int)N;
   a.nc = cdiv(L, delta::Q);
   a.scale = (float)scale;

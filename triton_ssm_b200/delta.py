@@ -126,7 +126,7 @@ def gated_delta_rule_bwd(u, A_log, B, C, dt, beta, dy, saved, scale=1.0, dh_last
     f32 = dict(device=u.device, dtype=torch.float32)
     du, dB, dC, dA_log = torch.empty_like(u), torch.empty_like(B), torch.empty_like(C), torch.empty_like(A_log)
     ddt, dbeta, dh0 = torch.empty_like(dt), torch.empty_like(beta), torch.empty(Bt, H, P, N, **f32)
-    need = int(_lib.load_library().tssm_gated_delta_rule_bwd_workspace_size(Bt, L, H, G, P, N))
+    need = int(_lib.load_library().tssm_gated_delta_rule_bwd_workspace_size_dtype(Bt, L, H, G, P, N, dtype_code(u)))
     ws = torch.empty(need, dtype=torch.uint8, device=u.device) if need else None
     with on_device(dev):
         call("tssm_gated_delta_rule_bwd", addr(u), addr(A_log), addr(B), addr(C), addr(dt), addr(beta), addr(dy), addr(states),
