@@ -63,7 +63,7 @@ def group_norm_act(x, weight, bias, groups, eps=1e-5, act="silu", return_stats=F
     narrow = L == 1 and C // groups <= 128   # needs neither statistics nor workspace
     if return_stats or not narrow:
         mean, rstd = torch.empty(2, Bt, groups, device=x.device, dtype=torch.float32)
-        if L == 0:
+        if L == 0 or C == 0:
             mean.zero_()
             rstd.fill_(eps ** -0.5 if eps else float("inf"))
     if not narrow:
