@@ -93,3 +93,25 @@ def test_key_and_query_gradients_are_rounded_once(cuda_ops, N, P):
         d = (x[:, 1, :, :N // 2].double().cpu() - ref).abs() - half_step(ref)
         bad = d > 2.0 ** -19 * ref.abs()
         assert not bool(bad.any()), "%s: %d of %d values beyond" % (name, int(bad.sum()), d.numel())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,P", [(128, 128), (64, 64), (48, 80)])
+def test_state_under_many_small_writes(cuda_ops, N, P, dtype):
+    """1024 tokens whose writes take 2^-20 of one column of the state each: it is written four times a chunk, half a
+    step off at most each time; e and the decay's product add one step a chunk: 6 steps of 2^-24 a chunk.  So is the
+    state's gradient, with the signs of the backward's."""
+    Bt, L, H, n = 2, 1024, 2, N - 2
+    S = torch.rand(Bt, H, P, N, generator=torch.Generator().manual_seed(6)) + 0.5
+    k = one_hot(Bt, L, H, N, at=n, value=2.0 ** -10).to(dev).to(dtype)
+    u, zero = torch.zeros(Bt, L, H * P, device=dev, dtype=dtype), torch.zeros(Bt, L, H, device=dev)
+    args = (u, torch.zeros(H, device=dev), k, k, zero, torch.ones(Bt, L, H, device=dev))
+    _, h, saved = cuda_ops.gated_delta_rule(*args, h0=S.to(dev), return_state=True, save=True)
+    dh0 = cuda_ops.gated_delta_rule_bwd(*args, u, saved, dh_last=S.to(dev))[6]
+    other = [i for i in range(N) if i != n]
+    ref = S[..., n].double() * (1 - 2.0 ** -20) ** L
+    for x in (h.cpu(), dh0.cpu()):
+        assert torch.equal(x[..., other], S[..., other])
+        d = ((x[..., n].double() - ref) / ref).abs().max().item() * 2.0 ** 24
+        assert d <= 6 * L / 64, "off by %.1f steps of 2^-24" % d

@@ -52,6 +52,12 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// d = a b
+__device__ __forceinline__ void mma_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -107,18 +113,35 @@ __device__ __forceinline__ uint32_t at_a(uint32_t base, int r0, int c0, int lane
   return base + tile_off<RB>(r0 + (lane & 15), c0 + (lane >> 4));
 }
 
-// d0, d1 += sum over planes s + x < NM of a[s] b[x], smallest terms first.
-template <int NA, int NB, int NM>
+// d0, d1 += sum over planes s + x < NM of a[s] b[x], smallest terms first.  APART: they are summed
+// by themselves and then added, rounded, as the tensor core cuts a sum at every step: where a value
+// is added to a state that lasts, a cut is a whole step of the state, always towards 0.
+template <int NA, int NB, int NM, bool APART = false>
 __device__ __forceinline__ void mma_planes(float (&d0)[4], float (&d1)[4], const uint32_t (&a)[NA][4],
                                            const uint32_t (&b)[NB][4]) {
+  float p0[4], p1[4];
+  bool first = true;
 #pragma unroll
   for (int t = NM - 1; t >= 0; --t)
 #pragma unroll
     for (int s = 0; s < NA; ++s) {
       const int x = t - s;
       if (x < 0 || x >= NB) continue;
-      mma(d0, a[s], b[x][0], b[x][1]);
-      mma(d1, a[s], b[x][2], b[x][3]);
+      if (APART && first) {
+        mma_first(p0, a[s], b[x][0], b[x][1]);
+        mma_first(p1, a[s], b[x][2], b[x][3]);
+        first = false;
+        continue;
+      }
+      mma(APART ? p0 : d0, a[s], b[x][0], b[x][1]);
+      mma(APART ? p1 : d1, a[s], b[x][2], b[x][3]);
+    }
+  if constexpr (APART)
+#pragma unroll
+    for (int e = 0; e < 4; e += 2) {
+      const float2 u = fadd2(make_float2(d0[e], d0[e + 1]), make_float2(p0[e], p0[e + 1]));
+      const float2 v = fadd2(make_float2(d1[e], d1[e + 1]), make_float2(p1[e], p1[e + 1]));
+      d0[e] = u.x; d0[e + 1] = u.y; d1[e] = v.x; d1[e + 1] = v.y;
     }
 }
 

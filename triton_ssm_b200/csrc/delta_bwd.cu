@@ -232,10 +232,10 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(cons
         uint32_t w[XS][4];
 #pragma unroll
         for (int z = 0; z < XS; ++z) ldsm4t(w[z], at_a<RB>(s + SM::QQ + z * SM::PLANE, 16 * t, 2 * nn, lane));
-        mma_planes<NS, XS, NS>(S[2 * nn], S[2 * nn + 1], fd, w);
+        mma_planes<NS, XS, NS, true>(S[2 * nn], S[2 * nn + 1], fd, w);
 #pragma unroll
         for (int z = 0; z < XS; ++z) ldsm4t(w[z], at_a<RB>(s + SM::K + z * SM::PLANE, 16 * t, 2 * nn, lane));
-        mma_planes<NS, XS, NS>(S[2 * nn], S[2 * nn + 1], fk, w);
+        mma_planes<NS, XS, NS, true>(S[2 * nn], S[2 * nn + 1], fk, w);
       }
     }
     // dE for the gradient kernel

@@ -304,7 +304,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
         uint32_t w[XS][4];
 #pragma unroll
         for (int z = 0; z < XS; ++z) ldsm4t(w[z], at_a<RB>(s + SM::K + z * SM::PLANE, 16 * t, 2 * nn, lane));
-        mma_planes<NS, XS, NS>(S[2 * nn], S[2 * nn + 1], f, w);
+        mma_planes<NS, XS, NS, true>(S[2 * nn], S[2 * nn + 1], f, w);
       }
     }
   };
