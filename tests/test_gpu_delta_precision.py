@@ -96,6 +96,27 @@ def test_key_and_query_gradients_are_rounded_once(cuda_ops, N, P):
 
 
 @pytest.mark.gpu
+def test_f32_sums_over_the_width_of_the_state(cuda_ops):
+    """Sums of 128 positive terms in f32: y = scale sum_n q_n S_pn, the error u - sum_n k_n S_pn with u = 0, and
+    dC_n = scale sum_p S_pn dy_p (one token, beta = 0).  A piece of 16 terms is cut once at its full size (2 steps
+    of 2^-24) and five times at 2^-8 of it; eight pieces are added with one rounding each, onto 9/16 of the sum on
+    average (4.5 steps); the factors scale and exp(l) round twice and u - x once: 10 steps of 2^-24."""
+    Bt, H, N, P, scale = 4, 2, 128, 128, 0.3
+    g = torch.Generator().manual_seed(5)
+    S, k, q, dy = (torch.rand(*s, generator=g) + 0.5 for s in ((Bt, H, P, N), (Bt, 1, H, N), (Bt, 1, H, N), (Bt, 1, H, P)))
+    zero = torch.zeros(Bt, 1, H, device=dev)
+    args = (torch.zeros(Bt, 1, H * P, device=dev), torch.zeros(H, device=dev), k.to(dev), q.to(dev), zero, zero)
+    y, saved = cuda_ops.gated_delta_rule(*args, scale=scale, h0=S.to(dev), save=True)
+    dC = cuda_ops.gated_delta_rule_bwd(*args, dy.flatten(2).to(dev), saved, scale=scale)[3]
+    S, k, q, dy = (t.double() for t in (S, k[:, 0], q[:, 0], dy[:, 0]))
+    e = saved[1][:, :, 0, :, 0]
+    for name, x, ref in (("y", y.view(Bt, H, P), scale * (S * q[:, :, None]).sum(-1)), ("error", e, -(S * k[:, :, None]).sum(-1)),
+                         ("dC", dC.view(Bt, H, N), scale * (S * dy[..., None]).sum(2))):
+        d = ((x.double().cpu() - ref) / ref).abs().max().item() * 2.0 ** 24
+        assert d <= 10, "%s: off by %.1f steps of 2^-24" % (name, d)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("N,P", [(128, 128), (64, 64), (48, 80)])
 def test_state_under_many_small_writes(cuda_ops, N, P, dtype):

@@ -153,7 +153,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_bwd_chain_kernel(cons
         uint32_t w[XS][4];
 #pragma unroll
         for (int z = 0; z < XS; ++z) ldsm4(w[z], at_b<RB>(s + SM::K + z * SM::PLANE, 16 * np, 2 * kk, lane));
-        mma_planes<NS, XS, NS>(x[2 * np], x[2 * np + 1], f, w);
+        mma_planes<NS, XS, NS, XS == 3>(x[2 * np], x[2 * np + 1], f, w);
       }
     }
 #pragma unroll
@@ -387,15 +387,15 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
       if (qt <= mt) {
 #pragma unroll
         for (int z = 0; z < 3; ++z) ldsm4(w[z], at_b<SQ_RB>(s + SM::E + z * SQ_BYTES, 16 * qt, 2 * kk, lane));
-        mma_planes<XS, 3, 3>(m1[0], m1[1], fo, w);
-        mma_planes<3, 3, 3>(m2[0], m2[1], fe, w);
+        mma_planes<XS, 3, 3, XS == 3>(m1[0], m1[1], fo, w);
+        mma_planes<3, 3, 3, XS == 3>(m2[0], m2[1], fe, w);
       }
 #pragma unroll
       for (int nn = 0; nn < NTQ / 2; ++nn) {
 #pragma unroll
         for (int z = 0; z < 3; ++z) ldsm4t(w[z], at_a<RB>(s + SM::S + z * SM::PLANE, 16 * kk, qt * NTQ + 2 * nn, lane));
-        mma_planes<XS, 3, 3>(dq0[2 * nn], dq0[2 * nn + 1], fo, w);
-        mma_planes<3, 3, 3>(dk0[2 * nn], dk0[2 * nn + 1], fe, w);
+        mma_planes<XS, 3, 3, XS == 3>(dq0[2 * nn], dq0[2 * nn + 1], fo, w);
+        mma_planes<3, 3, 3, XS == 3>(dk0[2 * nn], dk0[2 * nn + 1], fe, w);
       }
     }
     __syncthreads();
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
       for (int nn = 0; nn < NTQ / 2; ++nn) {
 #pragma unroll
         for (int z = 0; z < 3; ++z) ldsm4t(w[z], at_a<RB>(s + SM::S + z * SM::PLANE, 16 * kk, qt * NTQ + 2 * nn, lane));
-        mma_planes<3, 3, 3>(dk1[2 * nn], dk1[2 * nn + 1], fe, w);
+        mma_planes<3, 3, 3, XS == 3>(dk1[2 * nn], dk1[2 * nn + 1], fe, w);
       }
     }
   }
@@ -482,8 +482,8 @@ __global__ void __launch_bounds__(GT, 1) delta_bwd_grad_kernel(const BwdArgs a) 
           ldsm4(fq[z], at_a<RB>(s + SM::QQ + z * SM::PLANE, 16 * mt, 2 * kk, lane));
           ldsm4(w[z], at_b<RB>(s + SM::K + z * SM::PLANE, 16 * qt, 2 * kk, lane));
         }
-        mma_planes<XS, XS, XS>(gk[0], gk[1], fk, w);
-        mma_planes<XS, XS, XS>(gq[0], gq[1], fq, w);
+        mma_planes<XS, XS, XS, XS == 3>(gk[0], gk[1], fk, w);
+        mma_planes<XS, XS, XS, XS == 3>(gq[0], gq[1], fq, w);
       }
     }
     float* Y = reinterpret_cast<float*>(smem + SM::Y);

@@ -148,7 +148,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
         uint32_t w[XS][4];
 #pragma unroll
         for (int z = 0; z < XS; ++z) ldsm4(w[z], at_b<RB>(s + SM::K + z * SM::PLANE, 16 * np, 2 * kk, lane));
-        mma_planes<NS, XS, NS>(x[2 * np], x[2 * np + 1], f, w);
+        mma_planes<NS, XS, NS, XS == 3>(x[2 * np], x[2 * np + 1], f, w);
       }
     }
 #pragma unroll
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__((NCW + 4) * 32, 1) delta_fwd_kernel(const FwdA
         uint32_t w[XS][4];
 #pragma unroll
         for (int z = 0; z < XS; ++z) ldsm4(w[z], at_b<RB>(s + SM::QQ + z * SM::PLANE, 16 * np, 2 * kk, lane));
-        mma_planes<NS, XS, NS>(x[2 * np], x[2 * np + 1], f, w);
+        mma_planes<NS, XS, NS, XS == 3>(x[2 * np], x[2 * np + 1], f, w);
       }
     }
 #pragma unroll
