@@ -11,7 +11,9 @@
 // x is read once.  A thread keeps the same channels from row to row, so its
 // weights (and the backward's dw, db sums) stay in registers.
 // L > 1: a statistics pass and an apply pass.  The batch goes through them in
-// pieces of about L2_BYTES, so that the second pass finds its inputs in L2.
+// pieces of about L2_BYTES, so that the second pass finds most of its inputs in L2
+// (it reads 13 of 61 MB from HBM at 4 x 5000 x 768 f32, and 25 of 134 MB in the
+// backward at 8 x 4096 x 1024 bf16).
 // Variances are merged from per-batch means and squared deviations (Chan's
 // pairwise update), never as E[x^2] - E[x]^2.
 // Measured: 32768 tokens x 4096 bf16 with SiLU take 107 us (5.0 TB/s of x and y);

@@ -97,7 +97,8 @@ class DeltaStream:
     """S independent streams of a gated-delta-rule layer: the state h [S,H,P,N]
     f32 stays in place on the device, ``prefill`` advances every stream by a prompt,
     ``step`` by one token.  Outputs are normalised per token and head (group
-    norm with H groups), then ``act``.
+    norm with H groups), then ``act``.  N at most 128 (256 for streams that only
+    step).
 
     A_log [H]; weight, bias [H*P] (default 1 and 0), f32; scale defaults to
     N ** -0.5.
